@@ -1,0 +1,182 @@
+"""Refusals of the token-sequence operators, and their 64-bit restatements
+against differences: no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import tokens_reference as R
+from uplift_b200 import _native, ops
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _native.load(build_if_missing=True)
+
+
+S2 = ctypes.c_int64 * 2
+
+
+def _attn(lib, **kw):
+    a = dict(q=16, k=16, v=16, out=16, st=S2(128, 64), lse=None, cu=16, B=1, T=4, S=4, Hq=2, Hk=1, D=64, scale=0.125,
+             causal=1, dtype=_native.BF16)
+    a.update(kw)
+    return lib.uplift_tok_attention_forward(
+        a["q"], a["st"], a["k"], a.get("kst", a["st"]), a["v"], a["st"], a["out"], a["st"], a["lse"], a["cu"], a["cu"],
+        None, a["B"], a["T"], a["S"], a["Hq"], a["Hk"], a["D"], a["scale"], a["causal"], a["dtype"], None, 0, None)
+
+
+def _attn_bwd(lib, **kw):
+    a = dict(p=16, st=S2(128, 64), lse=16, delta=16, cu=16, B=1, T=4, S=4, Hq=2, Hk=1, D=64, scale=0.125,
+             dtype=_native.BF16)
+    a.update(kw)
+    rows = []
+    for name in ("dout", "q", "k", "v", "out"):
+        rows += [a.get(name, a["p"]), a["st"]]
+    return lib.uplift_tok_attention_backward(
+        *rows, a["lse"], a["p"], a["st"], a["p"], a["st"], a["p"], a["st"], a["delta"], a["cu"], a["cu"], None, a["B"],
+        a["T"], a["S"], a["Hq"], a["Hk"], a["D"], a["scale"], 1, a["dtype"], None)
+
+
+def _nr(lib, **kw):
+    a = dict(q=16, k=16, st=S2(128, 64), wt=0, cos=16, pos=None, T=4, P=8, Hq=2, Hk=1, D=64, R=64, eps=1e-6, dtype=1)
+    a.update(kw)
+    return lib.uplift_tok_norm_rotate(a["q"], a["st"], a["q"], a["st"], a["k"], a["st"], a["k"], a["st"], None, None,
+                                      a["wt"], a["cos"], a["cos"], a["pos"], 0, a["T"], a["P"], a["Hq"], a["Hk"],
+                                      a["D"], a["R"], a["eps"], 0, a["dtype"], None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=5), "ERR_ARG"), (dict(Hq=3, Hk=2), "ERR_SHAPE"), (dict(Hk=0), "ERR_SHAPE"), (dict(D=0), "ERR_SHAPE"),
+    (dict(D=136), "ERR_SHAPE"), (dict(D=60), "ERR_SHAPE"), (dict(B=-1), "ERR_SHAPE"), (dict(T=-1), "ERR_SHAPE"),
+    (dict(T=1 << 31), "ERR_SHAPE"), (dict(S=1 << 31), "ERR_SHAPE"), (dict(scale=0.0), "ERR_ARG"),
+    (dict(scale=-1.0), "ERR_ARG"), (dict(scale=float("nan")), "ERR_ARG"), (dict(scale=float("inf")), "ERR_ARG"),
+    (dict(q=None), "ERR_ARG"), (dict(out=None), "ERR_ARG"), (dict(cu=None), "ERR_ARG"), (dict(q=8), "ERR_LAYOUT"),
+    (dict(st=S2(132, 64)), "ERR_LAYOUT"), (dict(st=S2(128, 4)), "ERR_LAYOUT"), (dict(st=S2(0, 64)), "ERR_LAYOUT"),
+    (dict(st=None), "ERR_ARG"),
+])
+def test_attention_entry_refuses(lib, kw, code):
+    assert _attn(lib, **kw) == getattr(_native, code)
+    assert lib.uplift_la_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=-1), "ERR_ARG"), (dict(lse=None), "ERR_ARG"), (dict(delta=None), "ERR_ARG"),
+    (dict(dout=None), "ERR_ARG"), (dict(out=None), "ERR_ARG"), (dict(v=24), "ERR_LAYOUT"),
+    (dict(D=129), "ERR_SHAPE"), (dict(Hq=5, Hk=2), "ERR_SHAPE"), (dict(cu=None), "ERR_ARG"),
+])
+def test_attention_backward_entry_refuses(lib, kw, code):
+    assert _attn_bwd(lib, **kw) == getattr(_native, code)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=9), "ERR_ARG"), (dict(wt=9), "ERR_ARG"), (dict(D=257), "ERR_SHAPE"), (dict(D=0), "ERR_SHAPE"),
+    (dict(R=63), "ERR_SHAPE"), (dict(R=66), "ERR_SHAPE"), (dict(R=-2), "ERR_SHAPE"), (dict(P=3), "ERR_SHAPE"),
+    (dict(Hq=0), "ERR_SHAPE"), (dict(T=-1), "ERR_SHAPE"), (dict(eps=-1.0), "ERR_ARG"),
+    (dict(eps=float("nan")), "ERR_ARG"), (dict(q=None), "ERR_ARG"), (dict(cos=None), "ERR_ARG"),
+    (dict(st=None), "ERR_ARG"),
+])
+def test_norm_rotate_entry_refuses(lib, kw, code):
+    assert _nr(lib, **kw) == getattr(_native, code)
+
+
+def test_empty_calls_touch_no_device(lib):
+    assert _attn(lib, T=0) == _native.OK
+    assert _attn_bwd(lib, T=0, S=0) == _native.OK
+    assert _nr(lib, T=0) == _native.OK
+    assert lib.uplift_tok_norm_rotate_partial_floats(64) > 0
+
+
+def _qkv(T=4, S=4, Hq=2, Hk=1, D=16, dt=torch.float32):
+    return torch.randn(T, Hq, D).to(dt), torch.randn(S, Hk, D).to(dt), torch.randn(S, Hk, D).to(dt)
+
+
+def _cu(*n):
+    return torch.tensor(n, dtype=torch.int32)
+
+
+def test_packed_attention_refuses():
+    q, k, v = _qkv()
+    cu = _cu(0, 4)
+    for bad in (dict(q=q.double()), dict(k=k.half()), dict(v=v[:3]), dict(q=q[..., :8]), dict(q=q[0]),
+                dict(cu_q=cu.long()), dict(cu_k=_cu(0, 2, 4)), dict(cu_q=cu[None]), dict(used_k=_cu(1, 2)),
+                dict(used_k=torch.tensor([4.0])), dict(scale=0.0), dict(scale=float("inf")),
+                dict(q=torch.randn(4, 3, 16), k=torch.randn(4, 2, 16), v=torch.randn(4, 2, 16)),
+                dict(q=torch.randn(4, 2, 136), k=torch.randn(4, 1, 136), v=torch.randn(4, 1, 136)),
+                dict(q=q.bfloat16()[..., :12], k=k.bfloat16()[..., :12], v=v.bfloat16()[..., :12]),
+                dict(cu_q=_cu(), cu_k=_cu()), dict(k=k[:, :0], v=v[:, :0])):
+        args = dict(q=q, k=k, v=v, cu_q=cu, cu_k=cu)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            ops.packed_attention(**args)
+    with pytest.raises(ValueError, match="pass cu_k"):
+        ops.packed_attention(q, k[:3], v[:3], cu)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.packed_attention(q, k, v, cu)
+
+
+def test_norm_rotate_refuses():
+    q, k, _ = _qkv()
+    cos = torch.ones(8, 8)
+    w = torch.ones(16)
+    ok = dict(q=q, k=k, q_weight=w, k_weight=w, cos=cos, sin=cos)
+    for bad in (dict(q=q.double()), dict(k=k[:3]), dict(k=k[..., :8]), dict(q_weight=w[:8]), dict(q_weight=w.double()),
+                dict(k_weight=w.half()), dict(cos=cos.half()), dict(sin=cos[:4]), dict(cos=cos[:3], sin=cos[:3]),
+                dict(cos=torch.ones(8, 9), sin=torch.ones(8, 9)), dict(positions=torch.zeros(3, dtype=torch.int32)),
+                dict(positions=torch.zeros(4)), dict(cos=cos.clone().requires_grad_()),
+                dict(q=torch.randn(4, 1, 264), k=torch.randn(4, 1, 264), q_weight=None, k_weight=None)):
+        args = dict(ok)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            ops.norm_rotate(**args)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.norm_rotate(**ok)
+
+
+def test_operators_are_traced_under_fake_tensors():
+    """The custom ops have fake kernels with the outputs' shapes and types."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q, k, v = _qkv(dt=torch.bfloat16)
+        out, lse = torch.ops.uplift_b200.packed_attention(q, k, v, _cu(0, 4), _cu(0, 4), None, True, 0.25)
+        assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (2, 4) and lse.dtype == torch.float32
+        a, b = torch.ops.uplift_b200.norm_rotate(q, k, None, None, torch.ones(4, 8), torch.ones(4, 8), None, 1e-6, False)
+        assert a.shape == q.shape and b.shape == k.shape
+
+
+# ---------------------------------------- the restatements against differences
+def _difference(f, x, d, h=1e-5):
+    return (f(x + h * d) - f(x - h * d)) / (2 * h)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_reference_attention_gradients_are_differences(causal):
+    torch.manual_seed(0)
+    q, k, v = (t.double() for t in _qkv(T=7, S=9, Hq=4, Hk=2, D=8))
+    cu_q, cu_k, used = _cu(0, 5, 7), _cu(0, 3, 9), torch.tensor([3, 5], dtype=torch.int32)
+    g = torch.randn_like(q)
+    r = R.attention(q, k, v, cu_q, cu_k, used, causal, 0.3, g)
+    for n, i in (("dq", 0), ("dk", 1), ("dv", 2)):
+        d = torch.randn_like((q, k, v)[i])
+
+        def f(x):
+            args = [q, k, v]
+            args[i] = x
+            return (R.attention(*args, cu_q, cu_k, used, causal, 0.3)["out"] * g).sum()
+
+        # central differences with h = 1e-5: h^2 times third derivatives (order 1 here), 1e-16 / h of cancellation
+        assert abs(_difference(f, (q, k, v)[i], d) - (r[n] * d).sum()) < 1e-8
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_reference_norm_rotate_gradients_are_differences(interleaved):
+    torch.manual_seed(0)
+    x, w, g = torch.randn(5, 2, 8).double(), torch.randn(8).double(), torch.randn(5, 2, 8).double()
+    ang = torch.randn(6, 3).double()
+    pos = torch.tensor([3, -1, 0, 5, 2])
+    args = (ang.cos(), ang.sin(), pos, 1e-3, interleaved)
+    _, dx, dw = R.norm_rotate(x, w, *args, g=g)
+    d = torch.randn_like(x)
+    assert abs(_difference(lambda t: (R.norm_rotate(t, w, *args) * g).sum(), x, d) - (dx * d).sum()) < 1e-8
+    e = torch.randn_like(w)
+    assert abs(_difference(lambda t: (R.norm_rotate(x, t, *args) * g).sum(), w, e) - (dw * e).sum()) < 1e-8

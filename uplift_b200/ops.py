@@ -8,6 +8,9 @@ registered as torch custom ops (``torch.ops.uplift_b200.*``) with fake
 implementations, so torch.compile traces them without a graph break (the
 reference's Triton module takes one, uplift/kernels/triton_attender.py:335).
 
+`norm_rotate` and `packed_attention`, the operators on token sequences, live
+in tokens.py and are offered here too.
+
 Inputs are accepted in any layout; the kernels read channels_last (NHWC)
 storage, so other layouts are converted first.  The output is channels_last
 in the value dtype.
@@ -19,6 +22,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _native
+from .tokens import norm_rotate, packed_attention  # noqa: F401  (include/uplift_tokens.h)
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 

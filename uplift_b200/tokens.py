@@ -1,0 +1,426 @@
+"""Token-sequence operators over the C ABI of include/uplift_tokens.h: the
+attention of transformer tokens and the per-head norm with position rotation
+that feeds it (sm_100a kernels in uplift_b200/csrc/tok_*.cu).
+
+They stand beside the Local Attender (`ops.local_attender`, a softmax over K
+neighbours of a pixel) and the fast mode's layer norm (`glue.layernorm_act_`):
+
+  norm_rotate        RMS norm of every query and key head and the rotation of
+                     its channel pairs by position, in one pass
+  packed_attention   softmax attention over packed sequences of different
+                     lengths (prompts, images, or one new token per sequence
+                     on a long history), grouped heads, causal or not
+
+Tensors are [rows, heads, D] on an sm_100 device in float32, bfloat16 or
+float16; views into a fused projection output are read in place.  Both are
+differentiable (gradients are deterministic) and registered as torch custom
+ops, so torch.compile traces them.  Launches go to the current stream of the
+tensors' device; workspaces come from torch's allocator, so calls on several
+streams and in captured graphs share nothing.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _native
+
+_DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+_I64_2 = ctypes.c_int64 * 2
+
+
+def _check(what: str, named) -> torch.device:
+    """The common device of (name, tensor) pairs; raises where they differ or are not on CUDA."""
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"uplift_b200 {what} runs on CUDA (sm_100) tensors only; {name} is a "
+                               f"{t.device} tensor (there is no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices: {dev} vs {t.device} ({name})")
+    return dev
+
+
+def _check_rows(what: str, named) -> None:
+    first = named[0][1]
+    if first.dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported dtype {first.dtype} (float32, bfloat16, float16)")
+    for name, t in named:
+        if t.dim() != 3:
+            raise ValueError(f"{what}: {name} must be [rows, heads, D], got {tuple(t.shape)}")
+        if t.dtype != first.dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}, {named[0][0]} is {first.dtype}")
+        if t.shape[2] != first.shape[2]:
+            raise ValueError(f"{what}: {name} has head dimension {t.shape[2]}, {named[0][0]} has {first.shape[2]}")
+        if t.shape[1] < 1 or t.shape[2] < 1:
+            raise ValueError(f"{what}: {name} has no heads or channels: {tuple(t.shape)}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy where the kernels cannot read it in place: channel stride 1 and, in 16 bits,
+    16-byte aligned rows."""
+    st, hd = t.stride(), t.shape
+    ok = st[2] == 1 or hd[2] == 1
+    if ok and t.element_size() == 2:
+        ok = (t.data_ptr() & 15) == 0 and (hd[0] <= 1 or (st[0] > 0 and st[0] % 8 == 0)) and (
+            hd[1] <= 1 or (st[1] > 0 and st[1] % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _st(t: torch.Tensor):
+    s = t.stride()
+    return _I64_2(s[0], s[1])
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------- norm_rotate
+def _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions):
+    what = "norm_rotate"
+    _check_rows(what, (("q", q), ("k", k)))
+    T, _, D = q.shape
+    if k.shape[0] != T:
+        raise ValueError(f"{what}: q has {T} tokens, k has {k.shape[0]}")
+    if D > 256:
+        raise ValueError(f"{what}: head dimension {D} is above 256")
+    ws = [w for w in (q_weight, k_weight) if w is not None]
+    for w in ws:
+        if tuple(w.shape) != (D,) or w.dtype not in _DTYPES:
+            raise ValueError(f"{what}: weights must be [{D}] in float32, bfloat16 or float16, got "
+                             f"{tuple(w.shape)} {w.dtype}")
+        if w.dtype != ws[0].dtype:
+            raise ValueError(f"{what}: q_weight is {ws[0].dtype}, k_weight is {w.dtype}")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"{what}: cos and sin must be float32 [P, R / 2] tables of one shape, got "
+                         f"{tuple(cos.shape)} {cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
+    if 2 * cos.shape[1] > D:
+        raise ValueError(f"{what}: tables rotate {2 * cos.shape[1]} channels, heads have {D}")
+    if positions is None:
+        if cos.shape[1] > 0 and cos.shape[0] < T:
+            raise ValueError(f"{what}: {cos.shape[0]} table rows for {T} tokens without positions")
+    elif tuple(positions.shape) != (T,) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: positions must be int32 or int64 [{T}], got {tuple(positions.shape)} "
+                         f"{positions.dtype}")
+    dev = _check(what, (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos),
+                        ("sin", sin), ("positions", positions)))
+    return dev, (_DTYPES[ws[0].dtype] if ws else _native.F32)
+
+
+def _c(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
+def norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
+    """Launch uplift_tok_norm_rotate (no autograd)."""
+    dev, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    q, k = _rows(q), _rows(k)
+    qw, kw, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
+    qo = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    ko = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        rc = _native.load().uplift_tok_norm_rotate(
+            q.data_ptr(), _st(q), qo.data_ptr(), _st(qo), k.data_ptr(), _st(k), ko.data_ptr(), _st(ko),
+            _ptr(qw), _ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), _ptr(positions),
+            int(positions is not None and positions.dtype == torch.int64), T, cos.shape[0], Hq, Hk, D,
+            2 * cos.shape[1], float(eps), int(bool(interleaved)), _DTYPES[q.dtype],
+            torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "uplift_tok_norm_rotate")
+    return qo, ko
+
+
+def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
+                             interleaved=False, need_weights=True):
+    """Launch uplift_tok_norm_rotate_backward: (dq, dk, dweights [2, D] fp32; empty when not needed)."""
+    dev, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    gq, gk, q, k = _rows(gq.to(q.dtype)), _rows(gk.to(q.dtype)), _rows(q), _rows(k)
+    qw, kw, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
+    lib = _native.load()
+    dq = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
+    dw = torch.empty((2, D) if need_weights else (0,), dtype=torch.float32, device=dev)
+    partial = torch.empty(lib.uplift_tok_norm_rotate_partial_floats(D) if need_weights else 0,
+                          dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.uplift_tok_norm_rotate_backward(
+            gq.data_ptr(), _st(gq), gk.data_ptr(), _st(gk), q.data_ptr(), _st(q), k.data_ptr(), _st(k),
+            dq.data_ptr(), _st(dq), dk.data_ptr(), _st(dk), dw.data_ptr() if need_weights else None, _ptr(qw),
+            _ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), _ptr(positions),
+            int(positions is not None and positions.dtype == torch.int64),
+            partial.data_ptr() if need_weights else None, T, cos.shape[0], Hq, Hk, D, 2 * cos.shape[1], float(eps),
+            int(bool(interleaved)), _DTYPES[q.dtype], torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "uplift_tok_norm_rotate_backward")
+    return dq, dk, dw
+
+
+def _norm_rotate_grads(ctx_needs, dq, dk, dw, q_weight, k_weight):
+    nq, nk, nqw, nkw = ctx_needs
+    return (dq if nq else None, dk if nk else None, dw[0].to(q_weight.dtype) if nqw else None,
+            dw[1].to(k_weight.dtype) if nkw else None)
+
+
+class _NormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+        needs = ctx.needs_input_grad[:4]
+        dq, dk, dw = norm_rotate_backward_raw(gq, gk, q, k, qw, kw, cos, sin, positions, ctx.eps, ctx.interleaved,
+                                              need_weights=needs[2] or needs[3])
+        return (*_norm_rotate_grads(needs, dq, dk, dw, qw, kw), None, None, None, None, None)
+
+
+@torch.library.custom_op("uplift_b200::norm_rotate", mutates_args=())
+def _norm_rotate_op(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                    k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+                    positions: Optional[torch.Tensor], eps: float,
+                    interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+@_norm_rotate_op.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("uplift_b200::norm_rotate_backward", mutates_args=())
+def _norm_rotate_backward_op(gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                             q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                             cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor], eps: float,
+                             interleaved: bool, need_weights: bool
+                             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved,
+                                    need_weights)
+
+
+@_norm_rotate_backward_op.register_fake
+def _(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, need_weights):
+    return (q.new_empty(q.shape), k.new_empty(k.shape),
+            q.new_empty((2, q.shape[2]) if need_weights else (0,), dtype=torch.float32))
+
+
+def _nr_setup_context(ctx, inputs, output):
+    q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved = inputs
+    ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+    ctx.eps, ctx.interleaved = eps, interleaved
+
+
+def _nr_backward(ctx, gq, gk):
+    q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+    needs = ctx.needs_input_grad[:4]
+    dq, dk, dw = torch.ops.uplift_b200.norm_rotate_backward(gq, gk, q, k, qw, kw, cos, sin, positions, ctx.eps,
+                                                            ctx.interleaved, needs[2] or needs[3])
+    return (*_norm_rotate_grads(needs, dq, dk, dw, qw, kw), None, None, None, None, None)
+
+
+torch.library.register_autograd("uplift_b200::norm_rotate", _nr_backward, setup_context=_nr_setup_context)
+
+
+def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
+    """RMS norm of query and key heads and position rotation, in one pass.
+
+    q [T, Hq, D] and k [T, Hk, D] -> new contiguous tensors of these shapes:
+
+        y = x / sqrt(mean(x**2) + eps) * weight                   (per token and head)
+        (a, b) -> (a cos - b sin, b cos + a sin)                  (per pair of channels)
+
+    q_weight, k_weight: [D], or None for ones.  cos, sin: float32 [P, R / 2]
+    tables (R <= D; channels from R on are not rotated); token t uses row
+    positions[t] (int32 or int64), or row t without positions.  A negative
+    position leaves the token unrotated (class tokens); one beyond the table
+    makes its rotated channels NaN.  Pairs are (i, i + R/2), or (2i, 2i + 1)
+    when interleaved.  Arithmetic in fp32, one rounding per result.
+    Differentiable in q, k and the weights; the tables are constants.
+    """
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("norm_rotate: cos and sin are constants and must not require gradients")
+    eps, interleaved = float(eps), bool(interleaved)
+    if torch.compiler.is_compiling():
+        return torch.ops.uplift_b200.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _NormRotate.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+# -------------------------------------------------------- packed_attention
+def _starts(what: str, name: str, t: torch.Tensor, entries: Optional[int] = None) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() < 1 if entries is None else t.numel() != entries):
+        raise ValueError(f"{what}: {name} must be an int32 vector" +
+                         ("" if entries is None else f" of {entries} entries") +
+                         f", got {tuple(t.shape)} {t.dtype}")
+
+
+def _attention_args(q, k, v, cu_q, cu_k, used_k, scale):
+    what = "packed_attention"
+    _check_rows(what, (("q", q), ("k", k), ("v", v)))
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: k is {tuple(k.shape)}, v is {tuple(v.shape)}")
+    if q.shape[1] % k.shape[1] != 0:
+        raise ValueError(f"{what}: {q.shape[1]} query heads are not a multiple of {k.shape[1]} key heads")
+    D = q.shape[2]
+    if D > 128 or (q.element_size() == 2 and D % 8 != 0):
+        raise ValueError(f"{what}: head dimension {D} (at most 128; a multiple of 8 in 16 bits)")
+    _starts(what, "cu_q", cu_q)
+    _starts(what, "cu_k", cu_k, cu_q.numel())
+    if used_k is not None:
+        _starts(what, "used_k", used_k, cu_q.numel() - 1)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
+    return _check(what, (("q", q), ("k", k), ("v", v), ("cu_q", cu_q), ("cu_k", cu_k), ("used_k", used_k)))
+
+
+def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=None, need_lse=False):
+    """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, empty when not needed)."""
+    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    dev = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
+    (T, Hq, D), (S, Hk, _) = q.shape, k.shape
+    B = cu_q.numel() - 1
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    cu_q, cu_k, used_k = _c(cu_q), _c(cu_k), _c(used_k)
+    dt = _DTYPES[q.dtype]
+    lib = _native.load()
+    _native.host_status.raise_if_set()
+    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((Hq, T) if need_lse else (0,), dtype=torch.float32, device=dev)
+    nbytes = lib.uplift_tok_attention_workspace(B, T, S, Hq, Hk, D, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+    with torch.cuda.device(dev):
+        rc = lib.uplift_tok_attention_forward(
+            q.data_ptr(), _st(q), k.data_ptr(), _st(k), v.data_ptr(), _st(v), out.data_ptr(), _st(out),
+            lse.data_ptr() if need_lse else None, cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), B, T, S, Hq, Hk, D,
+            scale, int(bool(causal)), dt, _ptr(ws), nbytes, torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "uplift_tok_attention_forward")
+    return out, lse
+
+
+def packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k=None, causal=True, scale=None):
+    """Launch uplift_tok_attention_backward: (dq, dk, dv)."""
+    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    dev = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
+    (T, Hq, D), (S, Hk, _) = q.shape, k.shape
+    g, q, k, v, out = _rows(g.to(q.dtype)), _rows(q), _rows(k), _rows(v), _rows(out)
+    cu_q, cu_k, used_k, lse = _c(cu_q), _c(cu_k), _c(used_k), lse.contiguous()
+    dq = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((S, Hk, D), dtype=q.dtype, device=dev)
+    dv = torch.empty((S, Hk, D), dtype=q.dtype, device=dev)
+    delta = torch.empty((Hq, T), dtype=torch.float32, device=dev)
+    lib = _native.load()
+    _native.host_status.raise_if_set()
+    with torch.cuda.device(dev):
+        rc = lib.uplift_tok_attention_backward(
+            g.data_ptr(), _st(g), q.data_ptr(), _st(q), k.data_ptr(), _st(k), v.data_ptr(), _st(v),
+            out.data_ptr(), _st(out), lse.data_ptr(), dq.data_ptr(), _st(dq), dk.data_ptr(), _st(dk),
+            dv.data_ptr(), _st(dv), delta.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k),
+            cu_q.numel() - 1, T, S, Hq, Hk, D, scale, int(bool(causal)), _DTYPES[q.dtype],
+            torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "uplift_tok_attention_backward")
+    return dq, dk, dv
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, used_k, causal, scale):
+        out, lse = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, used_k)
+        ctx.causal, ctx.scale = causal, scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
+        grads = packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal, ctx.scale)
+        return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+
+
+@torch.library.custom_op("uplift_b200::packed_attention", mutates_args=())
+def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                         used_k: Optional[torch.Tensor], causal: bool,
+                         scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True)
+
+
+@_packed_attention_op.register_fake
+def _(q, k, v, cu_q, cu_k, used_k, causal, scale):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op("uplift_b200::packed_attention_backward", mutates_args=())
+def _packed_attention_backward_op(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                                  out: torch.Tensor, lse: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                                  used_k: Optional[torch.Tensor], causal: bool,
+                                  scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale)
+
+
+@_packed_attention_backward_op.register_fake
+def _(g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+def _pa_setup_context(ctx, inputs, output):
+    q, k, v, cu_q, cu_k, used_k, causal, scale = inputs
+    out, lse = output
+    ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, used_k)
+    ctx.causal, ctx.scale = causal, scale
+
+
+def _pa_backward(ctx, g, _):
+    q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
+    grads = torch.ops.uplift_b200.packed_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal,
+                                                            ctx.scale)
+    return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+
+
+torch.library.register_autograd("uplift_b200::packed_attention", _pa_backward, setup_context=_pa_setup_context)
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=None, return_lse=False):
+    """Softmax attention over packed sequences with grouped heads.
+
+    q [T, Hq, D], k and v [S, Hk, D] (Hq a multiple of Hk; query head h reads
+    key head h // (Hq // Hk)) -> out [T, Hq, D], contiguous.
+
+    cu_q, cu_k: int32 vectors of B + 1 ascending row numbers on the device;
+    sequence b owns the rows cu[b] .. cu[b + 1] - 1 (cu_k defaults to cu_q).
+    used_k: int32 [B], how many rows of each key segment hold keys (a cache
+    with room to grow); all of them by default.  A causal query i of n_q sees
+    the keys j <= i + n_k - n_q, so the last query sees all n_k.  scale
+    defaults to D ** -0.5.  Queries that see no key, and rows of no sequence,
+    get zeros (lse -inf) and gradients zero.
+
+    With return_lse also returns log(sum_j exp(scale q_i . k_j)), fp32
+    [Hq, T], a constant for autograd.  Differentiable in q, k, v.
+    """
+    if cu_k is None:
+        if q.shape[0] != k.shape[0]:
+            raise ValueError(f"packed_attention: q has {q.shape[0]} rows and k has {k.shape[0]}: pass cu_k")
+        cu_k = cu_q
+    scale, causal = (float(scale) if scale is not None else q.shape[-1] ** -0.5), bool(causal)
+    if torch.compiler.is_compiling():
+        out, lse = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale)
+        lse = lse.detach()
+    elif torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, used_k, causal, scale)
+    else:
+        out, lse = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=return_lse)
+    return (out, lse) if return_lse else out
