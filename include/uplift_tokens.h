@@ -95,8 +95,9 @@ int uplift_tok_norm_rotate_backward(const void* dq_out, const int64_t dq_out_str
  *   scale  positive and finite
  *   workspace: uplift_tok_attention_workspace(...) bytes, 16-byte aligned
  *             (may be 0 / NULL)
- * bf16 / fp16: D a multiple of 8, pointers 16-byte aligned and strides
- * multiples of 8 elements (UPLIFT_LA_ERR_LAYOUT otherwise).
+ * bf16 / fp16: D a multiple of 8; pointers 16-byte aligned, strides
+ * multiples of 8 elements and row strides multiples of the head stride
+ * (UPLIFT_LA_ERR_LAYOUT otherwise).
  */
 int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int Hk, int D, int dtype);
 int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], const void* k,

@@ -93,6 +93,9 @@ bool dl_tc_eligible(const DlArgs& a, const char** why);
 int dl_tc_launch(const DlArgs& a, cudaStream_t stream);
 int dl_device_status(bool clear);
 
+// Status word of the packed-sequence attention kernels (tok_attn.cu).
+int tok_device_status(bool clear);
+
 // Record an error message for uplift_la_last_error().
 int fail(int code, const char* fmt, ...);
 

@@ -445,8 +445,9 @@ int uplift_la_device_status(int clear) {
   const int b = ula::tcw_device_status(clear != 0);
   const int c = ula::dv_device_status(clear != 0);
   const int d = ula::dl_device_status(clear != 0);
-  if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
-  return a != 0 ? a : (b != 0 ? b : (c != 0 ? c : d));
+  const int e = ula::tok_device_status(clear != 0);
+  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
+  return a != 0 ? a : (b != 0 ? b : (c != 0 ? c : (d != 0 ? d : e)));
 }
 
 int uplift_la_set_host_status_word(unsigned int* word) {

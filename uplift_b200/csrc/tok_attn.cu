@@ -36,6 +36,8 @@ int check_rows(const char* what, const char* name, const Rows& r, int64_t rows, 
     return fail(UPLIFT_LA_ERR_LAYOUT, "%s: %s is not 16-byte aligned", what, name);
   if ((rows > 1 && (r.t % 8 != 0 || r.t <= 0)) || (heads > 1 && (r.h % 8 != 0 || r.h <= 0)))
     return fail(UPLIFT_LA_ERR_LAYOUT, "%s: the strides of %s must be positive multiples of 8 elements", what, name);
+  if (rows > 1 && heads > 1 && r.t % r.h != 0)  // as tensor maps want it
+    return fail(UPLIFT_LA_ERR_LAYOUT, "%s: the row stride of %s must be a multiple of its head stride", what, name);
   return UPLIFT_LA_OK;
 }
 
@@ -50,6 +52,9 @@ Rows rows_of(const void* p, const int64_t* st, int64_t rows, int heads, int D) {
 
 }  // namespace
 }  // namespace tok
+
+int tok_device_status(bool clear) { return tok::attn_fwd_device_status(clear); }
+
 }  // namespace ula
 
 extern "C" {
@@ -85,7 +90,8 @@ int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], cons
   a.lse = lse;
   a.pk = Packing{cu_q, cu_k, used_k, B, (int)T, (int)S, causal != 0};
   a.Hq = Hq; a.Hk = Hk; a.D = D; a.scale = scale; a.dtype = dtype;
-  return attn_simt_forward(a, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == UPLIFT_LA_F32 ? attn_simt_forward(a, s) : attn_tc_forward(a, s);
 }
 
 int uplift_tok_attention_backward(const void* dout, const int64_t dout_strides[2], const void* q,

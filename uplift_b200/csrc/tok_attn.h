@@ -26,6 +26,10 @@ struct AttnArgs {
   float* delta;  // [Hq][T]
 };
 
+// bf16 / fp16 attention on the tensor cores (tok_attn_fwd.cu).
+int attn_tc_forward(const AttnArgs& a, cudaStream_t s);
+int attn_fwd_device_status(bool clear);
+
 // fp32 attention on CUDA cores (tok_attn_simt.cu).
 int attn_simt_forward(const AttnArgs& a, cudaStream_t s);
 int attn_simt_backward(const AttnArgs& a, cudaStream_t s);

@@ -1,0 +1,682 @@
+// Attention over packed sequences on the tensor cores of B200 (sm_100a),
+// bf16 / fp16, D <= 128.
+//
+// An item is 256 query rows of one head of one sequence (two tiles of
+// M = 128), which walks the key tiles (128 keys) that its rows see:
+//
+//   S_t[128 x 128] = Q_t . K_j^T                    (tcgen05, fp32 in TMEM)
+//   m = max(m, rowmax S), P = exp2((S - m) scale log2 e), l += rowsum P
+//   O_t[128 x D]  += P . V_j                        (P from TMEM, V MN-major)
+//
+// with the running maximum m and sum l in the registers of the thread that
+// owns the row (TMEM lane = query row), so that one pass over K and V
+// suffices and S never leaves the SM.  O stays in TMEM for the whole item; a
+// row is rescaled by exp2((m_old - m_new) scale log2 e) only when its maximum
+// has grown by more than 2^8 (weights up to 2^8 lose nothing in fp32 and bf16
+// or fp16, and the final division by l takes any common factor out), which
+// after the first tiles hardly ever happens.
+//
+// Roles (384 threads, one persistent CTA per SM): warps 0-3 and 4-7 one
+// softmax group per tile (a thread per row); warp 8 looks the items up and
+// issues the TMA loads; warp 9 issues the MMAs.  The two tiles share each
+// K / V tile in shared memory and alternate: while one group computes its
+// exponentials the tensor cores work for the other.  P is rounded to the
+// storage type in place of S (half of its columns) -- the tensor cores
+// multiply 16-bit operands; the sum l uses the unrounded weights.
+//
+// Scores that a row does not see -- behind its sequence's end, where a tile
+// holds rows of the next sequence, or behind the causal edge -- are set to
+// -inf before the maximum.  P = 0 there, which an infinity or NaN in the same
+// V row would turn into NaN: in the tiles that some row sees only in part the
+// groups look V through, replace such values by zero and add them at the end
+// to the rows that see them.
+//
+// Every mbarrier wait is bounded; on expiry the CTA records the role in this
+// kernel's status word (and the registered host word), drains and exits.
+
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "tok_attn_tc.h"
+
+namespace ula {
+
+__device__ unsigned int g_tok_fwd_status;
+
+namespace tok {
+namespace fwd {
+
+constexpr int kM = 128;            // query rows of a tile
+constexpr int kItemRows = 2 * kM;
+constexpr int kN = 128;            // keys of a tile
+constexpr int kChunkBytes = 128 * 128;  // 128 rows x 64 channels
+constexpr int kThreads = 384;
+constexpr int kTmemCols = 512;
+constexpr int kItems = 2;          // ring of looked-up items
+constexpr uint64_t kTimeoutNs = 2000000000ull;
+// Registers of the softmax groups and of the other warps after the split:
+// 2 x 128 x 208 + 128 x 88 = 384 x 168, what the CTA is launched with.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.f;    // log2 of the growth of the maximum that O is rescaled for
+
+template <int DP>
+struct Cfg {
+  static constexpr int kChunks = DP / 64;
+  static constexpr int kQBytes = kChunks * kChunkBytes;  // one query tile
+  static constexpr int kSlotBytes = kChunks * kChunkBytes;
+  static constexpr int kSlots = DP == 128 ? 4 : 8;       // K and V tiles in turn
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffKV = 2 * kQBytes;
+  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;
+  static constexpr int kStageBytes = 32 * 128;           // a warp's 32 rows x 64 channels
+  static constexpr int kOffBar = kOffStage + 8 * kStageBytes;
+  static constexpr int kNumBars = 2 + 2 * kSlots + 3 * 2 + 2 * kItems + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kOffItems = kOffMisc + 32;
+  static constexpr int kSmem = kOffItems + kItems * 48 + 1024;  // + base alignment slack
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct Item {
+  int row;        // first query row in the tensor
+  int n;          // its rows, 1..256; 0: no more items
+  int h;          // query head
+  int k0;         // first key row in the tensor
+  int nk;         // keys of the sequence
+  int see;        // keys that the first row sees (may be negative; each next row sees one more when causal)
+  int nt[2];      // key tiles of each query tile
+};
+
+struct Params {
+  CUtensorMap qmap, kmap, vmap;  // boxes {64, 1, 128, 1}
+  CUtensorMap omap;              // box {64, 1, 32, 1}
+  Rows v, out;
+  float* lse;
+  Packing pk;
+  int Hq, group, D;
+  float scale;
+  uint64_t timeout_ns;
+  unsigned int* host_status;
+};
+
+// Bounded wait, inline: a kernel that splits its registers between warps
+// cannot call functions.
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
+                                          const WaitLimit& limit) {
+  return mbar_wait_inline(b, parity, abort_flag, where, limit, &g_tok_fwd_status);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_probe(uint32_t acc, uint32_t x);  // acc stays 0 in both halves iff x is finite
+template <>
+__device__ __forceinline__ uint32_t nonfinite_probe<__nv_bfloat16>(uint32_t acc, uint32_t x) {
+  __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&x), __nv_bfloat162(__nv_bfloat16(0.f), __nv_bfloat16(0.f)),
+                             *reinterpret_cast<__nv_bfloat162*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t nonfinite_probe<__half>(uint32_t acc, uint32_t x) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&x), __half2(__half(0.f), __half(0.f)), *reinterpret_cast<__half2*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// Replaces infinities and NaN in row r of a V tile by zero; true if there were any.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ void clean_row(uint8_t* tile, int r) {
+#pragma unroll 1
+  for (int i = 0; i < CHUNKS * 64; ++i) {
+    T* e = reinterpret_cast<T*>(tile + (i >> 6) * kChunkBytes + r * 128 + (((((i & 63) >> 3) ^ (r & 7)) << 4)) + (i & 7) * 2);
+    if (!isfinite(St<T>::f(*e))) *e = St<T>::t(0.f);
+  }
+}
+template <typename T, int CHUNKS>
+__device__ __forceinline__ bool row_is_finite(const uint8_t* tile, int r) {
+  uint32_t acc = 0;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll 4
+    for (int i = 0; i < 8; ++i) {  // pieces in an order that spreads the lanes over the banks
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kChunkBytes + r * 128 + ((i ^ (r & 7)) << 4));
+      acc = nonfinite_probe<T>(acc, v.x);
+      acc = nonfinite_probe<T>(acc, v.y);
+      acc = nonfinite_probe<T>(acc, v.z);
+      acc = nonfinite_probe<T>(acc, v.w);
+    }
+  }
+  const float2 f = St<T>::unpack(acc);
+  return f.x == 0.f && f.y == 0.f;
+}
+
+// Adds the infinities and NaN of the rows j0 .. j1 - 1 of v (`channels`
+// channels of them) to a staged output row.
+template <typename T>
+__device__ __forceinline__ void add_nonfinite(uint8_t* row, int lane, const T* v, int64_t stride, int j0, int j1, int channels) {
+#pragma unroll 1
+  for (int j = j0; j < j1; ++j) {
+#pragma unroll 1
+    for (int i = 0; i < channels; ++i) {
+      const float x = St<T>::f(v[j * stride + i]);
+      if (isfinite(x)) continue;
+      T* e = reinterpret_cast<T*>(row + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2);
+      *e = St<T>::t(St<T>::f(*e) + x);
+    }
+  }
+}
+
+// Scores from column lim on are not seen.
+template <int N>
+__device__ __forceinline__ void cut(float* f, int lim) {
+  if (lim < N) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) f[c] = c < lim ? f[c] : -INFINITY;
+  }
+}
+template <int N>
+__device__ __forceinline__ float row_max(float* f, int lim) {
+  cut<N>(f, lim);
+  float mx[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+  for (int c = 4; c < N; c += 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (c % 8 == 4 && c + 4 < N) mx[e] = max3(mx[e], f[c + e], f[c + 4 + e]);
+      else if (c % 8 == 4) mx[e] = fmaxf(mx[e], f[c + e]);
+    }
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem + C::kOffQ;
+  uint8_t* sKV = smem + C::kOffKV;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = q_full + 1;             // the item's score MMAs are done
+  uint64_t* kv_full = q_empty + 1;            // [kSlots]
+  uint64_t* kv_empty = kv_full + C::kSlots;   // [kSlots]
+  uint64_t* s_full = kv_empty + C::kSlots;    // [2] scores of a tile
+  uint64_t* p_full = s_full + 2;              // [2] weights of a tile
+  uint64_t* o_full = p_full + 2;              // [2] an item's output
+  uint64_t* item_full = o_full + 2;           // [kItems]
+  uint64_t* item_empty = item_full + kItems;  // [kItems]
+  uint64_t* drain = item_empty + kItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  volatile int* v_cleaned = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 16);
+  volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);  // 4 warps
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 9);  // 8 softmax warps, MMA
+    }
+    mbar_init(drain, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
+    *v_cleaned = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto t_s = [&](int t) { return tmem + t * kN; };            // scores, then weights of tile t
+  auto t_o = [&](int t) { return tmem + 2 * kN + t * DP; };   // output of tile t
+  const WaitLimit tmo{p.timeout_ns, p.host_status};
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // ---------------------------------------------------------- producer
+      if (lane == 0) {
+        prefetch_map(&p.qmap);
+        prefetch_map(&p.kmap);
+        prefetch_map(&p.vmap);
+        prefetch_map(&p.omap);
+      }
+      TileWalk walk;
+      bool ok = true;
+      uint32_t g = 0;  // K / V slot uses
+      uint32_t nq = 0;  // items with loads
+      for (int n = 0;; ++n) {
+        const int64_t i = (int64_t)blockIdx.x + (int64_t)n * gridDim.x;
+        int b = 0, local = 0, tiles = 0;
+        const int64_t tile = i / p.Hq;
+        const bool more = tile < (1ll << 31) && walk.find(p.pk, false, kItemRows, (int)tile, &b, &local, &tiles);
+        Item it{};
+        if (more) {
+          const Seq s = sequence(p.pk, b);
+          // the rows that see most come first
+          const int i0 = (p.pk.causal ? tiles - 1 - local : local) * kItemRows;
+          it.row = s.q0 + i0;
+          it.n = min(kItemRows, s.nq - i0);
+          it.h = (int)(i - tile * p.Hq);
+          it.k0 = s.k0;
+          it.nk = s.nk;
+          it.see = p.pk.causal ? i0 + 1 + s.nk - s.nq : s.nk;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int last = min(it.n, (t + 1) * kM) - 1;  // last row of the tile
+            const int see = p.pk.causal ? max(0, min(s.nk, it.see + last)) : s.nk;
+            it.nt[t] = last >= t * kM ? (see + kN - 1) / kN : 0;
+          }
+        }
+        if (lane == 0) {
+          const int slot = n % kItems;
+          ok = mbar_wait(&item_empty[slot], ((n / kItems) & 1) ^ 1, abort_flag, 1, tmo);
+          if (ok) {
+            items[slot].row = it.row; items[slot].n = it.n; items[slot].h = it.h; items[slot].k0 = it.k0;
+            items[slot].nk = it.nk; items[slot].see = it.see; items[slot].nt[0] = it.nt[0]; items[slot].nt[1] = it.nt[1];
+            mbar_arrive(&item_full[slot]);
+          }
+          const int tiles_k = max(it.nt[0], it.nt[1]);
+          if (ok && tiles_k > 0) {
+            ok = mbar_wait(q_empty, (nq & 1) ^ 1, abort_flag, 1, tmo);
+            if (ok) {
+              const int qt = it.n > kM ? 2 : 1;  // query tiles with rows
+              mbar_expect_tx(q_full, qt * C::kQBytes);
+              for (int t = 0; t < qt; ++t) {
+#pragma unroll
+                for (int c = 0; c < C::kChunks; ++c)
+                  load_rows(sQ + t * C::kQBytes + c * kChunkBytes, &p.qmap, q_full, 64 * c, it.h, it.row + t * kM);
+              }
+            }
+            ++nq;
+            const int hk = it.h / p.group;
+            for (int j = 0; j < tiles_k && ok; ++j) {
+#pragma unroll
+              for (int w = 0; w < 2; ++w, ++g) {  // K_j, V_j
+                const int s = g % C::kSlots;
+                ok = ok && mbar_wait(&kv_empty[s], ((g / C::kSlots) & 1) ^ 1, abort_flag, 1, tmo);
+                if (!ok) break;
+                mbar_expect_tx(&kv_full[s], C::kSlotBytes);
+#pragma unroll
+                for (int c = 0; c < C::kChunks; ++c)
+                  load_rows(sKV + s * C::kSlotBytes + c * kChunkBytes, w == 0 ? &p.kmap : &p.vmap, &kv_full[s], 64 * c, hk,
+                            it.k0 + j * kN);
+              }
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok || !more) break;
+      }
+      if (!ok) {  // let issued loads land before the CTA can exit
+        const uint64_t t0 = gtimer();
+        while (gtimer() - t0 < 200000ull) {}
+      }
+    } else if (warp == 9 && lane == 0) {
+      // -------------------------------------------------------- MMA issuer
+      constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
+      constexpr uint32_t kIdO = idesc_f16(St<T>::kFmt, 1, kM, DP);
+      const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
+      const uint32_t aQ = su32(sQ), aKV = su32(sKV);
+      bool ok = true;
+      uint32_t g = 0, nq = 0;
+      uint32_t np[2] = {0, 0};
+      auto scores = [&](int t, uint32_t slot) {
+        const uint32_t a = aQ + t * C::kQBytes, b = aKV + slot * C::kSlotBytes;
+        for (int ks = 0; ks < ksteps; ++ks) {
+          const uint32_t off = (ks >> 2) * kChunkBytes + 32 * (ks & 3);
+          tc_mma(t_s(t), mdesc(a + off, 16, 1024, kLayoutSw128), mdesc(b + off, 16, 1024, kLayoutSw128), kIdS, ks > 0);
+        }
+        tc_commit(&s_full[t]);
+      };
+      for (int n = 0; ok; ++n) {
+        const int islot = n % kItems;
+        ok = mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 2, tmo);
+        if (!ok) break;
+        const int rows = items[islot].n;
+        const int nt[2] = {items[islot].nt[0], items[islot].nt[1]};
+        mbar_arrive(&item_empty[islot]);
+        if (rows == 0) break;
+        const int tiles = max(nt[0], nt[1]);
+        if (tiles == 0) continue;
+        ok = mbar_wait(q_full, nq & 1, abort_flag, 2, tmo) &&
+             mbar_wait(&kv_full[g % C::kSlots], (g / C::kSlots) & 1, abort_flag, 2, tmo);
+        ++nq;
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (nt[t] > 0) scores(t, g % C::kSlots);
+        tc_commit(&kv_empty[g % C::kSlots]);
+        if (tiles == 1) tc_commit(q_empty);
+        for (int j = 0; j < tiles && ok; ++j) {
+          const uint32_t gv = g + 2 * j + 1, gk = gv + 1;  // V_j, K_j+1
+          const uint32_t sv = gv % C::kSlots, sk = gk % C::kSlots;
+          ok = mbar_wait(&kv_full[sv], (gv / C::kSlots) & 1, abort_flag, 2, tmo) &&
+               (j + 1 >= tiles || mbar_wait(&kv_full[sk], (gk / C::kSlots) & 1, abort_flag, 2, tmo));
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t] || !ok) continue;
+            ok = mbar_wait(&p_full[t], np[t] & 1, abort_flag, 2, tmo);
+            if (!ok) break;
+            ++np[t];
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < kN / 16; ++ks)
+              mma_tmem_a(t_o(t), t_s(t) + 8 * ks, mdesc(aKV + sv * C::kSlotBytes + 2048 * ks, kChunkBytes, 1024, kLayoutSw128),
+                         kIdO, (j > 0 || ks > 0) ? 1u : 0u);
+            if (j + 1 < nt[t]) scores(t, sk);
+            else tc_commit(&o_full[t]);
+          }
+          if (!ok) break;
+          tc_commit(&kv_empty[sv]);
+          if (j + 1 < tiles) tc_commit(&kv_empty[sk]);
+          if (j + 2 == tiles) tc_commit(q_empty);
+        }
+        g += 2 * tiles;
+      }
+      // all issued MMAs complete before TMEM can be released (this wait
+      // ignores the abort flag: it must not be cut short by another role)
+      tc_commit(drain);
+      mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2;
+    const int q = warp & 3;
+    const int r = 32 * q + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)(32 * q) << 16;
+    const uint32_t ts = t_s(t) + lane_off, to = t_o(t) + lane_off;
+    const float c2 = p.scale * kLog2e;
+    uint8_t* stage = smem + C::kOffStage + warp * C::kStageBytes;
+    uint32_t ns = 0, no = 0, g = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int islot = n % kItems;
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 3, tmo));
+      if (!ok) break;
+      Item it;
+      it.row = items[islot].row; it.n = items[islot].n; it.h = items[islot].h; it.k0 = items[islot].k0;
+      it.nk = items[islot].nk; it.see = items[islot].see;
+      const int tiles = items[islot].nt[t], all_tiles = max(items[islot].nt[0], items[islot].nt[1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[islot]);
+      if (it.n == 0) break;
+      const int rows = min(kM, it.n - t * kM);  // of this tile; may be <= 0
+      const int see = p.pk.causal ? max(0, min(it.nk, it.see + t * kM + r)) : it.nk;  // keys this row sees
+      // tiles from edge on hold keys that the tile's first row does not see
+      const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + t * kM)) : it.nk) / kN;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < tiles; ++j, ++ns) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], ns & 1, abort_flag, 3, tmo));
+        if (!ok) break;
+        tc_fence_after();
+        // The row maximum, then the weights.  A thread holds 64 of its 128
+        // scores at a time: columns 64.. are read for the maximum and again
+        // for the weights (128 more cycles of TMEM reads per tile, hidden
+        // behind the exponentials), since all 128 with the packed weights
+        // and the addresses do not fit a thread's registers.
+        const int lim = j >= edge ? see - j * kN : kN;
+        uint32_t sa[64], sb[32];
+        float* fa = reinterpret_cast<float*>(sa);
+        float* fb = reinterpret_cast<float*>(sb);
+        float mj = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tc_ld32(ts + 64 + 32 * c, sb);
+          tc_wait_ld_regs(sb);
+          mj = fmaxf(mj, row_max<32>(fb, lim - 64 - 32 * c));
+        }
+        tc_ld32(ts, sa);
+        tc_ld32(ts + 32, sa + 32);
+        tc_wait_ld_regs(sa);
+        tc_wait_ld_regs(sa + 32);
+        mj = fmaxf(mj, row_max<64>(fa, lim));
+        if (j == 0) {
+          m = mj;
+        } else {
+          const bool grow = (mj - m) * c2 > kRescale;  // also from m = -inf
+          if (__any_sync(0xffffffffu, grow)) {
+            // the score MMAs of this tile came after the product that last
+            // wrote O, so O is complete
+            const float a = grow ? ex2((m - mj) * c2) : 1.f;
+            if (grow) m = mj;
+            l *= a;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+              uint32_t o[16];
+              tc_ld16(to + c, o);
+              tc_wait_ld_regs16(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+              tmem_st16(to + c, o);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c2;
+        const float2 c22 = make_float2(c2, c2), mc2 = make_float2(-mc, -mc);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // 32 scores -> weights in columns 16 h.. of the tile (the scores
+        // there have been read before)
+        auto weights = [&](const float* f, int h) {
+          uint32_t w[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float2 x = __ffma2_rn(make_float2(f[c], f[c + 1]), c22, mc2);
+            const float2 y = make_float2(ex2(x.x), ex2(x.y));
+            sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], y);
+            w[c / 2] = St<T>::pack(y.x, y.y);
+          }
+          tmem_st16(ts + 16 * h, w);
+        };
+        tc_ld32(ts + 64, sb);
+        weights(fa, 0);
+        weights(fa + 32, 1);
+        tc_wait_ld_regs(sb);
+        tc_ld32(ts + 96, sa);
+        cut<32>(fb, lim - 64);
+        weights(fb, 2);
+        tc_wait_ld_regs(sa);
+        cut<32>(fa, lim - 96);
+        weights(fa, 3);
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        if (j >= edge) {
+          // V tile j: infinities and NaN out (see the top of the file)
+          const uint32_t gv = g + 2 * j + 1;
+          uint8_t* tile = sKV + (gv % C::kSlots) * C::kSlotBytes;
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[gv % C::kSlots], (gv / C::kSlots) & 1, abort_flag, 3, tmo));
+          if (!ok) break;
+          if (!row_is_finite<T, C::kChunks>(tile, r)) {
+            *v_cleaned = 1;
+            __threadfence_block();
+            clean_row<T, C::kChunks>(tile, r);
+            fence_proxy_async();
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      g += 2 * all_tiles;
+      if (rows <= 0) continue;
+      // ---------------------------------------------------------- epilogue
+      if (tiles > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1, abort_flag, 4, tmo));
+        if (!ok) break;
+        ++no;
+        tc_fence_after();
+      }
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+      if (p.lse != nullptr && r < rows)
+        p.lse[(int64_t)it.h * p.pk.T + it.row + t * kM + r] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+      const int wrows = min(32, rows - 32 * q);  // of this warp
+      const bool fix = *v_cleaned != 0;
+#pragma unroll 1
+      for (int c = 0; c < C::kChunks; ++c) {
+        if (64 * c >= p.D) break;
+        uint32_t o[64];
+        if (tiles > 0) {
+          tc_ld32(to + 64 * c, o);
+          tc_ld32(to + 64 * c + 32, o + 32);
+          tc_wait_ld_regs(o);
+          tc_wait_ld_regs(o + 32);
+        }
+        if (lane == 0) bulk_wait_read0();  // the staging buffer is free
+        __syncwarp();
+        uint8_t* row = stage + lane * 128;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = inv == 0.f ? 0.f : __uint_as_float(o[8 * e + i]) * inv;
+          *reinterpret_cast<uint4*>(row + ((e ^ (lane & 7)) << 4)) =
+              make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
+        }
+        if (fix && tiles > 0) {
+          // add the values taken out of the tiles on the edge of this item
+          const int e0 = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN * kN;
+          add_nonfinite<T>(row, lane, static_cast<const T*>(p.v.p) + (int64_t)it.k0 * p.v.t + (it.h / p.group) * p.v.h + 64 * c,
+                           p.v.t, e0, see, min(64, p.D - 64 * c));
+        }
+        fence_proxy_async();
+        __syncwarp();
+        const int row0 = it.row + t * kM + 32 * q;
+        if (wrows == 32) {
+          if (lane == 0) {
+            tma_store(&p.omap, stage, 64 * c, it.h, row0, 0);
+            bulk_commit();
+          }
+        } else {  // the rows behind the sequence are not ours
+          for (int e = lane; e < wrows * 8; e += 32) {
+            const int rr = e >> 3, piece = e & 7;
+            if (64 * c + 8 * piece < p.D)
+              *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(p.out.p)) + (int64_t)(row0 + rr) * p.out.t +
+                                        (int64_t)it.h * p.out.h + 64 * c + 8 * piece) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();  // O has been read: the next item's first product (after p_full) may overwrite it
+    }
+    // rows of no sequence: zeros, lse -inf
+    const int lo = p.pk.B > 0 ? segment(p.pk.cu_q, 0, p.pk.T).x : 0;
+    int hi = lo;
+    if (p.pk.B > 0) {
+      const int2 e = segment(p.pk.cu_q, p.pk.B - 1, p.pk.T);
+      hi = max(lo, e.x + e.y);
+    }
+    const int64_t gap = (int64_t)lo + (p.pk.T - hi);
+    for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < gap * p.Hq; i += (int64_t)gridDim.x * 8) {
+      const int64_t k = i / p.Hq;
+      const int h = (int)(i - k * p.Hq);
+      const int64_t row = k < lo ? k : hi + (k - lo);
+      T* o = static_cast<T*>(const_cast<void*>(p.out.p)) + row * p.out.t + (int64_t)h * p.out.h;
+      for (int e = lane * 8; e < p.D; e += 256) *reinterpret_cast<uint4*>(o + e) = make_uint4(0, 0, 0, 0);
+      if (p.lse != nullptr && lane == 0) p.lse[(int64_t)h * p.pk.T + row] = -INFINITY;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+template <typename T, int DP>
+int launch(const Params& p, int dev, int grid, cudaStream_t s) {
+  static std::atomic<bool> configured[64] = {};
+  const int rc = opt_in_smem(attention_kernel<T, DP>, Cfg<DP>::kSmem, configured, dev);
+  if (rc != UPLIFT_LA_OK) return rc;
+  attention_kernel<T, DP><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(p);
+  return launched("attention");
+}
+
+}  // namespace fwd
+
+int make_row_map(CUtensorMap* map, int dtype, const Rows& r, int64_t rows, int heads, int D, int box_rows) {
+  const CUtensorMapDataType dt = dtype == UPLIFT_LA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return tc_make_map(map, dt, 2, r.p, D, heads, (int)rows, 1, r.h, r.t, r.t * rows, 64, 1, box_rows);
+}
+
+int sm_count(int* dev, int* sms) {
+  if (cudaGetDevice(dev) != cudaSuccess) return fail(UPLIFT_LA_ERR_NO_DEVICE, "cudaGetDevice failed");
+  static std::atomic<int> counts[64] = {};
+  *sms = (*dev >= 0 && *dev < 64) ? counts[*dev].load(std::memory_order_relaxed) : 0;
+  if (*sms == 0) {
+    if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess || *sms < 1)
+      return fail(UPLIFT_LA_ERR_NO_DEVICE, "no multiprocessor count");
+    if (*dev >= 0 && *dev < 64) counts[*dev].store(*sms, std::memory_order_relaxed);
+  }
+  return UPLIFT_LA_OK;
+}
+
+int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
+  using namespace fwd;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  int dev = 0, sms = 0;
+  int rc = sm_count(&dev, &sms);
+  if (rc == UPLIFT_LA_OK) rc = make_row_map(&p.qmap, a.dtype, a.q, a.pk.T, a.Hq, a.D, kM);
+  // without key rows no K / V box is ever loaded; the maps stay empty
+  if (rc == UPLIFT_LA_OK && a.pk.S > 0) rc = make_row_map(&p.kmap, a.dtype, a.k, a.pk.S, a.Hk, a.D, kN);
+  if (rc == UPLIFT_LA_OK && a.pk.S > 0) rc = make_row_map(&p.vmap, a.dtype, a.v, a.pk.S, a.Hk, a.D, kN);
+  if (rc == UPLIFT_LA_OK) rc = make_row_map(&p.omap, a.dtype, a.out, a.pk.T, a.Hq, a.D, 32);
+  if (rc != UPLIFT_LA_OK) return rc;
+  p.v = a.v;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.pk = a.pk;
+  p.Hq = a.Hq;
+  p.group = a.Hq / a.Hk;
+  p.D = a.D;
+  p.scale = a.scale;
+  p.timeout_ns = tc_test_timeout_ns() != 0 ? tc_test_timeout_ns() : kTimeoutNs;
+  p.host_status = host_status_word();
+  const int64_t most = ((int64_t)a.pk.T / kItemRows + a.pk.B) * a.Hq;  // items, at most
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
+  if (a.dtype == UPLIFT_LA_BF16)
+    return a.D <= 64 ? launch<__nv_bfloat16, 64>(p, dev, grid, s) : launch<__nv_bfloat16, 128>(p, dev, grid, s);
+  return a.D <= 64 ? launch<__half, 64>(p, dev, grid, s) : launch<__half, 128>(p, dev, grid, s);
+}
+
+int attn_fwd_device_status(bool clear) {
+  unsigned int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_tok_fwd_status, sizeof(v));
+  if (e == cudaSuccess && clear && v != 0) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbol(g_tok_fwd_status, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) {
+    fail(UPLIFT_LA_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
+    return -1;
+  }
+  return (int)v;
+}
+
+}  // namespace tok
+}  // namespace ula

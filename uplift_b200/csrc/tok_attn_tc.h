@@ -1,0 +1,141 @@
+// Parts shared by the tensor-core kernels of the packed-sequence attention
+// (tok_attn_fwd.cu, tok_attn_bwd.cu): tensor maps, bounded waits, the walk
+// over sequences, TMEM operands and packed fp32 arithmetic.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "la_tc_common.h"
+#include "tok_attn.h"
+
+namespace ula {
+namespace tok {
+
+using namespace ::ula::tc;
+
+// ------------------------------------------------------------ tensor maps
+// [rows, heads, D] as axes (D, head, row), box {64 channels, 1, box_rows}.
+// Boxes that reach beyond a sequence hold rows of the next one (zeros behind
+// the tensor's last row); the kernels see to it that these reach no result.
+int make_row_map(CUtensorMap* map, int dtype, const Rows& r, int64_t rows, int heads, int D, int box_rows);
+
+__device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, uint64_t* bar, int c, int h, int row) {
+  tma_load(dst, map, bar, c, h, row, 0);
+}
+
+// ------------------------------------------------------------ waits
+// mbar_wait_status of la_tc_common.h as inline code.
+__device__ __forceinline__ bool mbar_wait_inline(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
+                                                 const WaitLimit& limit, unsigned int* status) {
+  if (mbar_try(b, parity)) return true;
+  const uint64_t t0 = gtimer();
+  bool ok = true;
+#pragma unroll 1
+  for (uint32_t it = 1; !mbar_try(b, parity); ++it) {
+    if ((it & 63u) != 0) continue;
+    if (*abort_flag) {
+      ok = false;
+      break;
+    }
+    if (gtimer() - t0 > limit.ns) {
+      *abort_flag = 1;
+      atomicCAS(status, 0u, where);
+      if (limit.host_word != nullptr) {
+        *reinterpret_cast<volatile unsigned int*>(limit.host_word) = where;
+        __threadfence_system();
+      }
+      ok = false;
+      break;
+    }
+  }
+  return ok;
+}
+
+// ------------------------------------------------------------ sequences
+// Tile number -> (sequence, tile of the sequence), for numbers that only
+// grow: a warp looks at 32 sequences at a time and goes on from where the
+// last search ended.  `by_keys`: tiles of the key segments, else of the
+// queries.
+struct TileWalk {
+  int b0 = 0;       // first sequence of the window
+  int before = 0;   // tiles before the window
+  // all lanes; false: there is no such tile
+  __device__ __forceinline__ bool find(const Packing& p, bool by_keys, int tile_rows, int tile, int* b, int* local,
+                                       int* tiles) {
+    const int lane = threadIdx.x & 31;
+    while (b0 < p.B) {
+      int n = 0;
+      if (b0 + lane < p.B)
+        n = ((by_keys ? segment(p.cu_k, b0 + lane, p.S).y : segment(p.cu_q, b0 + lane, p.T).y) + tile_rows - 1) /
+            tile_rows;
+      int sum = n;  // inclusive scan
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const int total = __shfl_sync(0xffffffffu, sum, 31);
+      if (tile < before + total) {
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < before + sum);
+        const int l = __ffs(hit) - 1;
+        *tiles = __shfl_sync(0xffffffffu, n, l);
+        *local = tile - before - (__shfl_sync(0xffffffffu, sum, l) - *tiles);
+        *b = b0 + l;
+        return true;
+      }
+      before += total;
+      b0 += 32;
+    }
+    return false;
+  }
+};
+
+// ------------------------------------------------------------ TMEM
+// kind::f16 MMA with the A operand in TMEM (lane = row; a 32-bit column
+// holds two consecutive K elements).
+__device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ------------------------------------------------------------ arithmetic
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+}  // namespace tok
+}  // namespace ula

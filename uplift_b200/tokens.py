@@ -65,12 +65,12 @@ def _check_rows(what: str, named) -> None:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy where the kernels cannot read it in place: channel stride 1 and, in 16 bits,
-    16-byte aligned rows."""
+    16-byte aligned rows whose stride is a multiple of the heads'."""
     st, hd = t.stride(), t.shape
     ok = st[2] == 1 or hd[2] == 1
     if ok and t.element_size() == 2:
         ok = (t.data_ptr() & 15) == 0 and (hd[0] <= 1 or (st[0] > 0 and st[0] % 8 == 0)) and (
-            hd[1] <= 1 or (st[1] > 0 and st[1] % 8 == 0))
+            hd[1] <= 1 or (st[1] > 0 and st[1] % 8 == 0 and (hd[0] <= 1 or st[0] % st[1] == 0)))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
