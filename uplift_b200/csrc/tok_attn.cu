@@ -53,7 +53,10 @@ Rows rows_of(const void* p, const int64_t* st, int64_t rows, int heads, int D) {
 }  // namespace
 }  // namespace tok
 
-int tok_device_status(bool clear) { return tok::attn_fwd_device_status(clear); }
+int tok_device_status(bool clear) {
+  const int f = tok::attn_fwd_device_status(clear), b = tok::attn_bwd_device_status(clear);
+  return f < 0 || b < 0 ? -1 : (f != 0 ? f : b);
+}
 
 }  // namespace ula
 
@@ -131,7 +134,8 @@ int uplift_tok_attention_backward(const void* dout, const int64_t dout_strides[2
   a.delta = delta;
   a.pk = Packing{cu_q, cu_k, used_k, B, (int)T, (int)S, causal != 0};
   a.Hq = Hq; a.Hk = Hk; a.D = D; a.scale = scale; a.dtype = dtype;
-  return attn_simt_backward(a, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == UPLIFT_LA_F32 ? attn_simt_backward(a, s) : attn_tc_backward(a, s);
 }
 
 }  // extern "C"

@@ -29,6 +29,9 @@ struct AttnArgs {
 // bf16 / fp16 attention on the tensor cores (tok_attn_fwd.cu).
 int attn_tc_forward(const AttnArgs& a, cudaStream_t s);
 int attn_fwd_device_status(bool clear);
+// Their gradients (tok_attn_bwd.cu).
+int attn_tc_backward(const AttnArgs& a, cudaStream_t s);
+int attn_bwd_device_status(bool clear);
 
 // fp32 attention on CUDA cores (tok_attn_simt.cu).
 int attn_simt_forward(const AttnArgs& a, cudaStream_t s);

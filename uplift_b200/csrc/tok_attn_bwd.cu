@@ -1,0 +1,693 @@
+// Gradients of the packed-sequence attention on the tensor cores of B200
+// (sm_100a), bf16 / fp16, D <= 128.  With P = exp(scale S - lse), S = Q K^T,
+//
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O),
+//   dQ = scale dS K,  dK = scale dS^T Q.
+//
+// Two passes of one kernel, each of which owns the rows it writes, so that
+// no sum needs atomics and results do not depend on the order of CTAs:
+//
+//   KEYS:  128 keys of one key head stay, 64 queries at a time go by, over
+//          all heads of the group (their sum is dK / dV):
+//            S^T[128 x 64] = K Q^T,  dP^T[128 x 64] = V dO^T,
+//            dV[128 x D] += P^T dO,  dK[128 x D] += dS^T Q;
+//   else:  128 queries of one head stay, 64 keys at a time go by:
+//            S[128 x 64] = Q K^T,    dP[128 x 64] = dO V^T,
+//            dQ[128 x D] += dS K.
+//
+// That is 7 products where 5 would do if dQ were summed over CTAs.  In both
+// passes the rows that stay (X0, X1) are the A operands of the first two
+// products from shared memory, and P / dS, written over S / dP in TMEM in the
+// storage type, are the A operands of the others; the tiles that go by
+// (Y0, Y1) are read K-major by the first and MN-major by the second, so
+// nothing is transposed or stored.  Two TMEM buffers of S and dP alternate:
+// while one group of warps forms P and dS of a step the tensor cores work on
+// the next.
+//
+// Roles (384 threads, one persistent CTA per SM): warps 0-3 and 4-7 the two
+// groups, taking steps in turn (a thread per row that stays) and storing the
+// results; warp 8 looks items up and issues TMA loads; warp 9 issues MMAs;
+// warp 10 (KEYS) fetches lse and delta of the queries that go by.
+//
+// Rows that go by behind the end of their sequence belong to the next one:
+// their P and dS are set to zero and the rows in shared memory too, since an
+// infinity or NaN in them would turn the products into NaN.
+
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "tok_attn_tc.h"
+
+namespace ula {
+
+__device__ unsigned int g_tok_bwd_status;
+
+namespace tok {
+namespace bwd {
+
+constexpr int kM = 128;   // rows that stay
+constexpr int kN = 64;    // rows that go by in a step
+constexpr int kThreads = 384;
+constexpr int kTmemCols = 512;
+constexpr int kItems = 2;
+constexpr int kAux = 4;   // ring of lse / delta
+constexpr uint64_t kTimeoutNs = 2000000000ull;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DP>
+struct Cfg {
+  static constexpr int kChunks = DP / 64;
+  static constexpr int kXChunk = kM * 128, kYChunk = kN * 128;  // 64 channels of a tile
+  static constexpr int kXBytes = kChunks * kXChunk;
+  static constexpr int kYBytes = kChunks * kYChunk;
+  static constexpr int kStages = DP == 128 ? 3 : 6;             // Y0 and Y1 together
+  static constexpr int kOffX = 0;
+  static constexpr int kOffY = 2 * kXBytes;
+  static constexpr int kOffStage = kOffY + kStages * 2 * kYBytes;
+  static constexpr int kStageBytes = 32 * 128;                  // a warp's 32 rows x 64 channels
+  static constexpr int kOffAux = kOffStage + 8 * kStageBytes;
+  static constexpr int kOffBar = kOffAux + kAux * 2 * kN * 4;
+  static constexpr int kNumBars = 2 + 2 * kStages + 2 * kAux + 4 + 2 + 2 * kItems + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kOffItems = kOffMisc + 32;
+  static constexpr int kSmem = kOffItems + kItems * 48 + 1024;  // + base alignment slack
+  static_assert(kSmem <= 232448, "shared memory");
+  // TMEM columns: two buffers of S and dP, then the sums
+  static constexpr int kColAcc = 4 * kN;
+  static_assert(kColAcc + 2 * DP <= kTmemCols, "TMEM");
+};
+
+struct Item {
+  int n;       // rows that stay, 1..128; 0: no more items
+  int live;    // of these, rows with a gradient (keys in use); the others get zeros
+  int row;     // their first row in the tensor
+  int h;       // head of the rows that stay
+  int y0;      // first row that goes by (in the tensor)
+  int ny;      // number of them (per head)
+  int steps;   // steps of 64 of them (per head)
+  int off;     // row r that stays and column c that goes by see each other, if causal, when KEYS: c >= r + off
+               // at the first step (64 less at each further one); else: c < r + off (64 less ..)
+};
+
+struct Params {
+  CUtensorMap x0, x1;  // rows that stay: K, V or Q, dO; box {64, 1, 128}
+  CUtensorMap y0, y1;  // rows that go by: Q, dO or K, V; box {64, 1, 64}
+  CUtensorMap o0, o1;  // results: dV, dK or dQ; box {64, 1, 32}
+  Rows out0, out1;
+  const float* lse;
+  const float* delta;
+  Packing pk;
+  int heads, group, D;  // heads of the rows that stay
+  float scale;
+  uint64_t timeout_ns;
+  unsigned int* host_status;
+};
+
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
+                                          const WaitLimit& limit) {
+  return mbar_wait_inline(b, parity, abort_flag, where, limit, &g_tok_bwd_status);
+}
+
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem + C::kOffX;
+  uint8_t* sY = smem + C::kOffY;
+  float* sAux = reinterpret_cast<float*>(smem + C::kOffAux);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* x_full = bars;
+  uint64_t* x_empty = x_full + 1;
+  uint64_t* y_full = x_empty + 1;             // [kStages]
+  uint64_t* y_empty = y_full + C::kStages;    // [kStages]
+  uint64_t* a_full = y_empty + C::kStages;    // [kAux]
+  uint64_t* a_empty = a_full + kAux;          // [kAux]
+  uint64_t* s_full = a_empty + kAux;          // [2] S and dP of a step
+  uint64_t* p_full = s_full + 2;              // [2] P and dS of a step
+  uint64_t* acc_full = p_full + 2;            // an item's sums
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* item_full = acc_empty + 1;        // [kItems]
+  uint64_t* item_empty = item_full + kItems;  // [kItems]
+  uint64_t* drain = item_empty + kItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(x_full, 1);
+    mbar_init(x_empty, 1);
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&y_full[i], 1);
+      mbar_init(&y_empty[i], 1);
+    }
+    for (int i = 0; i < kAux; ++i) {
+      mbar_init(&a_full[i], 1);
+      mbar_init(&a_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 8);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], KEYS ? 10 : 9);  // 8 warps of the groups, MMA, lse / delta
+    }
+    mbar_init(drain, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto col_s = [&](uint32_t b) { return tmem + b * 2 * kN; };
+  auto col_dp = [&](uint32_t b) { return tmem + b * 2 * kN + kN; };
+  const uint32_t col_acc = tmem + C::kColAcc;
+  const WaitLimit tmo{p.timeout_ns, p.host_status};
+  // heads that go by per item
+  const int passes = KEYS ? p.group : 1;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      prefetch_map(&p.x0);
+      prefetch_map(&p.x1);
+      if (p.pk.T > 0 && p.pk.S > 0) {
+        prefetch_map(&p.y0);
+        prefetch_map(&p.y1);
+      }
+    }
+    TileWalk walk;
+    bool ok = true;
+    uint32_t g = 0, nx = 0;
+    for (int n = 0;; ++n) {
+      const int64_t i = (int64_t)blockIdx.x + (int64_t)n * gridDim.x;
+      int b = 0, local = 0, tiles = 0;
+      const int64_t tile = i / p.heads;
+      const bool more = tile < (1ll << 31) && walk.find(p.pk, KEYS, kM, (int)tile, &b, &local, &tiles);
+      Item it{};
+      if (more) {
+        const Seq s = sequence(p.pk, b);
+        it.h = (int)(i - tile * p.heads);
+        const int shift = s.nk - s.nq;  // causal: query i sees keys <= i + shift
+        if (KEYS) {
+          const int seg = segment(p.pk.cu_k, b, p.pk.S).y;
+          const int j0 = local * kM;  // the first keys are seen by most queries
+          it.row = s.k0 + j0;
+          it.n = min(kM, seg - j0);
+          it.live = max(0, min(it.n, s.nk - j0));
+          const int i0 = p.pk.causal ? max(0, j0 - shift) : 0;
+          it.y0 = s.q0 + i0;
+          it.ny = it.live > 0 ? max(0, s.nq - i0) : 0;
+          it.off = j0 - shift - i0;
+        } else {
+          const int i0 = (p.pk.causal ? tiles - 1 - local : local) * kM;  // the last queries see most keys
+          it.row = s.q0 + i0;
+          it.n = min(kM, s.nq - i0);
+          it.live = it.n;
+          it.y0 = s.k0;
+          it.ny = p.pk.causal ? max(0, min(s.nk, i0 + it.n + shift)) : s.nk;
+          it.off = i0 + 1 + shift;
+        }
+        it.steps = (it.ny + kN - 1) / kN;
+      }
+      if (lane == 0) {
+        const int slot = n % kItems;
+        ok = mbar_wait(&item_empty[slot], ((n / kItems) & 1) ^ 1, abort_flag, 1, tmo);
+        if (ok) {
+          items[slot].n = it.n; items[slot].live = it.live; items[slot].row = it.row; items[slot].h = it.h;
+          items[slot].y0 = it.y0; items[slot].ny = it.ny; items[slot].steps = it.steps; items[slot].off = it.off;
+          mbar_arrive(&item_full[slot]);
+        }
+        if (ok && it.steps > 0) {
+          ok = mbar_wait(x_empty, (nx & 1) ^ 1, abort_flag, 1, tmo);
+          ++nx;
+          if (ok) {
+            mbar_expect_tx(x_full, 2 * C::kXBytes);
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c) {
+              load_rows(sX + c * C::kXChunk, &p.x0, x_full, 64 * c, it.h, it.row);
+              load_rows(sX + C::kXBytes + c * C::kXChunk, &p.x1, x_full, 64 * c, it.h, it.row);
+            }
+          }
+          for (int e = 0; e < passes && ok; ++e) {
+            const int hy = KEYS ? it.h * p.group + e : it.h / p.group;
+            for (int j = 0; j < it.steps; ++j, ++g) {
+              const int s = g % C::kStages;
+              ok = mbar_wait(&y_empty[s], ((g / C::kStages) & 1) ^ 1, abort_flag, 1, tmo);
+              if (!ok) break;
+              uint8_t* y = sY + s * 2 * C::kYBytes;
+              mbar_expect_tx(&y_full[s], 2 * C::kYBytes);
+#pragma unroll
+              for (int c = 0; c < C::kChunks; ++c) {
+                load_rows(y + c * C::kYChunk, &p.y0, &y_full[s], 64 * c, hy, it.y0 + j * kN);
+                load_rows(y + C::kYBytes + c * C::kYChunk, &p.y1, &y_full[s], 64 * c, hy, it.y0 + j * kN);
+              }
+            }
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (!ok || !more) break;
+    }
+    if (!ok) {  // let issued loads land before the CTA can exit
+      const uint64_t t0 = gtimer();
+      while (gtimer() - t0 < 200000ull) {}
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
+      constexpr uint32_t kIdA = idesc_f16(St<T>::kFmt, 1, kM, DP);
+      const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
+      const uint32_t aX = su32(sX), aY = su32(sY);
+      bool ok = true;
+      uint32_t g = 0, nx = 0;  // steps and items with steps so far
+      auto first = [&](uint32_t gs) {  // S and dP of step gs
+        const uint32_t y = aY + (gs % C::kStages) * 2 * C::kYBytes;
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t d = w == 0 ? col_s(gs & 1) : col_dp(gs & 1);
+          for (int ks = 0; ks < ksteps; ++ks) {
+            const uint32_t c = ks >> 2, k = 32 * (ks & 3);
+            tc_mma(d, mdesc(aX + w * C::kXBytes + c * C::kXChunk + k, 16, 1024, kLayoutSw128),
+                   mdesc(y + w * C::kYBytes + c * C::kYChunk + k, 16, 1024, kLayoutSw128), kIdS, ks > 0);
+          }
+        }
+        tc_commit(&s_full[gs & 1]);
+      };
+      for (int n = 0; ok; ++n) {
+        const int islot = n % kItems;
+        ok = mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 2, tmo);
+        if (!ok) break;
+        const int rows = items[islot].n;
+        const int total = items[islot].steps * passes;
+        mbar_arrive(&item_empty[islot]);
+        if (rows == 0) break;
+        if (total == 0) continue;
+        ok = mbar_wait(x_full, nx & 1, abort_flag, 2, tmo);
+        // up to two steps of first products ahead of the second ones
+        for (int j = 0; j < min(2, total) && ok; ++j) {
+          ok = mbar_wait(&y_full[(g + j) % C::kStages], ((g + j) / C::kStages) & 1, abort_flag, 2, tmo);
+          if (!ok) break;
+          tc_fence_after();
+          first(g + j);
+        }
+        if (total <= 2) tc_commit(x_empty);
+        ok = ok && mbar_wait(acc_empty, (nx & 1) ^ 1, abort_flag, 2, tmo);
+        ++nx;
+        for (int j = 0; j < total && ok; ++j) {
+          const uint32_t gs = g + j, b = gs & 1;
+          ok = mbar_wait(&p_full[b], (gs >> 1) & 1, abort_flag, 2, tmo);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t y = aY + (gs % C::kStages) * 2 * C::kYBytes;
+          if (KEYS) {
+#pragma unroll
+            for (int ks = 0; ks < kN / 16; ++ks)
+              mma_tmem_a(col_acc, col_s(b) + 8 * ks, mdesc(y + C::kYBytes + 2048 * ks, C::kYChunk, 1024, kLayoutSw128), kIdA,
+                         (j > 0 || ks > 0) ? 1u : 0u);
+          }
+#pragma unroll
+          for (int ks = 0; ks < kN / 16; ++ks)
+            mma_tmem_a(col_acc + (KEYS ? DP : 0), col_dp(b) + 8 * ks, mdesc(y + 2048 * ks, C::kYChunk, 1024, kLayoutSw128),
+                       kIdA, (j > 0 || ks > 0) ? 1u : 0u);
+          tc_commit(&y_empty[gs % C::kStages]);
+          if (j + 2 < total) {
+            const uint32_t gn = gs + 2;
+            ok = mbar_wait(&y_full[gn % C::kStages], (gn / C::kStages) & 1, abort_flag, 2, tmo);
+            if (!ok) break;
+            tc_fence_after();
+            first(gn);
+            if (j + 3 == total) tc_commit(x_empty);
+          }
+        }
+        if (!ok) break;
+        tc_commit(acc_full);
+        g += total;
+      }
+      // all issued MMAs complete before TMEM can be released (this wait
+      // ignores the abort flag: it must not be cut short by another role)
+      tc_commit(drain);
+      mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------- lse and delta of the columns
+    if (KEYS) {
+      bool ok = true;
+      uint32_t g = 0;
+      for (int n = 0; ok; ++n) {
+        const int islot = n % kItems;
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 1, tmo));
+        if (!ok) break;
+        const int rows = items[islot].n, h = items[islot].h, y0 = items[islot].y0, ny = items[islot].ny,
+                  steps = items[islot].steps;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[islot]);
+        if (rows == 0) break;
+        for (int e = 0; e < passes && ok; ++e) {
+          const float* lse = p.lse + (int64_t)(h * p.group + e) * p.pk.T + y0;
+          const float* delta = p.delta + (int64_t)(h * p.group + e) * p.pk.T + y0;
+          for (int j = 0; j < steps; ++j, ++g) {
+            const int s = g % kAux;
+            ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], ((g / kAux) & 1) ^ 1, abort_flag, 1, tmo));
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < kN; c += 32) {
+              const int i = j * kN + c + lane;
+              float l = -INFINITY, d = 0.f;
+              if (i < ny) {
+                l = lse[i];
+                d = delta[i];
+              }
+              // negated, in powers of two; rows without keys: P = 0
+              sAux[s * 2 * kN + c + lane] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+              sAux[s * 2 * kN + kN + c + lane] = -d;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[s]);
+          }
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ P and dS
+    const int w = warp >> 2;
+    const int q = warp & 3;
+    const int r = 32 * q + lane;  // row that stays = TMEM lane
+    const uint32_t lane_off = (uint32_t)(32 * q) << 16;
+    const float c2 = p.scale * kLog2e;
+    uint8_t* stage = smem + C::kOffStage + warp * C::kStageBytes;
+    uint32_t g = 0, na = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int islot = n % kItems;
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 3, tmo));
+      if (!ok) break;
+      Item it;
+      it.n = items[islot].n; it.live = items[islot].live; it.row = items[islot].row; it.h = items[islot].h;
+      it.ny = items[islot].ny; it.steps = items[islot].steps; it.off = items[islot].off;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[islot]);
+      if (it.n == 0) break;
+      const int total = it.steps * passes;
+      float nlse = 0.f, ndelta = 0.f;
+      if (!KEYS) {
+        nlse = -INFINITY;
+        if (r < it.n) {
+          const int64_t at = (int64_t)it.h * p.pk.T + it.row + r;
+          const float l = p.lse[at];
+          nlse = l == -INFINITY ? -INFINITY : -l * kLog2e;
+          ndelta = -p.delta[at];
+        }
+      }
+      int j = 0;  // step within the head
+      for (int k = 0; k < total && ok; ++k, j = j + 1 == it.steps ? 0 : j + 1) {
+        const uint32_t gs = g + k;
+        if ((gs & 1) != (uint32_t)w) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[w], (gs >> 1) & 1, abort_flag, 3, tmo));
+        if (KEYS) ok = ok && __all_sync(0xffffffffu, mbar_wait(&a_full[gs % kAux], (gs / kAux) & 1, abort_flag, 3, tmo));
+        if (!ok) break;
+        tc_fence_after();
+        const float* aux = sAux + (gs % kAux) * 2 * kN;
+        // columns lo .. hi - 1 are seen
+        int lo = 0, hi = it.ny - j * kN;
+        if (p.pk.causal) {
+          if (KEYS) lo = r + it.off - j * kN;
+          else hi = min(hi, r + it.off - j * kN);
+        }
+        const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kN);
+        const uint32_t ts = col_s(w) + lane_off, td = col_dp(w) + lane_off;
+#pragma unroll
+        for (int c = 0; c < kN; c += 32) {
+          uint32_t s[32], d[32];
+          tc_ld32(ts + c, s);
+          tc_ld32(td + c, d);
+          tc_wait_ld_regs(s);
+          tc_wait_ld_regs(d);
+          float* fs = reinterpret_cast<float*>(s);
+          float* fd = reinterpret_cast<float*>(d);
+          const float2 c22 = make_float2(c2, c2);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndelta, ndelta, ndelta, ndelta);
+            if (KEYS) {
+              nl = *reinterpret_cast<const float4*>(aux + c + e);
+              nd = *reinterpret_cast<const float4*>(aux + kN + c + e);
+            }
+            const float2 x0 = __ffma2_rn(make_float2(fs[e], fs[e + 1]), c22, make_float2(nl.x, nl.y));
+            const float2 x1 = __ffma2_rn(make_float2(fs[e + 2], fs[e + 3]), c22, make_float2(nl.z, nl.w));
+            const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
+            const float2 d0 = __fmul2_rn(p0, __fadd2_rn(make_float2(fd[e], fd[e + 1]), make_float2(nd.x, nd.y)));
+            const float2 d1 = __fmul2_rn(p1, __fadd2_rn(make_float2(fd[e + 2], fd[e + 3]), make_float2(nd.z, nd.w)));
+            fs[e] = p0.x; fs[e + 1] = p0.y; fs[e + 2] = p1.x; fs[e + 3] = p1.y;
+            fd[e] = d0.x; fd[e + 1] = d0.y; fd[e + 2] = d1.x; fd[e + 3] = d1.y;
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const bool seen = c + e >= lo && c + e < hi;
+              fs[e] = seen ? fs[e] : 0.f;
+              fd[e] = seen ? fd[e] : 0.f;
+            }
+          }
+          uint32_t ps[16], ds[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            ps[e] = St<T>::pack(fs[2 * e], fs[2 * e + 1]);
+            ds[e] = St<T>::pack(fd[2 * e], fd[2 * e + 1]);
+          }
+          // over columns that have been read
+          if (KEYS) tmem_st16(ts + c / 2, ps);
+          tmem_st16(td + c / 2, ds);
+        }
+        const int rows = it.ny - j * kN;  // of the tile that goes by
+        if (rows < kN) {
+          // rows of the next sequence: zero (both tiles, all channels)
+          uint8_t* y = sY + (gs % C::kStages) * 2 * C::kYBytes;
+          for (int e = rows * 8 + (tid & 127); e < kN * 8; e += 128) {
+#pragma unroll
+            for (int c = 0; c < 2 * C::kChunks; ++c)
+              *reinterpret_cast<uint4*>(y + c * C::kYChunk + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (KEYS) mbar_arrive(&a_empty[gs % kAux]);
+          mbar_arrive(&p_full[w]);
+        }
+      }
+      if (!ok) break;
+      g += total;
+      // ---------------------------------------------------------- results
+      if (total > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_full, na & 1, abort_flag, 4, tmo));
+        if (!ok) break;
+        ++na;
+        tc_fence_after();
+      }
+      // KEYS: group 0 stores dV, group 1 dK; else each group every second chunk of dQ
+      const CUtensorMap* map = KEYS && w == 1 ? &p.o1 : &p.o0;
+      const Rows& out = KEYS && w == 1 ? p.out1 : p.out0;
+      const float f = KEYS && w == 0 ? 1.f : p.scale;
+      const int wrows = min(32, it.n - 32 * q);
+#pragma unroll 1
+      for (int c = KEYS ? 0 : w; c < C::kChunks; c += KEYS ? 1 : 2) {
+        if (64 * c >= p.D) break;
+        uint32_t o[64];
+        if (total > 0) {
+          const uint32_t src = col_acc + lane_off + (KEYS && w == 1 ? DP : 0) + 64 * c;
+          tc_ld32(src, o);
+          tc_ld32(src + 32, o + 32);
+          tc_wait_ld_regs(o);
+          tc_wait_ld_regs(o + 32);
+        }
+        const bool zero = total == 0 || r >= it.live;
+        if (lane == 0) bulk_wait_read0();  // the staging buffer is free
+        __syncwarp();
+        uint8_t* row = stage + lane * 128;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = zero ? 0.f : __uint_as_float(o[8 * e + i]) * f;
+          *reinterpret_cast<uint4*>(row + ((e ^ (lane & 7)) << 4)) =
+              make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
+        }
+        fence_proxy_async();
+        __syncwarp();
+        const int row0 = it.row + 32 * q;
+        if (wrows == 32) {
+          if (lane == 0) {
+            tma_store(map, stage, 64 * c, it.h, row0, 0);
+            bulk_commit();
+          }
+        } else {  // the rows behind the sequence are not ours
+          for (int e = lane; e < wrows * 8; e += 32) {
+            const int rr = e >> 3, piece = e & 7;
+            if (64 * c + 8 * piece < p.D)
+              *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(out.p)) + (int64_t)(row0 + rr) * out.t +
+                                        (int64_t)it.h * out.h + 64 * c + 8 * piece) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      }
+      if (total > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty);
+      }
+    }
+    // rows of no sequence: zeros
+    const int rows = KEYS ? p.pk.S : p.pk.T;
+    const int32_t* cu = KEYS ? p.pk.cu_k : p.pk.cu_q;
+    int lo = 0, hi = 0;
+    if (p.pk.B > 0) {
+      lo = segment(cu, 0, rows).x;
+      const int2 e = segment(cu, p.pk.B - 1, rows);
+      hi = max(lo, e.x + e.y);
+    }
+    const int64_t gap = (int64_t)lo + (rows - hi);
+    for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < gap * p.heads; i += (int64_t)gridDim.x * 8) {
+      const int64_t k = i / p.heads;
+      const int h = (int)(i - k * p.heads);
+      const int64_t row = k < lo ? k : hi + (k - lo);
+      for (int e = lane * 8; e < p.D; e += 256) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(p.out0.p)) + row * p.out0.t + (int64_t)h * p.out0.h + e) =
+            make_uint4(0, 0, 0, 0);
+        if (KEYS)
+          *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(p.out1.p)) + row * p.out1.t + (int64_t)h * p.out1.h + e) =
+              make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// delta = rowsum(dO O): eight lanes per row, 16 bytes each at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, float* delta, int T_, int Hq, int D) {
+  const int64_t item = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
+  const int l = threadIdx.x & 7;
+  float sum = 0.f;
+  const bool live = item < (int64_t)T_ * Hq;
+  const int64_t t = live ? item / Hq : 0;
+  const int h = live ? (int)(item - t * Hq) : 0;
+  if (live) {
+    const T* g = static_cast<const T*>(dout.p) + t * dout.t + (int64_t)h * dout.h;
+    const T* o = static_cast<const T*>(out.p) + t * out.t + (int64_t)h * out.h;
+    for (int c = l * 8; c < D; c += 64) {
+      const uint4 a = *reinterpret_cast<const uint4*>(g + c), b = *reinterpret_cast<const uint4*>(o + c);
+      const uint32_t ua[4] = {a.x, a.y, a.z, a.w}, ub[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = St<T>::unpack(ua[i]), y = St<T>::unpack(ub[i]);
+        sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (live && l == 0) delta[(int64_t)h * T_ + t] = sum;
+}
+
+template <typename T, int DP, bool KEYS>
+int launch(const Params& p, int dev, int grid, cudaStream_t s) {
+  static std::atomic<bool> configured[64] = {};
+  const int rc = opt_in_smem(gradient_kernel<T, DP, KEYS>, Cfg<DP>::kSmem, configured, dev);
+  if (rc != UPLIFT_LA_OK) return rc;
+  gradient_kernel<T, DP, KEYS><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(p);
+  return launched("attention backward");
+}
+
+template <typename T, bool KEYS>
+int launch_d(const Params& p, int dev, int grid, cudaStream_t s) {
+  return p.D <= 64 ? launch<T, 64, KEYS>(p, dev, grid, s) : launch<T, 128, KEYS>(p, dev, grid, s);
+}
+
+}  // namespace bwd
+
+int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
+  using namespace bwd;
+  int dev = 0, sms = 0;
+  int rc = sm_count(&dev, &sms);
+  if (rc != UPLIFT_LA_OK) return rc;
+  const int T = a.pk.T, S = a.pk.S;
+  const bool bf16 = a.dtype == UPLIFT_LA_BF16;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.lse = a.lse;
+  p.delta = a.delta;
+  p.pk = a.pk;
+  p.group = a.Hq / a.Hk;
+  p.D = a.D;
+  p.scale = a.scale;
+  p.timeout_ns = tc_test_timeout_ns() != 0 ? tc_test_timeout_ns() : kTimeoutNs;
+  p.host_status = host_status_word();
+  if (T > 0) {
+    const int64_t blocks = ((int64_t)T * a.Hq + 31) / 32;
+    if (blocks >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "attention backward: too many rows");
+    if (bf16) delta_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.delta, T, a.Hq, a.D);
+    else delta_kernel<__half><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.delta, T, a.Hq, a.D);
+    if ((rc = launched("attention backward")) != UPLIFT_LA_OK) return rc;
+    // queries stay; without keys no box is loaded and the maps stay empty
+    if ((rc = make_row_map(&p.x0, a.dtype, a.q, T, a.Hq, a.D, kM)) != UPLIFT_LA_OK) return rc;
+    if ((rc = make_row_map(&p.x1, a.dtype, a.dout, T, a.Hq, a.D, kM)) != UPLIFT_LA_OK) return rc;
+    if (S > 0) {
+      if ((rc = make_row_map(&p.y0, a.dtype, a.k, S, a.Hk, a.D, kN)) != UPLIFT_LA_OK) return rc;
+      if ((rc = make_row_map(&p.y1, a.dtype, a.v, S, a.Hk, a.D, kN)) != UPLIFT_LA_OK) return rc;
+    }
+    if ((rc = make_row_map(&p.o0, a.dtype, a.dq, T, a.Hq, a.D, 32)) != UPLIFT_LA_OK) return rc;
+    p.out0 = a.dq;
+    p.heads = a.Hq;
+    const int64_t most = ((int64_t)T / kM + a.pk.B) * a.Hq;
+    const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
+    rc = bf16 ? launch_d<__nv_bfloat16, false>(p, dev, grid, s) : launch_d<__half, false>(p, dev, grid, s);
+    if (rc != UPLIFT_LA_OK) return rc;
+  }
+  if (S > 0) {
+    if ((rc = make_row_map(&p.x0, a.dtype, a.k, S, a.Hk, a.D, kM)) != UPLIFT_LA_OK) return rc;
+    if ((rc = make_row_map(&p.x1, a.dtype, a.v, S, a.Hk, a.D, kM)) != UPLIFT_LA_OK) return rc;
+    if (T > 0) {
+      if ((rc = make_row_map(&p.y0, a.dtype, a.q, T, a.Hq, a.D, kN)) != UPLIFT_LA_OK) return rc;
+      if ((rc = make_row_map(&p.y1, a.dtype, a.dout, T, a.Hq, a.D, kN)) != UPLIFT_LA_OK) return rc;
+    }
+    if ((rc = make_row_map(&p.o0, a.dtype, a.dv, S, a.Hk, a.D, 32)) != UPLIFT_LA_OK) return rc;
+    if ((rc = make_row_map(&p.o1, a.dtype, a.dk, S, a.Hk, a.D, 32)) != UPLIFT_LA_OK) return rc;
+    p.out0 = a.dv;
+    p.out1 = a.dk;
+    p.heads = a.Hk;
+    const int64_t most = ((int64_t)S / kM + a.pk.B) * a.Hk;
+    const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
+    rc = bf16 ? launch_d<__nv_bfloat16, true>(p, dev, grid, s) : launch_d<__half, true>(p, dev, grid, s);
+  }
+  return rc;
+}
+
+int attn_bwd_device_status(bool clear) { return read_status(g_tok_bwd_status, clear); }
+
+}  // namespace tok
+}  // namespace ula

@@ -255,9 +255,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       // ---------------------------------------------------------- producer
       if (lane == 0) {
         prefetch_map(&p.qmap);
-        prefetch_map(&p.kmap);
-        prefetch_map(&p.vmap);
         prefetch_map(&p.omap);
+        if (p.pk.S > 0) {
+          prefetch_map(&p.kmap);
+          prefetch_map(&p.vmap);
+        }
       }
       TileWalk walk;
       bool ok = true;
@@ -664,19 +666,7 @@ int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
   return a.D <= 64 ? launch<__half, 64>(p, dev, grid, s) : launch<__half, 128>(p, dev, grid, s);
 }
 
-int attn_fwd_device_status(bool clear) {
-  unsigned int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_tok_fwd_status, sizeof(v));
-  if (e == cudaSuccess && clear && v != 0) {
-    const unsigned int zero = 0;
-    e = cudaMemcpyToSymbol(g_tok_fwd_status, &zero, sizeof(zero));
-  }
-  if (e != cudaSuccess) {
-    fail(UPLIFT_LA_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
-    return -1;
-  }
-  return (int)v;
-}
+int attn_fwd_device_status(bool clear) { return read_status(g_tok_fwd_status, clear); }
 
 }  // namespace tok
 }  // namespace ula

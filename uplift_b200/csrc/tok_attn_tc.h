@@ -25,6 +25,24 @@ __device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, uin
   tma_load(dst, map, bar, c, h, row, 0);
 }
 
+// Current device and its number of SMs.
+int sm_count(int* dev, int* sms);
+
+// Reads (and clears) a kernel's status word; -1 if that failed.
+inline int read_status(unsigned int& symbol, bool clear) {
+  unsigned int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, symbol, sizeof(v));
+  if (e == cudaSuccess && clear && v != 0) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbol(symbol, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) {
+    fail(UPLIFT_LA_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
+    return -1;
+  }
+  return (int)v;
+}
+
 // ------------------------------------------------------------ waits
 // mbar_wait_status of la_tc_common.h as inline code.
 __device__ __forceinline__ bool mbar_wait_inline(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
