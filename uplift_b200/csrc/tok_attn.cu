@@ -63,7 +63,9 @@ int tok_device_status(bool clear) {
 extern "C" {
 
 int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int Hk, int D, int dtype) {
-  return 0;
+  using namespace ula::tok;
+  if (T < 1 || Hk < 1 || Hq < Hk || D < 1 || !attn_step_applies(B, T, dtype)) return 0;
+  return attn_step_workspace(T, Hq, Hk, D);
 }
 
 int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], const void* k,
@@ -94,7 +96,13 @@ int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], cons
   a.pk = Packing{cu_q, cu_k, used_k, B, (int)T, (int)S, causal != 0};
   a.Hq = Hq; a.Hk = Hk; a.D = D; a.scale = scale; a.dtype = dtype;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == UPLIFT_LA_F32 ? attn_simt_forward(a, s) : attn_tc_forward(a, s);
+  if (dtype == UPLIFT_LA_F32) return attn_simt_forward(a, s);
+  if (!attn_step_applies(B, T, dtype)) return attn_tc_forward(a, s);
+  if (workspace == nullptr || workspace_bytes < attn_step_workspace(T, Hq, Hk, D) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what,
+                (long long)attn_step_workspace(T, Hq, Hk, D));
+  return attn_step_forward(a, workspace, s);
 }
 
 int uplift_tok_attention_backward(const void* dout, const int64_t dout_strides[2], const void* q,
