@@ -4,9 +4,8 @@
  * consumes, or any packed token sequences) and the per-head norm with
  * position rotation that feeds it.
  *
- * Token tensors are [rows, heads, D] with channel stride 1; `strides` gives
- * the row and head strides in elements (views into a fused projection
- * output work).  Sequences are packed: sequence b owns the rows
+ * Token tensors are [rows, heads, D] with channel stride 1, given as
+ * uplift_tok_rows: views into a fused projection output work.  Sequences are packed: sequence b owns the rows
  * cu[b] .. cu[b + 1] - 1 of its tensor; cu is a device array of B + 1
  * ascending int32 values.  Row numbers read from device arrays are clamped
  * to the tensors, so no content of these arrays makes a kernel leave them.
@@ -34,6 +33,12 @@ extern "C" {
 #define UPLIFT_TOK_MAX_NORM_DIM 256
 #define UPLIFT_TOK_MAX_ATTN_DIM 128
 
+/* A token tensor: first element, and the row and head strides in elements. */
+typedef struct {
+  void* data;
+  int64_t row, head;
+} uplift_tok_rows;
+
 /*
  * RMS norm of every query and key head and the position rotation, one pass:
  *
@@ -42,39 +47,33 @@ extern "C" {
  *
  * with c, s = cos, sin [positions[t]][i] for pair i: channels (i, i + R/2),
  * or (2i, 2i + 1) when interleaved; channels R .. D - 1 are not rotated.
- *
- *   q [T, Hq, D], k [T, Hk, D]; q_out, k_out the same shapes, not overlapping
- *   q_weight, k_weight [D] of weight_dtype, or NULL (ones)
- *   cos, sin  [P, R / 2] fp32, contiguous
- *   positions [T] int32 or int64 (positions64 = 1), or NULL: row t of the
- *             table for token t (then P >= T).  A negative position leaves
- *             the token unrotated (class and register tokens); a position
- *             >= P makes the token's rotated outputs and its gradients NaN.
- *   D <= UPLIFT_TOK_MAX_NORM_DIM; R even, 0 <= R <= D
  */
-int uplift_tok_norm_rotate(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
-                           const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
-                           const void* q_weight, const void* k_weight, int weight_dtype,
-                           const float* cos, const float* sin, const void* positions, int positions64,
-                           int64_t T, int64_t P, int Hq, int Hk, int D, int R, float eps, int interleaved,
-                           int dtype, void* stream);
+typedef struct {
+  int64_t size;               /* sizeof(uplift_tok_norm_rotate_args) */
+  uplift_tok_rows q, k;       /* [T, Hq, D], [T, Hk, D] */
+  uplift_tok_rows q_out, k_out; /* the outputs (not overlapping the inputs); backward: their gradients */
+  uplift_tok_rows dq, dk;     /* backward only: gradients of q and k */
+  const void* q_weight;       /* [D] of weight_dtype, or NULL: ones */
+  const void* k_weight;
+  const float* cos;           /* [P, R / 2], contiguous */
+  const float* sin;
+  const void* positions;      /* [T] int32, or int64 (positions64), or NULL: row t of the table for token t (P >= T).
+                                 Negative: the token is not rotated (class and register tokens).  >= P: its rotated
+                                 outputs and its gradients are NaN. */
+  float* dweights;            /* backward only: gradients of q_weight and k_weight, [2][D], written; or NULL */
+  float* partial;             /* backward only: workspace of uplift_tok_norm_rotate_partial_floats(D) floats */
+  int64_t T, P;
+  int32_t Hq, Hk;
+  int32_t D, R;               /* D <= UPLIFT_TOK_MAX_NORM_DIM; R even, 0 <= R <= D */
+  float eps;
+  int32_t interleaved, weight_dtype, positions64, dtype;
+  int32_t reserved;           /* 0 */
+} uplift_tok_norm_rotate_args;
 
-/*
- * Gradients of uplift_tok_norm_rotate: dq, dk from dq_out, dk_out (rows of
- * the forward's outputs) and the forward's inputs, and dweights: the
- * gradients of q_weight and k_weight, [2][D] fp32 (written, not added to).
- * partial: workspace of uplift_tok_norm_rotate_partial_floats(D) floats.
- */
+int uplift_tok_norm_rotate(const uplift_tok_norm_rotate_args* args, void* stream);
+/* The gradients dq, dk and dweights from the inputs and the outputs' gradients. */
+int uplift_tok_norm_rotate_backward(const uplift_tok_norm_rotate_args* args, void* stream);
 int64_t uplift_tok_norm_rotate_partial_floats(int D);
-int uplift_tok_norm_rotate_backward(const void* dq_out, const int64_t dq_out_strides[2],
-                                    const void* dk_out, const int64_t dk_out_strides[2],
-                                    const void* q, const int64_t q_strides[2], const void* k,
-                                    const int64_t k_strides[2], void* dq, const int64_t dq_strides[2],
-                                    void* dk, const int64_t dk_strides[2], float* dweights,
-                                    const void* q_weight, const void* k_weight, int weight_dtype,
-                                    const float* cos, const float* sin, const void* positions, int positions64,
-                                    float* partial, int64_t T, int64_t P, int Hq, int Hk, int D, int R, float eps,
-                                    int interleaved, int dtype, void* stream);
 
 /*
  * Attention over packed sequences with grouped heads.  Sequence b has the
@@ -90,36 +89,37 @@ int uplift_tok_norm_rotate_backward(const void* dq_out, const int64_t dq_out_str
  * no sequence.  What keys that a query does not see hold (NaN, infinities)
  * does not reach its output.
  *
- *   q, out [T, Hq, D]; k, v [S, Hk, D]; lse [Hq, T] fp32 or NULL
- *   used_k [B] int32 or NULL; Hq a multiple of Hk; D <= UPLIFT_TOK_MAX_ATTN_DIM
- *   scale  positive and finite
- *   workspace: uplift_tok_attention_workspace(...) bytes, 16-byte aligned
- *             (may be 0 / NULL)
- * bf16 / fp16: D a multiple of 8; pointers 16-byte aligned, strides
+ * bf16 / fp16: D a multiple of 8; tensors 16-byte aligned, strides
  * multiples of 8 elements and row strides multiples of the head stride
  * (UPLIFT_LA_ERR_LAYOUT otherwise).
  */
-int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int Hk, int D, int dtype);
-int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], const void* k,
-                                 const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
-                                 void* out, const int64_t out_strides[2], float* lse,
-                                 const int32_t* cu_q, const int32_t* cu_k, const int32_t* used_k,
-                                 int B, int64_t T, int64_t S, int Hq, int Hk, int D, float scale, int causal,
-                                 int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct {
+  int64_t size;             /* sizeof(uplift_tok_attention_args) */
+  uplift_tok_rows q;        /* [T, Hq, D] */
+  uplift_tok_rows k, v;     /* [S, Hk, D] */
+  uplift_tok_rows out;      /* [T, Hq, D] */
+  uplift_tok_rows dout;     /* backward only: gradient of out */
+  uplift_tok_rows dq, dk, dv; /* backward only: the gradients, written whole: zero for rows of no sequence and keys that
+                                 no query sees */
+  float* lse;               /* [Hq, T]; forward: written unless NULL; backward: read */
+  float* delta;             /* backward only: workspace of T * Hq floats */
+  const int32_t* cu_q;      /* [B + 1] */
+  const int32_t* cu_k;
+  const int32_t* used_k;    /* [B] or NULL */
+  void* workspace;          /* forward only: uplift_tok_attention_workspace(...) bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t T, S;
+  int32_t B, Hq, Hk;        /* Hq a multiple of Hk */
+  int32_t D;                /* <= UPLIFT_TOK_MAX_ATTN_DIM */
+  float scale;              /* positive and finite */
+  int32_t causal, dtype;
+  int32_t reserved;         /* 0 */
+} uplift_tok_attention_args;
 
-/*
- * Gradients of uplift_tok_attention_forward from dout, its inputs, out and
- * lse.  dq, dk, dv are written whole: zero for rows of no sequence and keys
- * that no query sees.  delta: workspace of T * Hq floats.
- */
-int uplift_tok_attention_backward(const void* dout, const int64_t dout_strides[2], const void* q,
-                                  const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
-                                  const void* v, const int64_t v_strides[2], const void* out,
-                                  const int64_t out_strides[2], const float* lse, void* dq,
-                                  const int64_t dq_strides[2], void* dk, const int64_t dk_strides[2], void* dv,
-                                  const int64_t dv_strides[2], float* delta, const int32_t* cu_q,
-                                  const int32_t* cu_k, const int32_t* used_k, int B, int64_t T, int64_t S, int Hq,
-                                  int Hk, int D, float scale, int causal, int dtype, void* stream);
+int uplift_tok_attention_forward(const uplift_tok_attention_args* args, void* stream);
+/* The gradients dq, dk and dv from the inputs, out, lse and dout. */
+int uplift_tok_attention_backward(const uplift_tok_attention_args* args, void* stream);
+int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int Hk, int D, int dtype);
 
 #ifdef __cplusplus
 }

@@ -1,12 +1,10 @@
 """Refusals of the token-sequence operators, and their 64-bit restatements
 against differences: no GPU."""
-import ctypes
-
 import pytest
 import torch
 
 import tokens_reference as R
-from uplift_b200 import _native, ops
+from uplift_b200 import _native, ops, tokens
 
 
 @pytest.fixture(scope="module")
@@ -14,36 +12,36 @@ def lib():
     return _native.load(build_if_missing=True)
 
 
-S2 = ctypes.c_int64 * 2
+def _attn_args(kw):
+    a = dict(q=16, k=16, v=16, out=16, dout=16, dq=16, dk=16, dv=16, st=(128, 64), lse=16, delta=16, cu=16, ws=0,
+             ws_bytes=0, B=1, T=40, S=4, Hq=2, Hk=1, D=64, scale=0.125, causal=1, dtype=_native.BF16,
+             size=tokens._PA_ARGS.size)
+    a.update(kw)
+    rows = [x for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv") for x in (a[n], *a["st"])]
+    return tokens._PA_ARGS.pack(a["size"], *rows, a["lse"], a["delta"], a["cu"], a["cu"], 0, a["ws"], a["ws_bytes"],
+                                a["T"], a["S"], a["B"], a["Hq"], a["Hk"], a["D"], a["scale"], a["causal"], a["dtype"],
+                                0)
 
 
 def _attn(lib, **kw):
-    a = dict(q=16, k=16, v=16, out=16, st=S2(128, 64), lse=None, cu=16, B=1, T=4, S=4, Hq=2, Hk=1, D=64, scale=0.125,
-             causal=1, dtype=_native.BF16)
-    a.update(kw)
-    return lib.uplift_tok_attention_forward(
-        a["q"], a["st"], a["k"], a.get("kst", a["st"]), a["v"], a["st"], a["out"], a["st"], a["lse"], a["cu"], a["cu"],
-        None, a["B"], a["T"], a["S"], a["Hq"], a["Hk"], a["D"], a["scale"], a["causal"], a["dtype"], None, 0, None)
+    return lib.uplift_tok_attention_forward(_attn_args(kw), None)
 
 
 def _attn_bwd(lib, **kw):
-    a = dict(p=16, st=S2(128, 64), lse=16, delta=16, cu=16, B=1, T=4, S=4, Hq=2, Hk=1, D=64, scale=0.125,
-             dtype=_native.BF16)
+    return lib.uplift_tok_attention_backward(_attn_args(kw), None)
+
+
+def _nr_args(kw):
+    a = dict(q=16, k=16, qo=16, ko=16, dq=16, dk=16, st=(128, 64), wt=0, cos=16, pos=0, dw=0, partial=0, T=4, P=8,
+             Hq=2, Hk=1, D=64, R=64, eps=1e-6, dtype=1, size=tokens._NR_ARGS.size)
     a.update(kw)
-    rows = []
-    for name in ("dout", "q", "k", "v", "out"):
-        rows += [a.get(name, a["p"]), a["st"]]
-    return lib.uplift_tok_attention_backward(
-        *rows, a["lse"], a["p"], a["st"], a["p"], a["st"], a["p"], a["st"], a["delta"], a["cu"], a["cu"], None, a["B"],
-        a["T"], a["S"], a["Hq"], a["Hk"], a["D"], a["scale"], 1, a["dtype"], None)
+    rows = [x for n in ("q", "k", "qo", "ko", "dq", "dk") for x in (a[n], *a["st"])]
+    return tokens._NR_ARGS.pack(a["size"], *rows, 0, 0, a["cos"], a["cos"], a["pos"], a["dw"], a["partial"], a["T"],
+                                a["P"], a["Hq"], a["Hk"], a["D"], a["R"], a["eps"], 0, a["wt"], 0, a["dtype"], 0)
 
 
 def _nr(lib, **kw):
-    a = dict(q=16, k=16, st=S2(128, 64), wt=0, cos=16, pos=None, T=4, P=8, Hq=2, Hk=1, D=64, R=64, eps=1e-6, dtype=1)
-    a.update(kw)
-    return lib.uplift_tok_norm_rotate(a["q"], a["st"], a["q"], a["st"], a["k"], a["st"], a["k"], a["st"], None, None,
-                                      a["wt"], a["cos"], a["cos"], a["pos"], 0, a["T"], a["P"], a["Hq"], a["Hk"],
-                                      a["D"], a["R"], a["eps"], 0, a["dtype"], None)
+    return lib.uplift_tok_norm_rotate(_nr_args(kw), None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -51,9 +49,9 @@ def _nr(lib, **kw):
     (dict(D=136), "ERR_SHAPE"), (dict(D=60), "ERR_SHAPE"), (dict(B=-1), "ERR_SHAPE"), (dict(T=-1), "ERR_SHAPE"),
     (dict(T=1 << 31), "ERR_SHAPE"), (dict(S=1 << 31), "ERR_SHAPE"), (dict(scale=0.0), "ERR_ARG"),
     (dict(scale=-1.0), "ERR_ARG"), (dict(scale=float("nan")), "ERR_ARG"), (dict(scale=float("inf")), "ERR_ARG"),
-    (dict(q=None), "ERR_ARG"), (dict(out=None), "ERR_ARG"), (dict(cu=None), "ERR_ARG"), (dict(q=8), "ERR_LAYOUT"),
-    (dict(st=S2(132, 64)), "ERR_LAYOUT"), (dict(st=S2(128, 4)), "ERR_LAYOUT"), (dict(st=S2(0, 64)), "ERR_LAYOUT"),
-    (dict(st=None), "ERR_ARG"),
+    (dict(q=0), "ERR_ARG"), (dict(out=0), "ERR_ARG"), (dict(cu=0), "ERR_ARG"), (dict(q=8), "ERR_LAYOUT"),
+    (dict(st=(132, 64)), "ERR_LAYOUT"), (dict(st=(128, 4)), "ERR_LAYOUT"), (dict(st=(0, 64)), "ERR_LAYOUT"),
+    (dict(size=8), "ERR_ARG"),
 ])
 def test_attention_entry_refuses(lib, kw, code):
     assert _attn(lib, **kw) == getattr(_native, code)
@@ -61,9 +59,9 @@ def test_attention_entry_refuses(lib, kw, code):
 
 
 @pytest.mark.parametrize("kw,code", [
-    (dict(dtype=-1), "ERR_ARG"), (dict(lse=None), "ERR_ARG"), (dict(delta=None), "ERR_ARG"),
-    (dict(dout=None), "ERR_ARG"), (dict(out=None), "ERR_ARG"), (dict(v=24), "ERR_LAYOUT"),
-    (dict(D=129), "ERR_SHAPE"), (dict(Hq=5, Hk=2), "ERR_SHAPE"), (dict(cu=None), "ERR_ARG"),
+    (dict(dtype=-1), "ERR_ARG"), (dict(lse=0), "ERR_ARG"), (dict(delta=0), "ERR_ARG"),
+    (dict(dout=0), "ERR_ARG"), (dict(out=0), "ERR_ARG"), (dict(v=24), "ERR_LAYOUT"),
+    (dict(D=129), "ERR_SHAPE"), (dict(Hq=5, Hk=2), "ERR_SHAPE"), (dict(cu=0), "ERR_ARG"),
 ])
 def test_attention_backward_entry_refuses(lib, kw, code):
     assert _attn_bwd(lib, **kw) == getattr(_native, code)
@@ -73,16 +71,34 @@ def test_attention_backward_entry_refuses(lib, kw, code):
     (dict(dtype=9), "ERR_ARG"), (dict(wt=9), "ERR_ARG"), (dict(D=257), "ERR_SHAPE"), (dict(D=0), "ERR_SHAPE"),
     (dict(R=63), "ERR_SHAPE"), (dict(R=66), "ERR_SHAPE"), (dict(R=-2), "ERR_SHAPE"), (dict(P=3), "ERR_SHAPE"),
     (dict(Hq=0), "ERR_SHAPE"), (dict(T=-1), "ERR_SHAPE"), (dict(eps=-1.0), "ERR_ARG"),
-    (dict(eps=float("nan")), "ERR_ARG"), (dict(q=None), "ERR_ARG"), (dict(cos=None), "ERR_ARG"),
-    (dict(st=None), "ERR_ARG"),
+    (dict(eps=float("nan")), "ERR_ARG"), (dict(q=0), "ERR_ARG"), (dict(cos=0), "ERR_ARG"),
+    (dict(size=8), "ERR_ARG"),
 ])
 def test_norm_rotate_entry_refuses(lib, kw, code):
     assert _nr(lib, **kw) == getattr(_native, code)
+    assert lib.uplift_tok_norm_rotate_backward(_nr_args(kw), None) == getattr(_native, code)
+
+
+def test_no_arguments_at_all(lib):
+    for name in ("norm_rotate", "norm_rotate_backward", "attention_forward", "attention_backward"):
+        assert getattr(lib, "uplift_tok_" + name)(None, None) == _native.ERR_ARG
+
+
+def test_backward_and_step_workspaces(lib):
+    assert lib.uplift_tok_norm_rotate_backward(_nr_args(dict(dw=16)), None) == _native.ERR_ARG
+    assert lib.uplift_tok_norm_rotate_backward(_nr_args(dict(dq=0)), None) == _native.ERR_ARG
+    need = lib.uplift_tok_attention_workspace(4, 4, 100, 8, 2, 64, _native.BF16)
+    assert need > 0 and lib.uplift_tok_attention_workspace(4, 4, 100, 8, 2, 64, _native.F32) == 0
+    step = dict(B=4, T=4, S=100, Hq=8, Hk=2, st=(512, 64))
+    assert _attn(lib, **step) == _native.ERR_ARG
+    assert _attn(lib, ws=16, ws_bytes=need - 1, **step) == _native.ERR_ARG
+    assert _attn(lib, ws=24, ws_bytes=need, **step) == _native.ERR_ARG
 
 
 def test_empty_calls_touch_no_device(lib):
     assert _attn(lib, T=0) == _native.OK
     assert _attn_bwd(lib, T=0, S=0) == _native.OK
+    assert _attn_bwd(lib, T=0, S=0, B=0, cu=0) == _native.OK
     assert _nr(lib, T=0) == _native.OK
     assert lib.uplift_tok_norm_rotate_partial_floats(64) > 0
 

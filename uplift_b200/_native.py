@@ -133,23 +133,16 @@ def load(build_if_missing: bool = False):
         lib.uplift_bias_act.argtypes = [vp, i64p, vp, vp, i64p, i, i, i, i, i, i, i, vp]
         lib.uplift_layernorm_act.restype = i
         lib.uplift_layernorm_act.argtypes = [vp, i64p, vp, vp, vp, ctypes.c_float, i, i, i, i, i, i, vp]
-        i64, f = ctypes.c_int64, ctypes.c_float
-        rows = [vp, i64p]
-        lib.uplift_tok_norm_rotate.restype = i
-        lib.uplift_tok_norm_rotate.argtypes = rows * 4 + [vp, vp, i, vp, vp, vp, i, i64, i64, i, i, i, i, f, i, i, vp]
+        # include/uplift_tokens.h: arguments in one struct, built with struct.pack (tokens.py)
+        i64 = ctypes.c_int64
+        for name in ("norm_rotate", "norm_rotate_backward", "attention_forward", "attention_backward"):
+            fn = getattr(lib, "uplift_tok_" + name)
+            fn.restype = i
+            fn.argtypes = [ctypes.c_char_p, vp]
         lib.uplift_tok_norm_rotate_partial_floats.restype = i64
         lib.uplift_tok_norm_rotate_partial_floats.argtypes = [i]
-        lib.uplift_tok_norm_rotate_backward.restype = i
-        lib.uplift_tok_norm_rotate_backward.argtypes = rows * 6 + [vp, vp, vp, i, vp, vp, vp, i, vp, i64, i64,
-                                                                   i, i, i, i, f, i, i, vp]
         lib.uplift_tok_attention_workspace.restype = i64
         lib.uplift_tok_attention_workspace.argtypes = [i, i64, i64, i, i, i, i]
-        lib.uplift_tok_attention_forward.restype = i
-        lib.uplift_tok_attention_forward.argtypes = rows * 4 + [vp, vp, vp, vp, i, i64, i64, i, i, i, f, i, i, vp, i64,
-                                                                vp]
-        lib.uplift_tok_attention_backward.restype = i
-        lib.uplift_tok_attention_backward.argtypes = rows * 5 + [vp] + rows * 3 + [vp, vp, vp, vp, i, i64, i64, i, i, i,
-                                                                                   f, i, i, vp]
         _lib = lib
     return _lib
 

@@ -11,20 +11,24 @@ namespace ula {
 namespace tok {
 namespace {
 
-int check_sizes(const char* what, int B, int64_t T, int64_t S, int Hq, int Hk, int D, float scale, int dtype) {
-  if (dtype != UPLIFT_LA_F32 && dtype != UPLIFT_LA_BF16 && dtype != UPLIFT_LA_F16)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+int check_sizes(const char* what, const uplift_tok_attention_args* a) {
+  if (a == nullptr || a->size != (int64_t)sizeof(*a)) return fail(UPLIFT_LA_ERR_ARG, "%s: no arguments, or of another version", what);
+  if (a->dtype != UPLIFT_LA_F32 && a->dtype != UPLIFT_LA_BF16 && a->dtype != UPLIFT_LA_F16)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, a->dtype);
   // the row limit leaves room for tile arithmetic in 32 bits
-  if (B < 0 || T < 0 || S < 0 || T >= (1ll << 31) - 65536 || S >= (1ll << 31) - 65536 || Hq < 1 || Hk < 1 || Hq > 65536)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes B=%d T=%lld S=%lld Hq=%d Hk=%d", what, B, (long long)T,
-                (long long)S, Hq, Hk);
-  if (Hq % Hk != 0)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %d query heads are not a multiple of %d key heads", what, Hq, Hk);
-  if (D < 1 || D > UPLIFT_TOK_MAX_ATTN_DIM)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: head dimension %d not in 1..%d", what, D, UPLIFT_TOK_MAX_ATTN_DIM);
-  if (dtype != UPLIFT_LA_F32 && D % 8 != 0)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: 16-bit tensors need a head dimension that is a multiple of 8 (got %d)", what, D);
-  if (!(scale > 0.f) || isinf(scale)) return fail(UPLIFT_LA_ERR_ARG, "%s: scale must be positive and finite", what);
+  constexpr int64_t kMaxRows = (1ll << 31) - 65536;
+  if (a->B < 0 || a->T < 0 || a->S < 0 || a->T >= kMaxRows || a->S >= kMaxRows || a->Hq < 1 || a->Hk < 1 || a->Hq > 65536)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes B=%d T=%lld S=%lld Hq=%d Hk=%d", what, a->B, (long long)a->T,
+                (long long)a->S, a->Hq, a->Hk);
+  if (a->Hq % a->Hk != 0)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %d query heads are not a multiple of %d key heads", what, a->Hq, a->Hk);
+  if (a->D < 1 || a->D > UPLIFT_TOK_MAX_ATTN_DIM)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: head dimension %d not in 1..%d", what, a->D, UPLIFT_TOK_MAX_ATTN_DIM);
+  if (a->dtype != UPLIFT_LA_F32 && a->D % 8 != 0)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: 16-bit tensors need a head dimension that is a multiple of 8 (got %d)", what, a->D);
+  if (!(a->scale > 0.f) || isinf(a->scale)) return fail(UPLIFT_LA_ERR_ARG, "%s: scale must be positive and finite", what);
+  if (a->B > 0 && (a->T > 0 || a->S > 0) && (a->cu_q == nullptr || a->cu_k == nullptr))
+    return fail(UPLIFT_LA_ERR_ARG, "%s: null sequence starts", what);
   return UPLIFT_LA_OK;
 }
 
@@ -43,11 +47,36 @@ int check_rows(const char* what, const char* name, const Rows& r, int64_t rows, 
 
 // Strides of axes of one entry do not matter: give them values that do not
 // trouble the tensor maps.
-Rows rows_of(const void* p, const int64_t* st, int64_t rows, int heads, int D) {
-  Rows r{p, st[0], st[1]};
+Rows rows_of(const uplift_tok_rows& t, int64_t rows, int heads, int D) {
+  Rows r{t.data, t.row, t.head};
   if (heads == 1) r.h = (D + 7) / 8 * 8;
   if (rows <= 1) r.t = (int64_t)r.h * heads;
   return r;
+}
+
+int prepare(const char* what, const uplift_tok_attention_args* in, bool bwd, AttnArgs* a) {
+  int rc = check_sizes(what, in);
+  if (rc != UPLIFT_LA_OK) return rc;
+  *a = AttnArgs{};
+  const struct { const char* name; const uplift_tok_rows* in; Rows* r; bool keys, used; } all[] = {
+      {"q", &in->q, &a->q, false, true},        {"k", &in->k, &a->k, true, true},
+      {"v", &in->v, &a->v, true, true},         {"out", &in->out, &a->out, false, true},
+      {"dout", &in->dout, &a->dout, false, bwd}, {"dq", &in->dq, &a->dq, false, bwd},
+      {"dk", &in->dk, &a->dk, true, bwd},       {"dv", &in->dv, &a->dv, true, bwd}};
+  for (const auto& e : all) {
+    if (!e.used) continue;
+    const int64_t rows = e.keys ? in->S : in->T;
+    const int heads = e.keys ? in->Hk : in->Hq;
+    *e.r = rows_of(*e.in, rows, heads, in->D);
+    if ((rc = check_rows(what, e.name, *e.r, rows, heads, in->dtype)) != UPLIFT_LA_OK) return rc;
+  }
+  if (bwd && in->T > 0 && (in->lse == nullptr || in->delta == nullptr))
+    return fail(UPLIFT_LA_ERR_ARG, "%s: null lse or delta", what);
+  a->lse = in->lse;
+  a->delta = in->delta;
+  a->pk = Packing{in->cu_q, in->cu_k, in->used_k, in->B, (int)in->T, (int)in->S, in->causal != 0};
+  a->Hq = in->Hq; a->Hk = in->Hk; a->D = in->D; a->scale = in->scale; a->dtype = in->dtype;
+  return UPLIFT_LA_OK;
 }
 
 }  // namespace
@@ -68,82 +97,30 @@ int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int 
   return attn_step_workspace(T, Hq, Hk, D);
 }
 
-int uplift_tok_attention_forward(const void* q, const int64_t q_strides[2], const void* k,
-                                 const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
-                                 void* out, const int64_t out_strides[2], float* lse,
-                                 const int32_t* cu_q, const int32_t* cu_k, const int32_t* used_k,
-                                 int B, int64_t T, int64_t S, int Hq, int Hk, int D, float scale, int causal,
-                                 int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+int uplift_tok_attention_forward(const uplift_tok_attention_args* args, void* stream) {
   using namespace ula;
   using namespace ula::tok;
   const char* what = "uplift_tok_attention_forward";
-  int rc = check_sizes(what, B, T, S, Hq, Hk, D, scale, dtype);
-  if (rc != UPLIFT_LA_OK) return rc;
-  if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || out_strides == nullptr)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: null strides", what);
-  if (T == 0) return UPLIFT_LA_OK;
-  if (B > 0 && (cu_q == nullptr || cu_k == nullptr)) return fail(UPLIFT_LA_ERR_ARG, "%s: null sequence starts", what);
-  AttnArgs a = {};
-  a.q = rows_of(q, q_strides, T, Hq, D);
-  a.k = rows_of(k, k_strides, S, Hk, D);
-  a.v = rows_of(v, v_strides, S, Hk, D);
-  a.out = rows_of(out, out_strides, T, Hq, D);
-  if ((rc = check_rows(what, "q", a.q, T, Hq, dtype)) != UPLIFT_LA_OK) return rc;
-  if ((rc = check_rows(what, "k", a.k, S, Hk, dtype)) != UPLIFT_LA_OK) return rc;
-  if ((rc = check_rows(what, "v", a.v, S, Hk, dtype)) != UPLIFT_LA_OK) return rc;
-  if ((rc = check_rows(what, "out", a.out, T, Hq, dtype)) != UPLIFT_LA_OK) return rc;
-  a.lse = lse;
-  a.pk = Packing{cu_q, cu_k, used_k, B, (int)T, (int)S, causal != 0};
-  a.Hq = Hq; a.Hk = Hk; a.D = D; a.scale = scale; a.dtype = dtype;
+  AttnArgs a;
+  const int rc = prepare(what, args, false, &a);
+  if (rc != UPLIFT_LA_OK || args->T == 0) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == UPLIFT_LA_F32) return attn_simt_forward(a, s);
-  if (!attn_step_applies(B, T, dtype)) return attn_tc_forward(a, s);
-  if (workspace == nullptr || workspace_bytes < attn_step_workspace(T, Hq, Hk, D) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what,
-                (long long)attn_step_workspace(T, Hq, Hk, D));
-  return attn_step_forward(a, workspace, s);
+  if (a.dtype == UPLIFT_LA_F32) return attn_simt_forward(a, s);
+  if (!attn_step_applies(a.pk.B, a.pk.T, a.dtype)) return attn_tc_forward(a, s);
+  const int64_t need = attn_step_workspace(a.pk.T, a.Hq, a.Hk, a.D);
+  if (args->workspace == nullptr || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15u) != 0)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
+  return attn_step_forward(a, args->workspace, s);
 }
 
-int uplift_tok_attention_backward(const void* dout, const int64_t dout_strides[2], const void* q,
-                                  const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
-                                  const void* v, const int64_t v_strides[2], const void* out,
-                                  const int64_t out_strides[2], const float* lse, void* dq,
-                                  const int64_t dq_strides[2], void* dk, const int64_t dk_strides[2], void* dv,
-                                  const int64_t dv_strides[2], float* delta, const int32_t* cu_q,
-                                  const int32_t* cu_k, const int32_t* used_k, int B, int64_t T, int64_t S, int Hq,
-                                  int Hk, int D, float scale, int causal, int dtype, void* stream) {
+int uplift_tok_attention_backward(const uplift_tok_attention_args* args, void* stream) {
   using namespace ula;
   using namespace ula::tok;
-  const char* what = "uplift_tok_attention_backward";
-  int rc = check_sizes(what, B, T, S, Hq, Hk, D, scale, dtype);
-  if (rc != UPLIFT_LA_OK) return rc;
-  if (dout_strides == nullptr || q_strides == nullptr || k_strides == nullptr || v_strides == nullptr ||
-      out_strides == nullptr || dq_strides == nullptr || dk_strides == nullptr || dv_strides == nullptr)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: null strides", what);
-  if (T == 0 && S == 0) return UPLIFT_LA_OK;
-  if (B > 0 && (cu_q == nullptr || cu_k == nullptr)) return fail(UPLIFT_LA_ERR_ARG, "%s: null sequence starts", what);
-  if (T > 0 && (lse == nullptr || delta == nullptr)) return fail(UPLIFT_LA_ERR_ARG, "%s: null lse or delta", what);
-  AttnArgs a = {};
-  a.q = rows_of(q, q_strides, T, Hq, D);
-  a.k = rows_of(k, k_strides, S, Hk, D);
-  a.v = rows_of(v, v_strides, S, Hk, D);
-  a.out = rows_of(out, out_strides, T, Hq, D);
-  a.dout = rows_of(dout, dout_strides, T, Hq, D);
-  a.dq = rows_of(dq, dq_strides, T, Hq, D);
-  a.dk = rows_of(dk, dk_strides, S, Hk, D);
-  a.dv = rows_of(dv, dv_strides, S, Hk, D);
-  const struct { const char* name; const Rows* r; int64_t rows; int heads; } all[] = {
-      {"q", &a.q, T, Hq}, {"k", &a.k, S, Hk}, {"v", &a.v, S, Hk}, {"out", &a.out, T, Hq},
-      {"dout", &a.dout, T, Hq}, {"dq", &a.dq, T, Hq}, {"dk", &a.dk, S, Hk}, {"dv", &a.dv, S, Hk}};
-  for (const auto& e : all)
-    if ((rc = check_rows(what, e.name, *e.r, e.rows, e.heads, dtype)) != UPLIFT_LA_OK) return rc;
-  a.lse = const_cast<float*>(lse);
-  a.delta = delta;
-  a.pk = Packing{cu_q, cu_k, used_k, B, (int)T, (int)S, causal != 0};
-  a.Hq = Hq; a.Hk = Hk; a.D = D; a.scale = scale; a.dtype = dtype;
+  AttnArgs a;
+  const int rc = prepare("uplift_tok_attention_backward", args, true, &a);
+  if (rc != UPLIFT_LA_OK || (args->T == 0 && args->S == 0)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == UPLIFT_LA_F32 ? attn_simt_backward(a, s) : attn_tc_backward(a, s);
+  return a.dtype == UPLIFT_LA_F32 ? attn_simt_backward(a, s) : attn_tc_backward(a, s);
 }
 
 }  // extern "C"

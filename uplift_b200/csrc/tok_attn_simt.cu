@@ -267,17 +267,8 @@ int backward(const AttnArgs& a, cudaStream_t s) {
 
 }  // namespace simt
 
-int attn_simt_forward(const AttnArgs& a, cudaStream_t s) {
-  if (a.dtype == UPLIFT_LA_F32) return simt::forward<float>(a, s);
-  if (a.dtype == UPLIFT_LA_BF16) return simt::forward<__nv_bfloat16>(a, s);
-  return simt::forward<__half>(a, s);
-}
-
-int attn_simt_backward(const AttnArgs& a, cudaStream_t s) {
-  if (a.dtype == UPLIFT_LA_F32) return simt::backward<float>(a, s);
-  if (a.dtype == UPLIFT_LA_BF16) return simt::backward<__nv_bfloat16>(a, s);
-  return simt::backward<__half>(a, s);
-}
+int attn_simt_forward(const AttnArgs& a, cudaStream_t s) { return simt::forward<float>(a, s); }
+int attn_simt_backward(const AttnArgs& a, cudaStream_t s) { return simt::backward<float>(a, s); }
 
 }  // namespace tok
 }  // namespace ula

@@ -516,23 +516,55 @@ int run(Args a, bool inter, bool bwd, cudaStream_t s) {
   return bwd ? -blocks : UPLIFT_LA_OK;
 }
 
-int check(const char* what, Args* a, int Hq, int Hk, int R, float eps, int wtype, int dtype) {
-  if (dtype != UPLIFT_LA_F32 && dtype != UPLIFT_LA_BF16 && dtype != UPLIFT_LA_F16)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, dtype);
-  if (wtype != UPLIFT_LA_F32 && wtype != UPLIFT_LA_BF16 && wtype != UPLIFT_LA_F16)
-    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown weight dtype %d", what, wtype);
-  if (a->T < 0 || a->T >= (1ll << 31) || a->P < 0 || Hq < 1 || Hk < 1 || Hq > 65536 || Hk > 65536)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes T=%lld P=%lld Hq=%d Hk=%d", what, (long long)a->T,
-                (long long)a->P, Hq, Hk);
-  if (a->D < 1 || a->D > UPLIFT_TOK_MAX_NORM_DIM)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: head dimension %d not in 1..%d", what, a->D, UPLIFT_TOK_MAX_NORM_DIM);
-  if (R < 0 || R > a->D || R % 2 != 0)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %d rotated channels (even, at most D = %d)", what, R, a->D);
-  if (!(eps >= 0.f) || isinf(eps)) return fail(UPLIFT_LA_ERR_ARG, "%s: eps must be finite and not negative", what);
-  if (a->pos == nullptr && R > 0 && a->P < a->T)
-    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %lld table rows for %lld tokens without positions", what, (long long)a->P,
-                (long long)a->T);
+// Validates the arguments and fills `a`.
+int prepare(const char* what, const uplift_tok_norm_rotate_args* in, bool bwd, Args* a) {
+  if (in == nullptr || in->size != (int64_t)sizeof(*in)) return fail(UPLIFT_LA_ERR_ARG, "%s: no arguments, or of another version", what);
+  const int dt = in->dtype, wt = in->weight_dtype;
+  if (dt != UPLIFT_LA_F32 && dt != UPLIFT_LA_BF16 && dt != UPLIFT_LA_F16)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, dt);
+  if (wt != UPLIFT_LA_F32 && wt != UPLIFT_LA_BF16 && wt != UPLIFT_LA_F16)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: unknown weight dtype %d", what, wt);
+  if (in->T < 0 || in->T >= (1ll << 31) || in->P < 0 || in->Hq < 1 || in->Hk < 1 || in->Hq > 65536 || in->Hk > 65536)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes T=%lld P=%lld Hq=%d Hk=%d", what, (long long)in->T,
+                (long long)in->P, in->Hq, in->Hk);
+  if (in->D < 1 || in->D > UPLIFT_TOK_MAX_NORM_DIM)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: head dimension %d not in 1..%d", what, in->D, UPLIFT_TOK_MAX_NORM_DIM);
+  if (in->R < 0 || in->R > in->D || in->R % 2 != 0)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %d rotated channels (even, at most D = %d)", what, in->R, in->D);
+  if (!(in->eps >= 0.f) || isinf(in->eps)) return fail(UPLIFT_LA_ERR_ARG, "%s: eps must be finite and not negative", what);
+  if (in->positions == nullptr && in->R > 0 && in->P < in->T)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: %lld table rows for %lld tokens without positions", what, (long long)in->P,
+                (long long)in->T);
+  if (bwd && in->dweights != nullptr && in->partial == nullptr)
+    return fail(UPLIFT_LA_ERR_ARG, "%s: weight gradients need the workspace", what);
+  if (in->T > 0 && (in->q.data == nullptr || in->k.data == nullptr || in->q_out.data == nullptr ||
+                    in->k_out.data == nullptr || (bwd && (in->dq.data == nullptr || in->dk.data == nullptr)) ||
+                    (in->R > 0 && in->P > 0 && (in->cos == nullptr || in->sin == nullptr))))
+    return fail(UPLIFT_LA_ERR_ARG, "%s: null pointer", what);
+  *a = Args{};
+  const uplift_tok_rows* x[2] = {&in->q, &in->k};
+  const uplift_tok_rows* z[2] = {&in->q_out, &in->k_out};
+  const uplift_tok_rows* d[2] = {&in->dq, &in->dk};
+  for (int i = 0; i < 2; ++i) {
+    Side& sd = a->side[i];
+    sd.x = x[i]->data; sd.x_t = x[i]->row; sd.x_h = x[i]->head;
+    const uplift_tok_rows* o = bwd ? d[i] : z[i];
+    sd.out = o->data; sd.o_t = o->row; sd.o_h = o->head;
+    if (bwd) { sd.g = z[i]->data; sd.g_t = z[i]->row; sd.g_h = z[i]->head; }
+    sd.w = i == 0 ? in->q_weight : in->k_weight;
+    sd.heads = i == 0 ? in->Hq : in->Hk;
+  }
+  a->cos = in->cos; a->sin = in->sin; a->pos = in->positions; a->pos64 = in->positions64; a->wtype = wt;
+  a->T = in->T; a->P = in->P; a->D = in->D; a->R = in->R; a->eps = in->eps; a->inv_d = 1.f / (float)in->D;
+  a->partial = in->partial;
+  a->want_dw = bwd && in->dweights != nullptr;
   return UPLIFT_LA_OK;
+}
+
+int run_dtype(const Args& a, int dtype, bool inter, bool bwd, cudaStream_t s) {
+  if (dtype == UPLIFT_LA_F32) return run<float>(a, inter, bwd, s);
+  if (dtype == UPLIFT_LA_BF16) return run<__nv_bfloat16>(a, inter, bwd, s);
+  return run<__half>(a, inter, bwd, s);
 }
 
 }  // namespace nr
@@ -541,82 +573,37 @@ int check(const char* what, Args* a, int Hq, int Hk, int R, float eps, int wtype
 
 extern "C" {
 
-int uplift_tok_norm_rotate(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
-                           const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
-                           const void* q_weight, const void* k_weight, int weight_dtype,
-                           const float* cos, const float* sin, const void* positions, int positions64,
-                           int64_t T, int64_t P, int Hq, int Hk, int D, int R, float eps, int interleaved,
-                           int dtype, void* stream) {
+int uplift_tok_norm_rotate(const uplift_tok_norm_rotate_args* args, void* stream) {
   using namespace ula;
   using namespace ula::tok::nr;
-  Args a = {};
-  a.cos = cos; a.sin = sin; a.pos = positions; a.pos64 = positions64; a.wtype = weight_dtype;
-  a.T = T; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = D > 0 ? 1.f / (float)D : 0.f;
-  const int rc = check("uplift_tok_norm_rotate", &a, Hq, Hk, R, eps, weight_dtype, dtype);
-  if (rc != UPLIFT_LA_OK) return rc;
-  if (q_strides == nullptr || q_out_strides == nullptr || k_strides == nullptr || k_out_strides == nullptr)
-    return fail(UPLIFT_LA_ERR_ARG, "uplift_tok_norm_rotate: null strides");
-  if (T == 0) return UPLIFT_LA_OK;
-  if (q == nullptr || k == nullptr || q_out == nullptr || k_out == nullptr ||
-      (R > 0 && P > 0 && (cos == nullptr || sin == nullptr)))
-    return fail(UPLIFT_LA_ERR_ARG, "uplift_tok_norm_rotate: null pointer");
-  a.side[0] = {q, q_strides[0], q_strides[1], nullptr, 0, 0, q_out, q_out_strides[0], q_out_strides[1], q_weight, Hq, 0};
-  a.side[1] = {k, k_strides[0], k_strides[1], nullptr, 0, 0, k_out, k_out_strides[0], k_out_strides[1], k_weight, Hk, 0};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int r;
-  if (dtype == UPLIFT_LA_F32) r = run<float>(a, interleaved != 0, false, s);
-  else if (dtype == UPLIFT_LA_BF16) r = run<__nv_bfloat16>(a, interleaved != 0, false, s);
-  else r = run<__half>(a, interleaved != 0, false, s);
-  return r != UPLIFT_LA_OK ? r : tok::launched("norm_rotate");
+  Args a;
+  int rc = prepare("uplift_tok_norm_rotate", args, false, &a);
+  if (rc != UPLIFT_LA_OK || args->T == 0) return rc;
+  rc = run_dtype(a, args->dtype, args->interleaved != 0, false, static_cast<cudaStream_t>(stream));
+  return rc != UPLIFT_LA_OK ? rc : tok::launched("norm_rotate");
 }
 
 int64_t uplift_tok_norm_rotate_partial_floats(int D) {
   return D < 1 ? 0 : 2ll * ula::tok::nr::kBwdBlocks * D;
 }
 
-int uplift_tok_norm_rotate_backward(const void* dq_out, const int64_t dq_out_strides[2], const void* dk_out,
-                                    const int64_t dk_out_strides[2], const void* q, const int64_t q_strides[2],
-                                    const void* k, const int64_t k_strides[2], void* dq,
-                                    const int64_t dq_strides[2], void* dk, const int64_t dk_strides[2],
-                                    float* dweights, const void* q_weight, const void* k_weight, int weight_dtype,
-                                    const float* cos, const float* sin, const void* positions, int positions64,
-                                    float* partial, int64_t T, int64_t P, int Hq, int Hk, int D, int R, float eps,
-                                    int interleaved, int dtype, void* stream) {
+int uplift_tok_norm_rotate_backward(const uplift_tok_norm_rotate_args* args, void* stream) {
   using namespace ula;
   using namespace ula::tok::nr;
-  Args a = {};
-  a.cos = cos; a.sin = sin; a.pos = positions; a.pos64 = positions64; a.wtype = weight_dtype;
-  a.T = T; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = D > 0 ? 1.f / (float)D : 0.f;
-  const int rc = check("uplift_tok_norm_rotate_backward", &a, Hq, Hk, R, eps, weight_dtype, dtype);
+  Args a;
+  int rc = prepare("uplift_tok_norm_rotate_backward", args, true, &a);
   if (rc != UPLIFT_LA_OK) return rc;
-  if (q_strides == nullptr || k_strides == nullptr || dq_strides == nullptr || dk_strides == nullptr ||
-      dq_out_strides == nullptr || dk_out_strides == nullptr)
-    return fail(UPLIFT_LA_ERR_ARG, "uplift_tok_norm_rotate_backward: null strides");
-  if (dweights != nullptr && partial == nullptr)
-    return fail(UPLIFT_LA_ERR_ARG, "uplift_tok_norm_rotate_backward: weight gradients need the workspace");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int blocks = 0;
-  if (T > 0) {
-    if (q == nullptr || k == nullptr || dq == nullptr || dk == nullptr || dq_out == nullptr || dk_out == nullptr ||
-        (R > 0 && P > 0 && (cos == nullptr || sin == nullptr)))
-      return fail(UPLIFT_LA_ERR_ARG, "uplift_tok_norm_rotate_backward: null pointer");
-    a.side[0] = {q, q_strides[0], q_strides[1], dq_out, dq_out_strides[0], dq_out_strides[1],
-                 dq, dq_strides[0], dq_strides[1], q_weight, Hq, 0};
-    a.side[1] = {k, k_strides[0], k_strides[1], dk_out, dk_out_strides[0], dk_out_strides[1],
-                 dk, dk_strides[0], dk_strides[1], k_weight, Hk, 0};
-    a.partial = partial;
-    a.want_dw = dweights != nullptr;
-    int r;
-    if (dtype == UPLIFT_LA_F32) r = run<float>(a, interleaved != 0, true, s);
-    else if (dtype == UPLIFT_LA_BF16) r = run<__nv_bfloat16>(a, interleaved != 0, true, s);
-    else r = run<__half>(a, interleaved != 0, true, s);
-    if (r > 0) return r;
-    blocks = -r;
-    const int e = tok::launched("norm_rotate backward");
-    if (e != UPLIFT_LA_OK) return e;
+  if (args->T > 0) {
+    rc = run_dtype(a, args->dtype, args->interleaved != 0, true, s);
+    if (rc > 0) return rc;
+    blocks = -rc;
+    if ((rc = tok::launched("norm_rotate backward")) != UPLIFT_LA_OK) return rc;
   }
-  if (dweights != nullptr) {
-    dweights_kernel<<<(2 * D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, s>>>(partial, dweights, blocks, D);
+  if (args->dweights != nullptr) {
+    dweights_kernel<<<(2 * args->D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, s>>>(args->partial, args->dweights,
+                                                                                            blocks, args->D);
     return tok::launched("norm_rotate weight gradients");
   }
   return UPLIFT_LA_OK;

@@ -20,8 +20,10 @@ streams and in captured graphs share nothing.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import struct
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -29,62 +31,85 @@ import torch
 from . import _native
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
-_I64_2 = ctypes.c_int64 * 2
+
+# the argument structs of include/uplift_tokens.h (a token tensor: pointer, row stride, head stride)
+_NR_ARGS = struct.Struct("@q" + 6 * "Pqq" + 7 * "P" + "qq" + "iiii" + "f" + "iiiii")
+_PA_ARGS = struct.Struct("@q" + 8 * "Pqq" + 6 * "P" + "qqq" + "iiii" + "f" + "iii")
+_NO_ROWS = (0, 0, 0)
+
+try:  # the stream's handle without making a Stream object (microseconds count in a decoding step)
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # pragma: no cover
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
-def _check(what: str, named) -> torch.device:
-    """The common device of (name, tensor) pairs; raises where they differ or are not on CUDA."""
-    dev = None
+def _on(index: int):
+    """Context in which `index` is the current device."""
+    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _device(what: str, named) -> int:
+    """The common CUDA device index of (name, tensor) pairs; raises where they differ or are not on CUDA."""
+    index = named[0][1].get_device()
     for name, t in named:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"uplift_b200 {what} runs on CUDA (sm_100) tensors only; {name} is a "
                                f"{t.device} tensor (there is no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: tensors on different devices: {dev} vs {t.device} ({name})")
-    return dev
+        if t.get_device() != index:
+            raise ValueError(f"{what}: tensors on different devices: {named[0][1].device} vs {t.device} ({name})")
+    return index
 
 
 def _check_rows(what: str, named) -> None:
-    first = named[0][1]
-    if first.dtype not in _DTYPES:
-        raise ValueError(f"{what}: unsupported dtype {first.dtype} (float32, bfloat16, float16)")
+    name0, first = named[0]
+    dtype, D = first.dtype, first.shape[-1]
+    if dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported dtype {dtype} (float32, bfloat16, float16)")
     for name, t in named:
-        if t.dim() != 3:
-            raise ValueError(f"{what}: {name} must be [rows, heads, D], got {tuple(t.shape)}")
-        if t.dtype != first.dtype:
-            raise ValueError(f"{what}: {name} is {t.dtype}, {named[0][0]} is {first.dtype}")
-        if t.shape[2] != first.shape[2]:
-            raise ValueError(f"{what}: {name} has head dimension {t.shape[2]}, {named[0][0]} has {first.shape[2]}")
-        if t.shape[1] < 1 or t.shape[2] < 1:
-            raise ValueError(f"{what}: {name} has no heads or channels: {tuple(t.shape)}")
+        shape = t.shape
+        if len(shape) != 3:
+            raise ValueError(f"{what}: {name} must be [rows, heads, D], got {tuple(shape)}")
+        if t.dtype is not dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}, {name0} is {dtype}")
+        if shape[2] != D:
+            raise ValueError(f"{what}: {name} has head dimension {shape[2]}, {name0} has {D}")
+        if shape[1] < 1 or D < 1:
+            raise ValueError(f"{what}: {name} has no heads or channels: {tuple(shape)}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t, or a contiguous copy where the kernels cannot read it in place: channel stride 1 and, in 16 bits,
-    16-byte aligned rows whose stride is a multiple of the heads'."""
-    st, hd = t.stride(), t.shape
-    ok = st[2] == 1 or hd[2] == 1
-    if ok and t.element_size() == 2:
-        ok = (t.data_ptr() & 15) == 0 and (hd[0] <= 1 or (st[0] > 0 and st[0] % 8 == 0)) and (
-            hd[1] <= 1 or (st[1] > 0 and st[1] % 8 == 0 and (hd[0] <= 1 or st[0] % st[1] == 0)))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor):
+    """(pointer, row stride, head stride) of t and the tensor that owns them: t, or a contiguous copy where the
+    kernels cannot read it in place (channel stride 1 and, in 16 bits, 16-byte aligned rows whose stride is a
+    multiple of the heads')."""
+    r, h, c = t.stride()
+    rows, heads, D = t.shape
+    ok = c == 1 or D == 1
+    p = t.data_ptr()
+    if ok and t.dtype is not torch.float32:
+        ok = p & 15 == 0 and (rows <= 1 or (r > 0 and r % 8 == 0)) and (
+            heads <= 1 or (h > 0 and h % 8 == 0 and (rows <= 1 or r % h == 0)))
+    if ok:
+        return (p, r, h), t
+    t = t.clone(memory_format=torch.contiguous_format)
+    return (t.data_ptr(), heads * D, D), t
 
 
-def _st(t: torch.Tensor):
-    s = t.stride()
-    return _I64_2(s[0], s[1])
+def _new_rows(t: torch.Tensor):
+    """A new contiguous tensor like t, as _rows gives it."""
+    n = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+    return (n.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]), n
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # ------------------------------------------------------------- norm_rotate
 def _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions):
+    """Checks the arguments: (device index, weights' type)."""
     what = "norm_rotate"
     _check_rows(what, (("q", q), ("k", k)))
     T, _, D = q.shape
@@ -92,27 +117,31 @@ def _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions):
         raise ValueError(f"{what}: q has {T} tokens, k has {k.shape[0]}")
     if D > 256:
         raise ValueError(f"{what}: head dimension {D} is above 256")
-    ws = [w for w in (q_weight, k_weight) if w is not None]
-    for w in ws:
-        if tuple(w.shape) != (D,) or w.dtype not in _DTYPES:
+    wdt = None
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        if w.shape != (D,) or w.dtype not in _DTYPES:
             raise ValueError(f"{what}: weights must be [{D}] in float32, bfloat16 or float16, got "
                              f"{tuple(w.shape)} {w.dtype}")
-        if w.dtype != ws[0].dtype:
-            raise ValueError(f"{what}: q_weight is {ws[0].dtype}, k_weight is {w.dtype}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        if wdt is not None and w.dtype is not wdt:
+            raise ValueError(f"{what}: q_weight is {wdt}, k_weight is {w.dtype}")
+        wdt = w.dtype
+    table = cos.shape
+    if len(table) != 2 or table != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError(f"{what}: cos and sin must be float32 [P, R / 2] tables of one shape, got "
                          f"{tuple(cos.shape)} {cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
-    if 2 * cos.shape[1] > D:
-        raise ValueError(f"{what}: tables rotate {2 * cos.shape[1]} channels, heads have {D}")
+    if 2 * table[1] > D:
+        raise ValueError(f"{what}: tables rotate {2 * table[1]} channels, heads have {D}")
     if positions is None:
-        if cos.shape[1] > 0 and cos.shape[0] < T:
-            raise ValueError(f"{what}: {cos.shape[0]} table rows for {T} tokens without positions")
-    elif tuple(positions.shape) != (T,) or positions.dtype not in (torch.int32, torch.int64):
+        if table[1] > 0 and table[0] < T:
+            raise ValueError(f"{what}: {table[0]} table rows for {T} tokens without positions")
+    elif positions.shape != (T,) or (positions.dtype is not torch.int32 and positions.dtype is not torch.int64):
         raise ValueError(f"{what}: positions must be int32 or int64 [{T}], got {tuple(positions.shape)} "
                          f"{positions.dtype}")
-    dev = _check(what, (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos),
-                        ("sin", sin), ("positions", positions)))
-    return dev, (_DTYPES[ws[0].dtype] if ws else _native.F32)
+    index = _device(what, (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos),
+                           ("sin", sin), ("positions", positions)))
+    return index, (_native.F32 if wdt is None else _DTYPES[wdt])
 
 
 def _c(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -121,47 +150,51 @@ def _c(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
     """Launch uplift_tok_norm_rotate (no autograd)."""
-    dev, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
     T, Hq, D = q.shape
-    Hk = k.shape[1]
-    q, k = _rows(q), _rows(k)
-    qw, kw, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
-    qo = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    ko = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        rc = _native.load().uplift_tok_norm_rotate(
-            q.data_ptr(), _st(q), qo.data_ptr(), _st(qo), k.data_ptr(), _st(k), ko.data_ptr(), _st(ko),
-            _ptr(qw), _ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), _ptr(positions),
-            int(positions is not None and positions.dtype == torch.int64), T, cos.shape[0], Hq, Hk, D,
-            2 * cos.shape[1], float(eps), int(bool(interleaved)), _DTYPES[q.dtype],
-            torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "uplift_tok_norm_rotate")
-    return qo, ko
+    P, half = cos.shape
+    lib = _native.load()
+    q_weight, k_weight, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
+    with _on(index):
+        rq, q = _rows(q)
+        rk, k = _rows(k)
+        ro, q_out = _new_rows(q)
+        rp, k_out = _new_rows(k)
+        rc = lib.uplift_tok_norm_rotate(
+            _NR_ARGS.pack(_NR_ARGS.size, *rq, *rk, *ro, *rp, *_NO_ROWS, *_NO_ROWS, _ptr(q_weight), _ptr(k_weight),
+                          cos.data_ptr(), sin.data_ptr(), _ptr(positions), 0, 0, T, P, Hq, k.shape[1], D, 2 * half,
+                          eps, interleaved, wt, positions is not None and positions.dtype is torch.int64,
+                          _DTYPES[q.dtype], 0), _raw_stream(index))
+    if rc:
+        _native.check(rc, "uplift_tok_norm_rotate")
+    return q_out, k_out
 
 
 def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
                              interleaved=False, need_weights=True):
     """Launch uplift_tok_norm_rotate_backward: (dq, dk, dweights [2, D] fp32; empty when not needed)."""
-    dev, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
     T, Hq, D = q.shape
-    Hk = k.shape[1]
-    gq, gk, q, k = _rows(gq.to(q.dtype)), _rows(gk.to(q.dtype)), _rows(q), _rows(k)
-    qw, kw, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
+    P, half = cos.shape
     lib = _native.load()
-    dq = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
-    dw = torch.empty((2, D) if need_weights else (0,), dtype=torch.float32, device=dev)
-    partial = torch.empty(lib.uplift_tok_norm_rotate_partial_floats(D) if need_weights else 0,
-                          dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    q_weight, k_weight, cos, sin, positions = _c(q_weight), _c(k_weight), _c(cos), _c(sin), _c(positions)
+    with _on(index):
+        rq, q = _rows(q)
+        rk, k = _rows(k)
+        rg, gq = _rows(gq.to(q.dtype))
+        rh, gk = _rows(gk.to(q.dtype))
+        rdq, dq = _new_rows(q)
+        rdk, dk = _new_rows(k)
+        dw = torch.empty((2, D) if need_weights else (0,), dtype=torch.float32, device=q.device)
+        partial = dw.new_empty(lib.uplift_tok_norm_rotate_partial_floats(D)) if need_weights else None
         rc = lib.uplift_tok_norm_rotate_backward(
-            gq.data_ptr(), _st(gq), gk.data_ptr(), _st(gk), q.data_ptr(), _st(q), k.data_ptr(), _st(k),
-            dq.data_ptr(), _st(dq), dk.data_ptr(), _st(dk), dw.data_ptr() if need_weights else None, _ptr(qw),
-            _ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), _ptr(positions),
-            int(positions is not None and positions.dtype == torch.int64),
-            partial.data_ptr() if need_weights else None, T, cos.shape[0], Hq, Hk, D, 2 * cos.shape[1], float(eps),
-            int(bool(interleaved)), _DTYPES[q.dtype], torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "uplift_tok_norm_rotate_backward")
+            _NR_ARGS.pack(_NR_ARGS.size, *rq, *rk, *rg, *rh, *rdq, *rdk, _ptr(q_weight), _ptr(k_weight),
+                          cos.data_ptr(), sin.data_ptr(), _ptr(positions), dw.data_ptr() if need_weights else 0,
+                          _ptr(partial), T, P, Hq, k.shape[1], D, 2 * half, eps, interleaved, wt,
+                          positions is not None and positions.dtype is torch.int64, _DTYPES[q.dtype], 0),
+            _raw_stream(index))
+    if rc:
+        _native.check(rc, "uplift_tok_norm_rotate_backward")
     return dq, dk, dw
 
 
@@ -261,77 +294,89 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
 
 
 # -------------------------------------------------------- packed_attention
-def _starts(what: str, name: str, t: torch.Tensor, entries: Optional[int] = None) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() < 1 if entries is None else t.numel() != entries):
-        raise ValueError(f"{what}: {name} must be an int32 vector" +
-                         ("" if entries is None else f" of {entries} entries") +
-                         f", got {tuple(t.shape)} {t.dtype}")
+def _starts(what: str, name: str, t: torch.Tensor, entries: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != entries or entries < (name != "used_k"):
+        raise ValueError(f"{what}: {name} must be an int32 vector of {entries} entries (sequences" +
+                         (")" if name == "used_k" else " + 1)") + f", got {tuple(t.shape)} {t.dtype}")
 
 
 def _attention_args(q, k, v, cu_q, cu_k, used_k, scale):
+    """Checks the arguments: the device index."""
     what = "packed_attention"
     _check_rows(what, (("q", q), ("k", k), ("v", v)))
     if k.shape != v.shape:
         raise ValueError(f"{what}: k is {tuple(k.shape)}, v is {tuple(v.shape)}")
-    if q.shape[1] % k.shape[1] != 0:
-        raise ValueError(f"{what}: {q.shape[1]} query heads are not a multiple of {k.shape[1]} key heads")
-    D = q.shape[2]
-    if D > 128 or (q.element_size() == 2 and D % 8 != 0):
+    _, Hq, D = q.shape
+    if Hq % k.shape[1] != 0:
+        raise ValueError(f"{what}: {Hq} query heads are not a multiple of {k.shape[1]} key heads")
+    if D > 128 or (D % 8 != 0 and q.dtype is not torch.float32):
         raise ValueError(f"{what}: head dimension {D} (at most 128; a multiple of 8 in 16 bits)")
-    _starts(what, "cu_q", cu_q)
-    _starts(what, "cu_k", cu_k, cu_q.numel())
+    n = cu_q.numel()
+    _starts(what, "cu_q", cu_q, n)
+    _starts(what, "cu_k", cu_k, n)
     if used_k is not None:
-        _starts(what, "used_k", used_k, cu_q.numel() - 1)
+        _starts(what, "used_k", used_k, n - 1)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
-    return _check(what, (("q", q), ("k", k), ("v", v), ("cu_q", cu_q), ("cu_k", cu_k), ("used_k", used_k)))
+    return _device(what, (("q", q), ("k", k), ("v", v), ("cu_q", cu_q), ("cu_k", cu_k), ("used_k", used_k)))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B, T, S, Hq, Hk, D, dtype) -> int:
+    return _native.load().uplift_tok_attention_workspace(B, T, S, Hq, Hk, D, dtype)
 
 
 def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=None, need_lse=False):
-    """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, empty when not needed)."""
+    """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, None when not needed)."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
-    dev = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
+    index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
-    B = cu_q.numel() - 1
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    cu_q, cu_k, used_k = _c(cu_q), _c(cu_k), _c(used_k)
+    B = cu_q.shape[0] - 1
     dt = _DTYPES[q.dtype]
     lib = _native.load()
     _native.host_status.raise_if_set()
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((Hq, T) if need_lse else (0,), dtype=torch.float32, device=dev)
-    nbytes = lib.uplift_tok_attention_workspace(B, T, S, Hq, Hk, D, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-    with torch.cuda.device(dev):
+    cu_q, cu_k, used_k = cu_q.contiguous(), cu_k.contiguous(), _c(used_k)
+    nbytes = _workspace_bytes(B, T, S, Hq, Hk, D, dt)
+    with _on(index):
+        rq, q = _rows(q)
+        rk, k = _rows(k)
+        rv, v = _rows(v)
+        ro, out = _new_rows(q)
+        lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device) if need_lse else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.uplift_tok_attention_forward(
-            q.data_ptr(), _st(q), k.data_ptr(), _st(k), v.data_ptr(), _st(v), out.data_ptr(), _st(out),
-            lse.data_ptr() if need_lse else None, cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), B, T, S, Hq, Hk, D,
-            scale, int(bool(causal)), dt, _ptr(ws), nbytes, torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "uplift_tok_attention_forward")
+            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, _ptr(lse), 0,
+                          cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), _ptr(ws), nbytes, T, S, B, Hq, Hk, D,
+                          scale, causal, dt, 0), _raw_stream(index))
+    if rc:
+        _native.check(rc, "uplift_tok_attention_forward")
     return out, lse
 
 
 def packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k=None, causal=True, scale=None):
     """Launch uplift_tok_attention_backward: (dq, dk, dv)."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
-    dev = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
+    index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
-    g, q, k, v, out = _rows(g.to(q.dtype)), _rows(q), _rows(k), _rows(v), _rows(out)
-    cu_q, cu_k, used_k, lse = _c(cu_q), _c(cu_k), _c(used_k), lse.contiguous()
-    dq = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((S, Hk, D), dtype=q.dtype, device=dev)
-    dv = torch.empty((S, Hk, D), dtype=q.dtype, device=dev)
-    delta = torch.empty((Hq, T), dtype=torch.float32, device=dev)
     lib = _native.load()
     _native.host_status.raise_if_set()
-    with torch.cuda.device(dev):
+    cu_q, cu_k, used_k, lse = cu_q.contiguous(), cu_k.contiguous(), _c(used_k), lse.contiguous()
+    with _on(index):
+        rg, g = _rows(g.to(q.dtype))
+        rq, q = _rows(q)
+        rk, k = _rows(k)
+        rv, v = _rows(v)
+        ro, out = _rows(out)
+        rdq, dq = _new_rows(q)
+        rdk, dk = _new_rows(k)
+        rdv, dv = _new_rows(v)
+        delta = torch.empty_like(lse)
         rc = lib.uplift_tok_attention_backward(
-            g.data_ptr(), _st(g), q.data_ptr(), _st(q), k.data_ptr(), _st(k), v.data_ptr(), _st(v),
-            out.data_ptr(), _st(out), lse.data_ptr(), dq.data_ptr(), _st(dq), dk.data_ptr(), _st(dk),
-            dv.data_ptr(), _st(dv), delta.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k),
-            cu_q.numel() - 1, T, S, Hq, Hk, D, scale, int(bool(causal)), _DTYPES[q.dtype],
-            torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "uplift_tok_attention_backward")
+            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *rg, *rdq, *rdk, *rdv, lse.data_ptr(), delta.data_ptr(),
+                          cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), 0, 0, T, S, cu_q.shape[0] - 1, Hq, Hk, D,
+                          scale, causal, _DTYPES[q.dtype], 0), _raw_stream(index))
+    if rc:
+        _native.check(rc, "uplift_tok_attention_backward")
     return dq, dk, dv
 
 
