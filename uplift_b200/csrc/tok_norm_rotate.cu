@@ -9,11 +9,10 @@
 //   dw = sum over rows of g h,   dx = r (g w - h mean(g w h)).
 //
 // Both are one pass over HBM: a row (token, head) sits in the registers of a
-// group of lanes, one 16-byte vector per lane, so the forward reads and
-// writes each element once and the backward reads x and dz and writes dx.
-// The partner channels of a half-split pair are in another lane of the group
-// and come by shuffle, still packed in the storage type.  A group keeps the
-// cos / sin row of its token over several heads.
+// group of lanes, two 8-byte pieces per lane, so the forward reads and writes
+// each element once and the backward reads x and dz and writes dx.  A lane
+// holds both channels of its pairs, and keeps the cos / sin row of its token
+// (times the weights) over several heads.
 
 #include <cuda_runtime.h>
 #include <math.h>
@@ -29,6 +28,10 @@ namespace tok {
 namespace nr {
 
 constexpr int kThreads = 256;
+#ifndef ULA_NR_HPG
+#define ULA_NR_HPG 4
+#endif
+constexpr int kManyHeads = ULA_NR_HPG;
 constexpr int kBwdBlocks = 148 * 4;  // fixed, so the order of the dw sums does not depend on the problem's size
 
 struct Side {  // queries or keys
@@ -36,7 +39,7 @@ struct Side {  // queries or keys
   const void* g; int64_t g_t, g_h;   // backward: gradient of the output
   void* out;     int64_t o_t, o_h;   // forward: the output; backward: dx
   const void* w;
-  int heads, chunks;                 // chunks of `hpg` heads
+  int heads, chunks;                 // chunks of heads that one group of lanes takes
 };
 
 struct Args {
@@ -45,8 +48,9 @@ struct Args {
   const float* sin;
   const void* pos;
   int pos64, wtype;
+  int weight_rows;  // the weights have the tensors' type and 8-byte alignment
   int64_t T, P;
-  int D, R, hpg;  // hpg: heads per group of lanes
+  int D, R;
   float eps, inv_d;
   float* partial;  // backward: [2][kBwdBlocks][D]
   int want_dw;
@@ -67,43 +71,101 @@ __device__ __forceinline__ float weight_at(const void* w, int wtype, int i) {
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
-template <typename T>
-struct Row {  // one lane's 16 bytes of a row
+// One lane's channels of a row: V / 2 channel pairs (a, b), packed in the
+// storage type as two 8-byte pieces.  Half-split: the first piece holds the
+// a's, the second, R / 2 channels on, the b's; interleaved: the pieces are
+// neighbours and hold a, b, a, b, ..  So a rotation stays within the lane.
+template <typename T, bool INTER>
+struct Row {
   static constexpr int kVec = 16 / sizeof(T);
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
-  __device__ __forceinline__ void to(float* v) const {
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+  static constexpr int kPairs = kVec / 2;
+  uint2 lo, hi;
+  __device__ __forceinline__ void load(const T* p, int step) {
+    lo = __ldg(reinterpret_cast<const uint2*>(p));
+    hi = __ldg(reinterpret_cast<const uint2*>(p + step));
+  }
+  __device__ __forceinline__ void store(T* p, int step) const {
+    *reinterpret_cast<uint2*>(p) = lo;
+    *reinterpret_cast<uint2*>(p + step) = hi;
+  }
+  __device__ __forceinline__ void to(float* a, float* b) const {
+    const uint32_t u[4] = {lo.x, lo.y, hi.x, hi.y};
+    if constexpr (sizeof(T) == 4) {
+      a[0] = __uint_as_float(u[0]);
+      (INTER ? b[0] : a[1]) = __uint_as_float(u[1]);
+      (INTER ? a[1] : b[0]) = __uint_as_float(u[2]);
+      b[1] = __uint_as_float(u[3]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        v[i] = __uint_as_float(u[i]);
-      } else {
+      for (int i = 0; i < 4; ++i) {
         const float2 f = St<T>::unpack(u[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        if (INTER) {
+          a[i] = f.x;
+          b[i] = f.y;
+        } else {
+          float* d = i < 2 ? a + 2 * i : b + 2 * (i - 2);
+          d[0] = f.x;
+          d[1] = f.y;
+        }
       }
     }
   }
-  __device__ __forceinline__ void from(const float* v) {
+  __device__ __forceinline__ void from(const float* a, const float* b) {
     uint32_t u[4];
+    if constexpr (sizeof(T) == 4) {
+      u[0] = __float_as_uint(a[0]);
+      u[1] = __float_as_uint(INTER ? b[0] : a[1]);
+      u[2] = __float_as_uint(INTER ? a[1] : b[0]);
+      u[3] = __float_as_uint(b[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) u[i] = __float_as_uint(v[i]);
-      else u[i] = St<T>::pack(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < 4; ++i)
+        u[i] = INTER ? St<T>::pack(a[i], b[i]) : (i < 2 ? St<T>::pack(a[2 * i], a[2 * i + 1]) : St<T>::pack(b[2 * i - 4], b[2 * i - 3]));
     }
-    raw = make_uint4(u[0], u[1], u[2], u[3]);
-  }
-  __device__ __forceinline__ Row shuffled(int src) const {
-    Row r;
-    r.raw.x = __shfl_sync(0xffffffffu, raw.x, src);
-    r.raw.y = __shfl_sync(0xffffffffu, raw.y, src);
-    r.raw.z = __shfl_sync(0xffffffffu, raw.z, src);
-    r.raw.w = __shfl_sync(0xffffffffu, raw.w, src);
-    return r;
+    lo = make_uint2(u[0], u[1]);
+    hi = make_uint2(u[2], u[3]);
   }
 };
+
+// Arithmetic on two fp32 values at a time: d = x y + z, x y, for N values.
+template <int N>
+__device__ __forceinline__ void fma_n(float* d, const float* x, const float* y, const float* z) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 r = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(y[i], y[i + 1]), make_float2(z[i], z[i + 1]));
+    d[i] = r.x;
+    d[i + 1] = r.y;
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_n(float* d, const float* x, const float* y) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 r = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(y[i], y[i + 1]));
+    d[i] = r.x;
+    d[i + 1] = r.y;
+  }
+}
+template <int N>
+__device__ __forceinline__ void scale_n(float* d, const float* x, float f) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 r = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(f, f));
+    d[i] = r.x;
+    d[i + 1] = r.y;
+  }
+}
+// sum of x y over N values of both elements of the pairs
+template <int N>
+__device__ __forceinline__ float dot_n(const float* xa, const float* ya, const float* xb, const float* yb) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    s = __ffma2_rn(make_float2(xa[i], xa[i + 1]), make_float2(ya[i], ya[i + 1]), s);
+    s = __ffma2_rn(make_float2(xb[i], xb[i + 1]), make_float2(yb[i], yb[i + 1]), s);
+  }
+  return s.x + s.y;
+}
 
 template <int LANES>
 __device__ __forceinline__ float group_sum(float v) {
@@ -115,69 +177,73 @@ __device__ __forceinline__ float group_sum(float v) {
 // What a lane needs to know of its channels, the same for every row.
 template <typename T, int LANES, bool INTER>
 struct Lane {
-  static constexpr int V = Row<T>::kVec;
-  int c0;        // first channel
+  static constexpr int V = Row<T, INTER>::kVec, N = V / 2;
+  int c0;        // first channel of the first piece
+  int step;      // channels from the first piece to the second
   bool active;   // it has channels
   bool rotated;  // they are rotated
-  bool upper;    // half-split: they are second elements of their pairs
-  int partner;   // half-split: lane of the warp that holds the partners
+  int pair;      // its first pair of the table
   __device__ __forceinline__ Lane(const Args& a) {
-    const int lane = threadIdx.x & 31, l = lane & (LANES - 1);
-    c0 = l * V;
-    active = c0 < a.D;
-    rotated = c0 < a.R;
-    upper = !INTER && c0 >= a.R / 2;
-    const int shift = (a.R / 2) / V;
-    partner = INTER || !rotated ? lane : (upper ? lane - shift : lane + shift);
+    const int l = threadIdx.x & (LANES - 1);
+    active = l * V < a.D;
+    rotated = l * V < a.R;
+    const bool split = !INTER && rotated;
+    c0 = split ? l * N : l * V;
+    step = split ? a.R / 2 : N;
+    pair = l * N;
   }
-  // c and s of the lane's channels (s with the sign of the channel's place
-  // in its pair: z = y c + y_partner s); false if they are not rotated.
+  // The weights of its channels.
+  __device__ __forceinline__ void weights(const Args& a, const void* w, float* wa, float* wb) const {
+    if (a.weight_rows && w != nullptr) {  // of the tensors' type
+      Row<T, INTER> r{};
+      if (active) r.load(static_cast<const T*>(w) + c0, step);
+      r.to(wa, wb);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      wa[i] = wb[i] = 0.f;
+      if (active) {
+        const int ca = INTER ? c0 + 2 * i : c0 + i, cb = INTER ? ca + 1 : ca + step;
+        wa[i] = weight_at(w, a.wtype, ca);
+        wb[i] = weight_at(w, a.wtype, cb);
+      }
+    }
+  }
+  // c and s of its pairs for a row of the table; false if they are not rotated.
   __device__ __forceinline__ bool angles(const Args& a, int64_t row, float* c, float* s) const {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < N; ++i) {
       c[i] = 1.f;
       s[i] = 0.f;
     }
     if (!rotated || row == -1) return false;
     if (row == -2) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+      for (int i = 0; i < N; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
       return true;
     }
-    if constexpr (INTER) {
-      const float* pc = a.cos + row * (a.R / 2) + c0 / 2;
-      const float* ps = a.sin + row * (a.R / 2) + c0 / 2;
+    const float2* pc = reinterpret_cast<const float2*>(a.cos + row * (a.R / 2) + pair);
+    const float2* ps = reinterpret_cast<const float2*>(a.sin + row * (a.R / 2) + pair);
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        c[2 * i] = c[2 * i + 1] = __ldg(pc + i);
-        s[2 * i + 1] = __ldg(ps + i);
-        s[2 * i] = -s[2 * i + 1];
-      }
-    } else {
-      const int i0 = upper ? c0 - a.R / 2 : c0;
-      const float4* pc = reinterpret_cast<const float4*>(a.cos + row * (a.R / 2) + i0);
-      const float4* ps = reinterpret_cast<const float4*>(a.sin + row * (a.R / 2) + i0);
-#pragma unroll
-      for (int i = 0; i < V / 4; ++i) {
-        const float4 fc = __ldg(pc + i), fs = __ldg(ps + i);
-        c[4 * i] = fc.x; c[4 * i + 1] = fc.y; c[4 * i + 2] = fc.z; c[4 * i + 3] = fc.w;
-        s[4 * i] = fs.x; s[4 * i + 1] = fs.y; s[4 * i + 2] = fs.z; s[4 * i + 3] = fs.w;
-      }
-      if (!upper) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = -s[i];
-      }
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 fc = __ldg(pc + i), fs = __ldg(ps + i);
+      c[2 * i] = fc.x; c[2 * i + 1] = fc.y;
+      s[2 * i] = fs.x; s[2 * i + 1] = fs.y;
     }
     return true;
   }
 };
 
-// Forward.  Group g of LANES lanes: token g / chunks, heads of one chunk.
+// Forward.  Group g of LANES lanes: token g / chunks, HPG heads of one side.
+// All rows are loaded before the first is used, and the token's angles times
+// the weights serve all of them:
+//   za = r (xa (wa c) - xb (wb s)),  zb = r (xb (wb c) + xa (wa s)).
 // Out-of-range groups compute on the last group's rows and store nothing, so
 // that every lane of a warp takes part in the shuffles.
-template <typename T, int LANES, bool INTER>
+template <typename T, int LANES, bool INTER, int HPG>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
-  constexpr int V = Row<T>::kVec;
+  constexpr int N = Row<T, INTER>::kPairs;
   const Lane<T, LANES, INTER> ln(a);
   const int chunks = a.side[0].chunks + a.side[1].chunks;
   const int64_t groups = a.T * chunks;
@@ -189,61 +255,52 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   const int which = ch >= a.side[0].chunks;
   const Side& sd = a.side[which];
   if (which) ch -= a.side[0].chunks;
-  const int h0 = ch * a.hpg;
-  const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + ln.c0;
-  T* out = static_cast<T*>(sd.out) + t * sd.o_t + ln.c0;
-  float c[V], s[V], w[V], wp[V];
+  const int h0 = ch * HPG;
+  const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h0 * sd.x_h + ln.c0;
+  T* out = static_cast<T*>(sd.out) + t * sd.o_t + h0 * sd.o_h + ln.c0;
+  Row<T, INTER> rows[HPG] = {};
+#pragma unroll
+  for (int j = 0; j < HPG; ++j)
+    if (ln.active && h0 + j < sd.heads) rows[j].load(x + j * sd.x_h, ln.step);
+  float c[N], s[N], wa[N], wb[N];
   const bool turn = ln.angles(a, table_row(a, t), c, s);
+  ln.weights(a, sd.w, wa, wb);
+  float ca[N], sb[N], cb[N], sa[N];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    w[i] = wp[i] = 0.f;
-    if (ln.active) {
-      w[i] = weight_at(sd.w, a.wtype, ln.c0 + i);
-      if (!INTER && ln.rotated) wp[i] = weight_at(sd.w, a.wtype, ln.upper ? ln.c0 + i - a.R / 2 : ln.c0 + i + a.R / 2);
-    }
+  for (int i = 0; i < N; ++i) {
+    ca[i] = wa[i] * c[i];
+    sb[i] = -wb[i] * s[i];
+    cb[i] = wb[i] * c[i];
+    sa[i] = wa[i] * s[i];
   }
-  // the loop count is that of the kernel, not of the chunk: uniform over the warp
-  Row<T> next{};
-  if (ln.active) next.load(x + min(h0, sd.heads - 1) * sd.x_h);
-  for (int j = 0; j < a.hpg; ++j) {
-    const int h = h0 + j;
-    const Row<T> cur = next;
-    if (ln.active && j + 1 < a.hpg) next.load(x + min(h + 1, sd.heads - 1) * sd.x_h);
-    float v[V];
-    cur.to(v);
-    float sq = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sq = fmaf(v[i], v[i], sq);
-    sq = group_sum<LANES>(sq);
-    const float r = 1.f / sqrtf(fmaf(sq, a.inv_d, a.eps));
-    float z[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = v[i] * r * w[i];
-    if constexpr (INTER) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = fmaf(v[i], c[i], v[i ^ 1] * s[i]);
-    } else {
-      float vp[V];
-      cur.shuffled(ln.partner).to(vp);
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = fmaf(v[i], c[i], vp[i] * r * wp[i] * s[i]);
-    }
-    if (live && ln.active && h < sd.heads) {
-      // a partner's infinity must not reach channels that are not rotated
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = turn ? z[i] : v[i];
-      Row<T> o;
-      o.from(z);
-      o.store(out + h * sd.o_h);
+  for (int j = 0; j < HPG; ++j) {
+    float xa[N], xb[N];
+    rows[j].to(xa, xb);
+    const float sq = group_sum<LANES>(dot_n<N>(xa, xa, xb, xb));
+    const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
+    if (live && ln.active && h0 + j < sd.heads) {
+      float za[N], zb[N];
+      mul_n<N>(za, xa, ca);
+      mul_n<N>(zb, xb, cb);
+      if (turn) {  // else a partner's infinity would make NaN of s = 0
+        fma_n<N>(za, xb, sb, za);
+        fma_n<N>(zb, xa, sa, zb);
+      }
+      scale_n<N>(za, za, r);
+      scale_n<N>(zb, zb, r);
+      Row<T, INTER> o;
+      o.from(za, zb);
+      o.store(out + j * sd.o_h, ln.step);
     }
   }
 }
 
 // Backward.  Blocks stride over the groups; each lane sums its channels' dw
 // over its rows, first of all query rows, then of all key rows.
-template <typename T, int LANES, bool INTER>
+template <typename T, int LANES, bool INTER, int HPG>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const Args a) {
-  constexpr int V = Row<T>::kVec;
+  constexpr int V = Row<T, INTER>::kVec, N = V / 2;
   constexpr int kGroups = kThreads / LANES;
   __shared__ float red[kGroups * LANES * V];
   const Lane<T, LANES, INTER> ln(a);
@@ -251,12 +308,10 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args a) {
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     const Side& sd = a.side[which];
-    float w[V], dw[V];
+    float wa[N], wb[N], dwa[N], dwb[N];
+    ln.weights(a, sd.w, wa, wb);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = ln.active ? weight_at(sd.w, a.wtype, ln.c0 + i) : 0.f;
-      dw[i] = 0.f;
-    }
+    for (int i = 0; i < N; ++i) dwa[i] = dwb[i] = 0.f;
     const int64_t groups = a.T * sd.chunks;
     const int64_t rounds = (groups + (int64_t)gridDim.x * kGroups - 1) / ((int64_t)gridDim.x * kGroups);
     for (int64_t n = 0; n < rounds; ++n) {
@@ -264,71 +319,73 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args a) {
       const bool live = g < groups;
       g = min(g, groups - 1);
       const int64_t t = g / sd.chunks;
-      const int h0 = (int)(g - t * sd.chunks) * a.hpg;
-      const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + ln.c0;
-      const T* gz = static_cast<const T*>(sd.g) + t * sd.g_t + ln.c0;
-      T* out = static_cast<T*>(sd.out) + t * sd.o_t + ln.c0;
-      float c[V], s[V];
-      const bool turn = ln.angles(a, table_row(a, t), c, s);
-      Row<T> nx{}, ng{};
-      if (ln.active) {
-        nx.load(x + min(h0, sd.heads - 1) * sd.x_h);
-        ng.load(gz + min(h0, sd.heads - 1) * sd.g_h);
+      const int h0 = (int)(g - t * sd.chunks) * HPG;
+      const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h0 * sd.x_h + ln.c0;
+      const T* gz = static_cast<const T*>(sd.g) + t * sd.g_t + h0 * sd.g_h + ln.c0;
+      T* out = static_cast<T*>(sd.out) + t * sd.o_t + h0 * sd.o_h + ln.c0;
+      Row<T, INTER> rx[HPG] = {}, rg[HPG] = {};
+#pragma unroll
+      for (int j = 0; j < HPG; ++j) {
+        if (ln.active && h0 + j < sd.heads) {
+          rx[j].load(x + j * sd.x_h, ln.step);
+          rg[j].load(gz + j * sd.g_h, ln.step);
+        }
       }
-      for (int j = 0; j < a.hpg; ++j) {
-        const int h = h0 + j;
-        const Row<T> cx = nx, cg = ng;
-        if (ln.active && j + 1 < a.hpg) {
-          nx.load(x + min(h + 1, sd.heads - 1) * sd.x_h);
-          ng.load(gz + min(h + 1, sd.heads - 1) * sd.g_h);
+      float c[N], s[N], ns[N];
+      const bool turn = ln.angles(a, table_row(a, t), c, s);
+#pragma unroll
+      for (int i = 0; i < N; ++i) ns[i] = -s[i];
+#pragma unroll
+      for (int j = 0; j < HPG; ++j) {
+        float xa[N], xb[N], ga[N], gb[N];
+        rx[j].to(xa, xb);
+        rg[j].to(ga, gb);
+        if (turn) {  // transpose of the rotation
+          float ya[N], yb[N];
+          mul_n<N>(ya, ga, c);
+          mul_n<N>(yb, gb, c);
+          fma_n<N>(ya, gb, s, ya);
+          fma_n<N>(gb, ga, ns, yb);
+#pragma unroll
+          for (int i = 0; i < N; ++i) ga[i] = ya[i];
         }
-        float v[V], gy[V];
-        cx.to(v);
-        cg.to(gy);
-        // transpose of the rotation: the signs of s swap
-        if constexpr (INTER) {
-          float gr[V];
+        float gwa[N], gwb[N];
+        mul_n<N>(gwa, ga, wa);
+        mul_n<N>(gwb, gb, wb);
+        const float sq = group_sum<LANES>(dot_n<N>(xa, xa, xb, xb));
+        const float dot = group_sum<LANES>(dot_n<N>(xa, gwa, xb, gwb));
+        const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
+        const float m = -dot * r * a.inv_d;  // -mean(g w h)
+        if (live && ln.active && h0 + j < sd.heads) {
+          const float mm[2] = {m, m};
+          scale_n<N>(xa, xa, r);  // h
+          scale_n<N>(xb, xb, r);
+          fma_n<N>(dwa, ga, xa, dwa);
+          fma_n<N>(dwb, gb, xb, dwb);
 #pragma unroll
-          for (int i = 0; i < V; ++i) gr[i] = fmaf(gy[i], c[i], -gy[i ^ 1] * s[i]);
-#pragma unroll
-          for (int i = 0; i < V; ++i) gy[i] = turn ? gr[i] : gy[i];
-        } else {
-          float gp[V];
-          cg.shuffled(ln.partner).to(gp);
-          if (turn) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) gy[i] = fmaf(gy[i], c[i], -gp[i] * s[i]);
+          for (int i = 0; i < N; i += 2) {
+            fma_n<2>(gwa + i, xa + i, mm, gwa + i);
+            fma_n<2>(gwb + i, xb + i, mm, gwb + i);
           }
-        }
-        float sq = 0.f, dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          sq = fmaf(v[i], v[i], sq);
-          dot = fmaf(gy[i] * w[i], v[i], dot);
-        }
-        sq = group_sum<LANES>(sq);
-        dot = group_sum<LANES>(dot);
-        const float r = 1.f / sqrtf(fmaf(sq, a.inv_d, a.eps));
-        const float m = dot * r * a.inv_d;  // mean(g w h)
-        if (live && ln.active && h < sd.heads) {
-          float d[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float hh = v[i] * r;
-            d[i] = r * fmaf(-hh, m, gy[i] * w[i]);
-            dw[i] = fmaf(gy[i], hh, dw[i]);
-          }
-          Row<T> o;
-          o.from(d);
-          o.store(out + h * sd.o_h);
+          scale_n<N>(gwa, gwa, r);
+          scale_n<N>(gwb, gwb, r);
+          Row<T, INTER> o;
+          o.from(gwa, gwb);
+          o.store(out + j * sd.o_h, ln.step);
         }
       }
     }
     if (a.want_dw) {
       // the block's groups in ascending order
       __syncthreads();
+      if (ln.active) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) red[gi * LANES * V + ln.c0 + i] = dw[i];
+        for (int i = 0; i < N; ++i) {
+          const int ch = INTER ? ln.c0 + 2 * i : ln.c0 + i;
+          red[gi * LANES * V + ch] = dwa[i];
+          red[gi * LANES * V + (INTER ? ch + 1 : ch + ln.step)] = dwb[i];
+        }
+      }
       __syncthreads();
       for (int d = threadIdx.x; d < a.D; d += kThreads) {
         float sum = 0.f;
@@ -360,7 +417,7 @@ __global__ void __launch_bounds__(kThreads) forward_any_kernel(const Args a, int
     sq = fmaf(v, v, sq);
   }
   sq = group_sum<32>(sq);
-  const float r = 1.f / sqrtf(fmaf(sq, a.inv_d, a.eps));
+  const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
   const int64_t tr = table_row(a, t);
   for (int i = lane; i < a.D; i += 32) {
     float z = St<T>::f(x[i]) * r * weight_at(sd.w, a.wtype, i);
@@ -423,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) backward_any_kernel(const Args a, in
       }
       sq = group_sum<32>(sq);
       dot = group_sum<32>(dot);
-      const float r = 1.f / sqrtf(fmaf(sq, a.inv_d, a.eps));
+      const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
       const float m = dot * r * a.inv_d;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
@@ -463,56 +520,54 @@ __global__ void __launch_bounds__(kThreads) dweights_kernel(const float* partial
   if (lane == 0) dweights[out] = (float)sum;
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, int HPG>
 void launch_vec(const Args& a, bool inter, bool bwd, int blocks, cudaStream_t s) {
   if (bwd) {
-    if (inter) backward_kernel<T, LANES, true><<<blocks, kThreads, 0, s>>>(a);
-    else backward_kernel<T, LANES, false><<<blocks, kThreads, 0, s>>>(a);
+    if (inter) backward_kernel<T, LANES, true, HPG><<<blocks, kThreads, 0, s>>>(a);
+    else backward_kernel<T, LANES, false, HPG><<<blocks, kThreads, 0, s>>>(a);
   } else {
-    if (inter) forward_kernel<T, LANES, true><<<blocks, kThreads, 0, s>>>(a);
-    else forward_kernel<T, LANES, false><<<blocks, kThreads, 0, s>>>(a);
+    if (inter) forward_kernel<T, LANES, true, HPG><<<blocks, kThreads, 0, s>>>(a);
+    else forward_kernel<T, LANES, false, HPG><<<blocks, kThreads, 0, s>>>(a);
   }
 }
 
+template <typename T, int HPG>
+void launch_lanes(const Args& a, int lanes, bool inter, bool bwd, int blocks, cudaStream_t s) {
+  switch (lanes) {
+    case 4: launch_vec<T, 4, HPG>(a, inter, bwd, blocks, s); break;
+    case 8: launch_vec<T, 8, HPG>(a, inter, bwd, blocks, s); break;
+    case 16: launch_vec<T, 16, HPG>(a, inter, bwd, blocks, s); break;
+    default: launch_vec<T, 32, HPG>(a, inter, bwd, blocks, s); break;
+  }
+}
+
+// Launches; the number of blocks (negative) for the backward.
 template <typename T>
-int run(Args a, bool inter, bool bwd, cudaStream_t s) {
-  constexpr int V = Row<T>::kVec;
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  const int half = a.R / 2;
-  bool vec = a.D % V == 0 && a.D / V <= 32 && (inter ? a.R % V == 0 : half % V == 0);
-  if (!inter && a.R > 0) vec = vec && al(a.cos) && al(a.sin);
+int run(Args a, int dtype, bool inter, bool bwd, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);  // channels of a lane, in two pieces of 8 bytes
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; };
+  bool vec = a.D % V == 0 && a.D / V <= 32 && a.R % V == 0 && (a.R == 0 || (al(a.cos) && al(a.sin)));
   for (int i = 0; i < 2; ++i) {
     const Side& d = a.side[i];
-    vec = vec && al(d.x) && al(d.out) && d.x_t % V == 0 && d.x_h % V == 0 && d.o_t % V == 0 && d.o_h % V == 0;
-    if (bwd) vec = vec && al(d.g) && d.g_t % V == 0 && d.g_h % V == 0;
+    vec = vec && al(d.x) && al(d.out) && d.x_t % (V / 2) == 0 && d.x_h % (V / 2) == 0 && d.o_t % (V / 2) == 0 && d.o_h % (V / 2) == 0;
+    if (bwd) vec = vec && al(d.g) && d.g_t % (V / 2) == 0 && d.g_h % (V / 2) == 0;
   }
-  int blocks = 0;
-  if (vec) {
-    int lanes = 4;
-    while (lanes * V < a.D) lanes *= 2;
-    // Heads per group: 4 amortise the token's angles, the weights and the
-    // latency of the first load; 1 where 4 would leave SMs without work.
-    const int64_t rows = a.T * (a.side[0].heads + a.side[1].heads);
-    a.hpg = rows * lanes >= 4ll * 148 * 2048 ? 4 : 1;
-    for (int i = 0; i < 2; ++i) a.side[i].chunks = (a.side[i].heads + a.hpg - 1) / a.hpg;
-    const int64_t groups = a.T * (a.side[0].chunks + a.side[1].chunks);
-    const int64_t need = (groups * lanes + kThreads - 1) / kThreads;
-    if (!bwd && need >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "norm_rotate: too many rows");
-    blocks = bwd ? (int)std::min<int64_t>(need, kBwdBlocks) : (int)need;
-    switch (lanes) {
-      case 4: launch_vec<T, 4>(a, inter, bwd, blocks, s); break;
-      case 8: launch_vec<T, 8>(a, inter, bwd, blocks, s); break;
-      case 16: launch_vec<T, 16>(a, inter, bwd, blocks, s); break;
-      default: launch_vec<T, 32>(a, inter, bwd, blocks, s); break;
-    }
-  } else {
-    const int64_t rows = a.T * (a.side[0].heads + a.side[1].heads);
-    const int64_t need = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    if (!bwd && need >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "norm_rotate: too many rows");
-    blocks = bwd ? (int)std::min<int64_t>(need, kBwdBlocks) : (int)need;
-    if (bwd) backward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
-    else forward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
-  }
+  a.weight_rows = a.wtype == dtype && al(a.side[0].w) && al(a.side[1].w);
+  const int64_t rows = a.T * (a.side[0].heads + a.side[1].heads);
+  int lanes = 4;
+  while (lanes * V < a.D) lanes *= 2;
+  // Heads per group: several amortise the token's angles and the weights and
+  // keep more loads in flight; one where several would leave SMs without work.
+  const int hpg = vec && rows * lanes >= 4ll * 148 * 2048 ? kManyHeads : 1;
+  for (int i = 0; i < 2; ++i) a.side[i].chunks = (a.side[i].heads + hpg - 1) / hpg;
+  const int64_t need = vec ? (a.T * (a.side[0].chunks + a.side[1].chunks) * lanes + kThreads - 1) / kThreads
+                           : (rows + kThreads / 32 - 1) / (kThreads / 32);
+  if (!bwd && need >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "norm_rotate: too many rows");
+  const int blocks = bwd ? (int)std::min<int64_t>(need, kBwdBlocks) : (int)need;
+  if (vec && hpg > 1) launch_lanes<T, kManyHeads>(a, lanes, inter, bwd, blocks, s);
+  else if (vec) launch_lanes<T, 1>(a, lanes, inter, bwd, blocks, s);
+  else if (bwd) backward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
+  else forward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
   return bwd ? -blocks : UPLIFT_LA_OK;
 }
 
@@ -562,9 +617,9 @@ int prepare(const char* what, const uplift_tok_norm_rotate_args* in, bool bwd, A
 }
 
 int run_dtype(const Args& a, int dtype, bool inter, bool bwd, cudaStream_t s) {
-  if (dtype == UPLIFT_LA_F32) return run<float>(a, inter, bwd, s);
-  if (dtype == UPLIFT_LA_BF16) return run<__nv_bfloat16>(a, inter, bwd, s);
-  return run<__half>(a, inter, bwd, s);
+  if (dtype == UPLIFT_LA_F32) return run<float>(a, dtype, inter, bwd, s);
+  if (dtype == UPLIFT_LA_BF16) return run<__nv_bfloat16>(a, dtype, inter, bwd, s);
+  return run<__half>(a, dtype, inter, bwd, s);
 }
 
 }  // namespace nr
