@@ -60,7 +60,7 @@ typedef struct {
   const void* positions;      /* [T] int32, or int64 (positions64), or NULL: row t of the table for token t (P >= T).
                                  Negative: the token is not rotated (class and register tokens).  >= P: its rotated
                                  outputs and its gradients are NaN. */
-  float* dweights;            /* backward only: gradients of q_weight and k_weight, [2][D], written; or NULL */
+  void* dweights;             /* backward only: gradients of q_weight and k_weight, [2][D] of weight_dtype, or NULL */
   float* partial;             /* backward only: workspace of uplift_tok_norm_rotate_partial_floats(D) floats */
   int64_t T, P;
   int32_t Hq, Hk;

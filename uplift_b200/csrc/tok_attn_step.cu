@@ -2,23 +2,28 @@
 // one new token per sequence -- for bf16 / fp16, D <= 128.
 //
 // Each key and value is read once and meets only the Hq / Hk queries of its
-// group, so HBM bounds it: the kernel is built to keep loads in flight.  The
-// keys of a query token are cut into chunks; an item is one chunk for one
-// token and key head, and its group's query heads are the 16 rows of
-// mma.m16n8k16 (fewer are padded, more make further items).  The CTA's four
-// warps take 16 keys in turn, each with its own running maximum and sum:
+// group, so HBM bounds it: the kernel is built to keep loads in flight with
+// few instructions.  The keys of a query token are cut into chunks; an item
+// is one chunk for one token and (up to) eight query heads of a group, which
+// are the N of mma.m16n8k16 (fewer are padded, more make further items).  The
+// CTA's four warps take 16 keys in turn, each with its own running maximum
+// and sum, and everything is transposed, so that the few heads are the short
+// side of the products:
 //
-//   S[16 x 16] = Q K^T,  P = exp2((S - m) scale log2 e),  O[16 x D] += P V
+//   S^T[16 keys x 8] = K Q^T,  P = exp2((S - m) scale log2 e),
+//   O^T[D x 8] += V^T P^T
 //
 // K and V go from global memory straight into the registers of the MMA
 // fragments, 16 bytes per load: the order of the channels in a product does
 // not matter, so a lane takes 8 neighbouring channels of a key as its part of
-// two k-steps (Q is laid out alike), and 8 neighbouring channels of four keys
-// of V as its columns of eight n-tiles (pairs of keys are merged by byte
-// permutes).  The next K is loaded while the weights are formed, V while the
-// scores are.  The warps' results are joined in shared memory; the chunks'
-// results go to a workspace and a second kernel joins them, unless the
-// token has one chunk only.
+// two k-steps of K (Q is laid out alike), and 8 neighbouring channels of four
+// keys of V as its rows of four m-tiles (pairs of keys are merged by byte
+// permutes).  P^T changes from accumulator to operand layout with movmatrix.
+// V is loaded while the scores are formed, the next K while the weights are.
+// The maximum is shared between a warp's lanes only when one of them saw it
+// grow by more than 2^8.  The warps' results are joined in shared memory; the
+// chunks' results go to a workspace and a second kernel joins them, unless
+// the token has one chunk only.
 
 #include <math.h>
 
@@ -34,10 +39,13 @@ namespace step {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;          // keys of a warp at a time
-constexpr int kRows = 16;          // query heads of an item
+constexpr int kRows = 8;           // query heads of an item
 constexpr int kMinChunk = kWarps * kKeys;
 constexpr int kMaxChunks = 128;    // of one token
-constexpr int kCtasPerSm = 3;
+#ifndef ULA_STEP_CTAS
+#define ULA_STEP_CTAS 4
+#endif
+constexpr int kCtasPerSm = ULA_STEP_CTAS;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;    // see tok_attn_fwd.cu
 
@@ -48,7 +56,7 @@ struct Params {
   float2* part_ml; // [T][chunks][Hq]: maximum (of scale S log2 e) and sum
   Packing pk;
   int Hq, Hk, group, D;
-  int row_tiles;   // ceil(group / 16)
+  int row_tiles;   // ceil(group / 8)
   int chunks;      // at most, per token
   int min_len;     // least keys of a chunk
   float scale;
@@ -76,19 +84,38 @@ template <> struct Mma<__half> {
   }
 };
 
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// Lanes with the same t (lane & 3): the keys of two heads.
+__device__ __forceinline__ float keys_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float keys_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 // Loads that are not kept in L1: every byte is used once.
-__device__ __forceinline__ uint4 load16(const void* p, bool there) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (there) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
+}
+__device__ __forceinline__ uint4 load16_if(const void* p, bool there) {  // zeros if not there; no branch
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}\n"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((uint32_t)there));
+  return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
 }
 
 // Units of a sequence: one per query token and chunk of its keys.
@@ -130,7 +157,8 @@ struct UnitWalk {
   }
 };
 
-template <typename T, int DP>
+// FULL: D == DP, no channel is missing.
+template <typename T, int DP, bool FULL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Params p) {
   constexpr int KB = DP / 32;  // blocks of 32 channels of Q and K
   constexpr int VB = DP / 64;  // blocks of 64 channels of V
@@ -157,122 +185,122 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
     const int j0 = chunk * len, j1 = min(see, j0 + len);
     if (j0 >= j1) continue;  // this token sees none of the chunk (the whole CTA skips it)
     const int64_t row = s.q0 + tok;
-    // Q: rows g and g + 8, 8 channels of each block of 32
-    uint32_t qa[KB][2][4];
+    // Q^T: head g, 8 channels of each block of 32
+    uint32_t qb[KB][4];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
       const int c = 32 * b + 8 * t;
-      const T* q = static_cast<const T*>(p.q.p) + row * p.q.t + (int64_t)h0 * p.q.h + c;
-      const uint4 lo = load16(q + g * p.q.h, g < rows && c < p.D);
-      const uint4 hi = load16(q + (g + 8) * p.q.h, g + 8 < rows && c < p.D);
-      qa[b][0][0] = lo.x; qa[b][0][1] = hi.x; qa[b][0][2] = lo.y; qa[b][0][3] = hi.y;
-      qa[b][1][0] = lo.z; qa[b][1][1] = hi.z; qa[b][1][2] = lo.w; qa[b][1][3] = hi.w;
+      const uint4 v = load16_if(static_cast<const T*>(p.q.p) + row * p.q.t + (int64_t)(h0 + g) * p.q.h + c, g < rows && c < p.D);
+      qb[b][0] = v.x; qb[b][1] = v.y; qb[b][2] = v.z; qb[b][3] = v.w;
     }
-    const T* kb = static_cast<const T*>(p.k.p) + (int64_t)s.k0 * p.k.t + (int64_t)hk * p.k.h + 8 * t;
-    const T* vb = static_cast<const T*>(p.v.p) + (int64_t)s.k0 * p.v.t + (int64_t)hk * p.v.h + 8 * g;
-    uint4 kr[KB][2];
-    auto load_k = [&](int j) {  // keys j + g, j + 8 + g
+    // keys j + g, j + 8 + g of K, and j + 2t, + 2t + 1, + 2t + 8, + 2t + 9 of V
+    int j = j0 + warp * kKeys;
+    const int64_t k8 = 8 * p.k.t, k_step = (int64_t)kMinChunk * p.k.t, v_step = (int64_t)kMinChunk * p.v.t;
+    const T* kp = static_cast<const T*>(p.k.p) + (int64_t)(s.k0 + j + g) * p.k.t + (int64_t)hk * p.k.h + 8 * t;
+    const T* vp = static_cast<const T*>(p.v.p) + (int64_t)(s.k0 + j + 2 * t) * p.v.t + (int64_t)hk * p.v.h + 8 * g;
+    uint4 kr[KB][2], vr[VB][4];
+    auto load_k = [&](int jj) {
+      const bool whole = jj + kKeys <= j1;
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          kr[b][u] = load16(kb + (int64_t)(j + 8 * u + g) * p.k.t + 32 * b, j + 8 * u + g < j1 && 32 * b + 8 * t < p.D);
+        for (int b = 0; b < KB; ++b) {
+          const T* at = kp + u * k8 + 32 * b;
+          if (FULL && whole) kr[b][u] = load16(at);
+          else kr[b][u] = load16_if(at, jj + 8 * u + g < j1 && (FULL || 32 * b + 8 * t < p.D));
+        }
       }
+      kp += k_step;
     };
-    float acc[VB][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    auto load_v = [&](int jj) {
+      const bool whole = jj + kKeys <= j1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = (e & 1) + 8 * (e >> 1);
+#pragma unroll
+        for (int b = 0; b < VB; ++b) {
+          const T* at = vp + key * p.v.t + 64 * b;
+          if (FULL && whole) vr[b][e] = load16(at);
+          else vr[b][e] = load16_if(at, jj + 2 * t + key < j1 && (FULL || 64 * b + 8 * g < p.D));
+        }
+      }
+      vp += v_step;
+    };
+    float acc[VB][4][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2t, 2t + 1
 #pragma unroll
     for (int b = 0; b < VB; ++b) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[b][e][0] = acc[b][e][1] = acc[b][e][2] = acc[b][e][3] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[b][e][0] = acc[b][e][1] = acc[b][e][2] = acc[b][e][3] = 0.f;
     }
-    int j = j0 + warp * kKeys;
     if (j < j1) load_k(j);
+#pragma unroll 1
     for (; j < j1; j += kMinChunk) {
-      uint4 vr[VB][4];  // keys j + 2t, + 2t + 1, + 2t + 8, + 2t + 9
-#pragma unroll
-      for (int b = 0; b < VB; ++b) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = j + 2 * t + (e & 1) + 8 * (e >> 1);
-          vr[b][e] = load16(vb + (int64_t)key * p.v.t + 64 * b, key < j1 && 64 * b + 8 * g < p.D);
-        }
-      }
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      load_v(j);
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};  // key g: heads 2t, 2t + 1; key g + 8: the same
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          Mma<T>::run(sc[u], qa[b][0], kr[b][u].x, kr[b][u].y);
-          Mma<T>::run(sc[u], qa[b][1], kr[b][u].z, kr[b][u].w);
-        }
+        const uint32_t a0[4] = {kr[b][0].x, kr[b][1].x, kr[b][0].y, kr[b][1].y};
+        const uint32_t a1[4] = {kr[b][0].z, kr[b][1].z, kr[b][0].w, kr[b][1].w};
+        Mma<T>::run(sc, a0, qb[b][0], qb[b][1]);
+        Mma<T>::run(sc, a1, qb[b][2], qb[b][3]);
       }
       if (j + kMinChunk < j1) load_k(j + kMinChunk);
       if (j + kKeys > j1) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (j + 8 * u + 2 * t + (e & 1) >= j1) sc[u][e] = -INFINITY;
-        }
+        if (j + g >= j1) sc[0] = sc[1] = -INFINITY;
+        if (j + g + 8 >= j1) sc[2] = sc[3] = -INFINITY;
       }
-      uint32_t pa[4];
+      const float mx[2] = {fmaxf(sc[0], sc[2]) * c2, fmaxf(sc[1], sc[3]) * c2};
+      if (__any_sync(0xffffffffu, mx[0] - m[0] > kRescale || mx[1] - m[1] > kRescale)) {  // also from m = -inf
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // rows g, g + 8
-        const float mx = quad_max(fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]))) * c2;
-        const bool grow = mx - m[h] > kRescale || (m[h] == -INFINITY && mx > m[h]);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? ex2(m[h] - mx) : 1.f;  // exp2(-inf) = 0 at the first keys
-          if (grow) m[h] = mx;
+        for (int h = 0; h < 2; ++h) {
+          const float mn = fmaxf(m[h], keys_max(mx[h]));
+          const float f = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
+          m[h] = mn;
           l[h] *= f;
 #pragma unroll
           for (int b = 0; b < VB; ++b) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              acc[b][e][2 * h] *= f;
-              acc[b][e][2 * h + 1] *= f;
+            for (int e = 0; e < 4; ++e) {
+              acc[b][e][h] *= f;
+              acc[b][e][2 + h] *= f;
             }
           }
         }
-        const float mm = m[h] == -INFINITY ? 0.f : m[h];
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = ex2(fmaf(sc[e >> 1][2 * h + (e & 1)], c2, -mm));
-        l[h] += (w[0] + w[1]) + (w[2] + w[3]);
-        pa[h] = St<T>::pack(w[0], w[1]);
-        pa[2 + h] = St<T>::pack(w[2], w[3]);
       }
+      const float mm[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = ex2(fmaf(sc[e], c2, mm[e & 1]));
+      l[0] += w[0] + w[2];
+      l[1] += w[1] + w[3];
+      const uint32_t p0 = transpose8x8(St<T>::pack(w[0], w[1]));  // head g, keys 2t, 2t + 1
+      const uint32_t p1 = transpose8x8(St<T>::pack(w[2], w[3]));  // keys 2t + 8, 2t + 9
 #pragma unroll
       for (int b = 0; b < VB; ++b) {
-        const uint32_t* x[4];
+        const uint32_t x[4][4] = {{vr[b][0].x, vr[b][0].y, vr[b][0].z, vr[b][0].w}, {vr[b][1].x, vr[b][1].y, vr[b][1].z, vr[b][1].w},
+                                  {vr[b][2].x, vr[b][2].y, vr[b][2].z, vr[b][2].w}, {vr[b][3].x, vr[b][3].y, vr[b][3].z, vr[b][3].w}};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = &vr[b][e].x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // channels 8g + 2e, 8g + 2e + 1
-          Mma<T>::run(acc[b][2 * e], pa, __byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x5410));
-          Mma<T>::run(acc[b][2 * e + 1], pa, __byte_perm(x[0][e], x[1][e], 0x7632), __byte_perm(x[2][e], x[3][e], 0x7632));
+        for (int e = 0; e < 4; ++e) {  // rows g, g + 8 of the tile: channels 8g + 2e, 8g + 2e + 1
+          const uint32_t a[4] = {__byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[0][e], x[1][e], 0x7632),
+                                 __byte_perm(x[2][e], x[3][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x7632)};
+          Mma<T>::run(acc[b][e], a, p0, p1);
         }
       }
     }
     // join the warps
 #pragma unroll
-    for (int h = 0; h < 2; ++h) l[h] = quad_sum(l[h]);
-    if (t == 0) {
-      s_m[warp][g] = m[0];
-      s_m[warp][g + 8] = m[1];
-      s_l[warp][g] = l[0];
-      s_l[warp][g + 8] = l[1];
-    }
-#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (g + 8 * h < rows) {
+      l[h] = keys_sum(l[h]);
+      if (g == 0) {
+        s_m[warp][2 * t + h] = m[h];
+        s_l[warp][2 * t + h] = l[h];
+      }
+      if (2 * t + h < rows) {
 #pragma unroll
         for (int b = 0; b < VB; ++b) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {  // accumulator columns 2t, 2t + 1: channels 8 (2t + n) + e
-            float* o = &s_o[warp][g + 8 * h][64 * b + 8 * (2 * t + n)];
-            *reinterpret_cast<float4*>(o) = make_float4(acc[b][0][2 * h + n], acc[b][1][2 * h + n], acc[b][2][2 * h + n], acc[b][3][2 * h + n]);
-            *reinterpret_cast<float4*>(o + 4) = make_float4(acc[b][4][2 * h + n], acc[b][5][2 * h + n], acc[b][6][2 * h + n], acc[b][7][2 * h + n]);
-          }
+          float* o = &s_o[warp][2 * t + h][64 * b + 8 * g];
+          *reinterpret_cast<float4*>(o) = make_float4(acc[b][0][h], acc[b][0][2 + h], acc[b][1][h], acc[b][1][2 + h]);
+          *reinterpret_cast<float4*>(o + 4) = make_float4(acc[b][2][h], acc[b][2][2 + h], acc[b][3][h], acc[b][3][2 + h]);
         }
       }
     }
@@ -403,7 +431,8 @@ template <typename T, int DP>
 int run(const Params& p, int sms, cudaStream_t s) {
   const int64_t most = (int64_t)p.pk.T * p.chunks * p.Hk * p.row_tiles;
   const int grid = (int)std::min<int64_t>(most, (int64_t)sms * kCtasPerSm);
-  chunk_kernel<T, DP><<<grid, kThreads, 0, s>>>(p);
+  if (p.D == DP) chunk_kernel<T, DP, true><<<grid, kThreads, 0, s>>>(p);
+  else chunk_kernel<T, DP, false><<<grid, kThreads, 0, s>>>(p);
   int rc = launched("attention");
   if (rc != UPLIFT_LA_OK) return rc;
   cudaLaunchConfig_t cfg = {};

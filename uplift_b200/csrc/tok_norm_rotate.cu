@@ -28,11 +28,9 @@ namespace tok {
 namespace nr {
 
 constexpr int kThreads = 256;
-#ifndef ULA_NR_HPG
-#define ULA_NR_HPG 4
-#endif
-constexpr int kManyHeads = ULA_NR_HPG;
-constexpr int kBwdBlocks = 148 * 4;  // fixed, so the order of the dw sums does not depend on the problem's size
+constexpr int kManyHeads = 8, kManyHeadsBwd = 4;  // heads that a group of lanes takes, forward and backward
+constexpr int kBwdBlocks = 148 * 2;  // of the backward: what the SMs hold at once
+constexpr int kMaxBwdY = 64;         // of these, over the heads of one side
 
 struct Side {  // queries or keys
   const void* x; int64_t x_t, x_h;
@@ -40,6 +38,7 @@ struct Side {  // queries or keys
   void* out;     int64_t o_t, o_h;   // forward: the output; backward: dx
   const void* w;
   int heads, chunks;                 // chunks of heads that one group of lanes takes
+  int blocks_y;                      // backward: blockIdx.y values of this side
 };
 
 struct Args {
@@ -52,7 +51,7 @@ struct Args {
   int64_t T, P;
   int D, R;
   float eps, inv_d;
-  float* partial;  // backward: [2][kBwdBlocks][D]
+  float* partial;  // backward: a row of D sums per block
   int want_dw;
 };
 
@@ -235,27 +234,22 @@ struct Lane {
   }
 };
 
-// Forward.  Group g of LANES lanes: token g / chunks, HPG heads of one side.
-// All rows are loaded before the first is used, and the token's angles times
+// Forward.  A group of LANES lanes takes one token and HPG heads of one side
+// (blockIdx.y).  All rows are loaded before the first is used, and the token's angles times
 // the weights serve all of them:
 //   za = r (xa (wa c) - xb (wb s)),  zb = r (xb (wb c) + xa (wa s)).
-// Out-of-range groups compute on the last group's rows and store nothing, so
-// that every lane of a warp takes part in the shuffles.
+// Groups behind the last token compute on its rows and store nothing, so that
+// every lane of a warp takes part in the shuffles.
 template <typename T, int LANES, bool INTER, int HPG>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   constexpr int N = Row<T, INTER>::kPairs;
   const Lane<T, LANES, INTER> ln(a);
-  const int chunks = a.side[0].chunks + a.side[1].chunks;
-  const int64_t groups = a.T * chunks;
-  int64_t g = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const bool live = g < groups;
-  g = min(g, groups - 1);
-  const int64_t t = g / chunks;
-  int ch = (int)(g - t * chunks);
-  const int which = ch >= a.side[0].chunks;
+  const int which = blockIdx.y >= a.side[0].chunks;
   const Side& sd = a.side[which];
-  if (which) ch -= a.side[0].chunks;
-  const int h0 = ch * HPG;
+  const int h0 = ((int)blockIdx.y - (which ? a.side[0].chunks : 0)) * HPG;
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const bool live = at < a.T;
+  const int64_t t = min(at, a.T - 1);
   const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h0 * sd.x_h + ln.c0;
   T* out = static_cast<T*>(sd.out) + t * sd.o_t + h0 * sd.o_h + ln.c0;
   Row<T, INTER> rows[HPG] = {};
@@ -296,30 +290,26 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   }
 }
 
-// Backward.  Blocks stride over the groups; each lane sums its channels' dw
-// over its rows, first of all query rows, then of all key rows.
+// Backward.  Blocks stride over the tokens with the heads of one chunk
+// (blockIdx.y); each lane sums its channels' dw over its rows.
 template <typename T, int LANES, bool INTER, int HPG>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Args a) {
   constexpr int V = Row<T, INTER>::kVec, N = V / 2;
   constexpr int kGroups = kThreads / LANES;
   __shared__ float red[kGroups * LANES * V];
   const Lane<T, LANES, INTER> ln(a);
   const int gi = threadIdx.x / LANES;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Side& sd = a.side[which];
-    float wa[N], wb[N], dwa[N], dwb[N];
-    ln.weights(a, sd.w, wa, wb);
+  const int which = blockIdx.y >= a.side[0].blocks_y;
+  const Side& sd = a.side[which];
+  float wa[N], wb[N], dwa[N], dwb[N];
+  ln.weights(a, sd.w, wa, wb);
 #pragma unroll
-    for (int i = 0; i < N; ++i) dwa[i] = dwb[i] = 0.f;
-    const int64_t groups = a.T * sd.chunks;
-    const int64_t rounds = (groups + (int64_t)gridDim.x * kGroups - 1) / ((int64_t)gridDim.x * kGroups);
-    for (int64_t n = 0; n < rounds; ++n) {
-      int64_t g = (n * gridDim.x + blockIdx.x) * kGroups + gi;
-      const bool live = g < groups;
-      g = min(g, groups - 1);
-      const int64_t t = g / sd.chunks;
-      const int h0 = (int)(g - t * sd.chunks) * HPG;
+  for (int i = 0; i < N; ++i) dwa[i] = dwb[i] = 0.f;
+  for (int ch = (int)blockIdx.y - (which ? a.side[0].blocks_y : 0); ch < sd.chunks; ch += sd.blocks_y) {
+    const int h0 = ch * HPG;
+    for (int64_t t0 = (int64_t)blockIdx.x * kGroups; t0 < a.T; t0 += (int64_t)gridDim.x * kGroups) {
+      const bool live = t0 + gi < a.T;
+      const int64_t t = min(t0 + gi, a.T - 1);
       const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h0 * sd.x_h + ln.c0;
       const T* gz = static_cast<const T*>(sd.g) + t * sd.g_t + h0 * sd.g_h + ln.c0;
       T* out = static_cast<T*>(sd.out) + t * sd.o_t + h0 * sd.o_h + ln.c0;
@@ -375,24 +365,23 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args a) {
         }
       }
     }
-    if (a.want_dw) {
-      // the block's groups in ascending order
-      __syncthreads();
-      if (ln.active) {
+  }
+  if (a.want_dw) {
+    // the block's groups in ascending order
+    if (ln.active) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int ch = INTER ? ln.c0 + 2 * i : ln.c0 + i;
-          red[gi * LANES * V + ch] = dwa[i];
-          red[gi * LANES * V + (INTER ? ch + 1 : ch + ln.step)] = dwb[i];
-        }
+      for (int i = 0; i < N; ++i) {
+        const int ch = INTER ? ln.c0 + 2 * i : ln.c0 + i;
+        red[gi * LANES * V + ch] = dwa[i];
+        red[gi * LANES * V + (INTER ? ch + 1 : ch + ln.step)] = dwb[i];
       }
-      __syncthreads();
-      for (int d = threadIdx.x; d < a.D; d += kThreads) {
-        float sum = 0.f;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += kThreads) {
+      float sum = 0.f;
 #pragma unroll 8
-        for (int k = 0; k < kGroups; ++k) sum += red[k * LANES * V + d];
-        a.partial[((int64_t)which * gridDim.x + blockIdx.x) * a.D + d] = sum;
-      }
+      for (int k = 0; k < kGroups; ++k) sum += red[k * LANES * V + d];
+      a.partial[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.D + d] = sum;
     }
   }
 }
@@ -441,87 +430,97 @@ __global__ void __launch_bounds__(kThreads) backward_any_kernel(const Args a, in
   __shared__ float red[kWarps * UPLIFT_TOK_MAX_NORM_DIM];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = a.R / 2;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Side& sd = a.side[which];
-    float dw[kPer];
+  const Side& sd = a.side[blockIdx.y];
+  float dw[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) dw[j] = 0.f;
-    const int64_t rows = a.T * sd.heads;
-    for (int64_t row = (int64_t)blockIdx.x * kWarps + warp; row < rows; row += (int64_t)gridDim.x * kWarps) {
-      const int64_t t = row / sd.heads;
-      const int h = (int)(row - t * sd.heads);
-      const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h * sd.x_h;
-      const T* gz = static_cast<const T*>(sd.g) + t * sd.g_t + h * sd.g_h;
-      T* out = static_cast<T*>(sd.out) + t * sd.o_t + h * sd.o_h;
-      const int64_t tr = table_row(a, t);
-      float gy[kPer], v[kPer], w[kPer];
-      float sq = 0.f, dot = 0.f;
+  for (int j = 0; j < kPer; ++j) dw[j] = 0.f;
+  const int64_t rows = a.T * sd.heads;
+  for (int64_t row = (int64_t)blockIdx.x * kWarps + warp; row < rows; row += (int64_t)gridDim.x * kWarps) {
+    const int64_t t = row / sd.heads;
+    const int h = (int)(row - t * sd.heads);
+    const T* x = static_cast<const T*>(sd.x) + t * sd.x_t + h * sd.x_h;
+    const T* gz = static_cast<const T*>(sd.g) + t * sd.g_t + h * sd.g_h;
+    T* out = static_cast<T*>(sd.out) + t * sd.o_t + h * sd.o_h;
+    const int64_t tr = table_row(a, t);
+    float gy[kPer], v[kPer], w[kPer];
+    float sq = 0.f, dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int i = lane + 32 * j;
-        gy[j] = v[j] = w[j] = 0.f;
-        if (i < a.D) {
-          v[j] = St<T>::f(x[i]);
-          w[j] = weight_at(sd.w, a.wtype, i);
-          float g = St<T>::f(gz[i]);
-          if (i < a.R && tr != -1) {
-            const bool second = inter ? (i & 1) : i >= half;
-            const int ip = inter ? (i ^ 1) : (second ? i - half : i + half);
-            const int64_t pair = inter ? i >> 1 : (second ? ip : i);
-            const float gp = St<T>::f(gz[ip]);
-            if (tr == -2) g = __int_as_float(0x7fc00000);
-            else g = fmaf(g, a.cos[tr * half + pair], gp * (second ? -a.sin[tr * half + pair] : a.sin[tr * half + pair]));
-          }
-          gy[j] = g;
+    for (int j = 0; j < kPer; ++j) {
+      const int i = lane + 32 * j;
+      gy[j] = v[j] = w[j] = 0.f;
+      if (i < a.D) {
+        v[j] = St<T>::f(x[i]);
+        w[j] = weight_at(sd.w, a.wtype, i);
+        float g = St<T>::f(gz[i]);
+        if (i < a.R && tr != -1) {
+          const bool second = inter ? (i & 1) : i >= half;
+          const int ip = inter ? (i ^ 1) : (second ? i - half : i + half);
+          const int64_t pair = inter ? i >> 1 : (second ? ip : i);
+          const float gp = St<T>::f(gz[ip]);
+          if (tr == -2) g = __int_as_float(0x7fc00000);
+          else g = fmaf(g, a.cos[tr * half + pair], gp * (second ? -a.sin[tr * half + pair] : a.sin[tr * half + pair]));
         }
-        sq = fmaf(v[j], v[j], sq);
-        dot = fmaf(gy[j] * w[j], v[j], dot);
+        gy[j] = g;
       }
-      sq = group_sum<32>(sq);
-      dot = group_sum<32>(dot);
-      const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
-      const float m = dot * r * a.inv_d;
+      sq = fmaf(v[j], v[j], sq);
+      dot = fmaf(gy[j] * w[j], v[j], dot);
+    }
+    sq = group_sum<32>(sq);
+    dot = group_sum<32>(dot);
+    const float r = rsqrtf(fmaf(sq, a.inv_d, a.eps));
+    const float m = dot * r * a.inv_d;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int i = lane + 32 * j;
-        if (i < a.D) {
-          const float hh = v[j] * r;
-          out[i] = St<T>::t(r * fmaf(-hh, m, gy[j] * w[j]));
-          dw[j] = fmaf(gy[j], hh, dw[j]);
-        }
+    for (int j = 0; j < kPer; ++j) {
+      const int i = lane + 32 * j;
+      if (i < a.D) {
+        const float hh = v[j] * r;
+        out[i] = St<T>::t(r * fmaf(-hh, m, gy[j] * w[j]));
+        dw[j] = fmaf(gy[j], hh, dw[j]);
       }
     }
-    if (a.want_dw) {
-      __syncthreads();
+  }
+  if (a.want_dw) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) red[warp * UPLIFT_TOK_MAX_NORM_DIM + lane + 32 * j] = dw[j];
-      __syncthreads();
-      for (int d = threadIdx.x; d < a.D; d += kThreads) {
-        float sum = 0.f;
-        for (int k = 0; k < kWarps; ++k) sum += red[k * UPLIFT_TOK_MAX_NORM_DIM + d];
-        a.partial[((int64_t)which * gridDim.x + blockIdx.x) * a.D + d] = sum;
-      }
+    for (int j = 0; j < kPer; ++j) red[warp * UPLIFT_TOK_MAX_NORM_DIM + lane + 32 * j] = dw[j];
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += kThreads) {
+      float sum = 0.f;
+      for (int k = 0; k < kWarps; ++k) sum += red[k * UPLIFT_TOK_MAX_NORM_DIM + d];
+      a.partial[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.D + d] = sum;
     }
   }
 }
 
-// dweights[which][d] = sum over blocks of partial[which][block][d], in a
-// fixed order (a warp per output, lanes over blocks) and in 64 bits: the sum
-// runs over all rows of the problem.
-__global__ void __launch_bounds__(kThreads) dweights_kernel(const float* partial, float* dweights, int blocks, int D) {
-  const int out = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (out >= 2 * D) return;
-  const int which = out / D, d = out - which * D;
+// dweights[which][d] = sum of the side's rows of partials (rows0 of the
+// queries, then rows1 of the keys), in a fixed order (32 channels a block, a
+// warp every 32nd row) and in 64 bits: the sum runs over all rows of the
+// problem.
+__global__ void __launch_bounds__(1024) dweights_kernel(const float* partial, void* dweights, int wtype, int rows0, int rows1, int D) {
+  __shared__ double red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int which = blockIdx.y, d = blockIdx.x * 32 + lane;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double sum = 0.0;
-  for (int b = lane; b < blocks; b += 32) sum += (double)partial[((int64_t)which * blocks + b) * D + d];
+  if (d < D) {
+#pragma unroll 8
+    for (int b = warp; b < (which ? rows1 : rows0); b += 32) sum += (double)partial[((int64_t)(which ? rows0 : 0) + b) * D + d];
+  }
+  red[warp][lane] = sum;
+  __syncthreads();
+  sum = red[lane][warp];  // channel `warp` of the block, partial sum `lane`
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) dweights[out] = (float)sum;
+  const int out = blockIdx.x * 32 + warp;
+  if (lane == 0 && out < D) {
+    const int64_t at = (int64_t)which * D + out;
+    if (wtype == UPLIFT_LA_F32) static_cast<float*>(dweights)[at] = (float)sum;
+    else if (wtype == UPLIFT_LA_BF16) static_cast<__nv_bfloat16*>(dweights)[at] = __double2bfloat16(sum);
+    else static_cast<__half*>(dweights)[at] = __double2half(sum);
+  }
 }
 
 template <typename T, int LANES, int HPG>
-void launch_vec(const Args& a, bool inter, bool bwd, int blocks, cudaStream_t s) {
+void launch_vec(const Args& a, bool inter, bool bwd, dim3 blocks, cudaStream_t s) {
   if (bwd) {
     if (inter) backward_kernel<T, LANES, true, HPG><<<blocks, kThreads, 0, s>>>(a);
     else backward_kernel<T, LANES, false, HPG><<<blocks, kThreads, 0, s>>>(a);
@@ -532,7 +531,7 @@ void launch_vec(const Args& a, bool inter, bool bwd, int blocks, cudaStream_t s)
 }
 
 template <typename T, int HPG>
-void launch_lanes(const Args& a, int lanes, bool inter, bool bwd, int blocks, cudaStream_t s) {
+void launch_lanes(const Args& a, int lanes, bool inter, bool bwd, dim3 blocks, cudaStream_t s) {
   switch (lanes) {
     case 4: launch_vec<T, 4, HPG>(a, inter, bwd, blocks, s); break;
     case 8: launch_vec<T, 8, HPG>(a, inter, bwd, blocks, s); break;
@@ -541,9 +540,9 @@ void launch_lanes(const Args& a, int lanes, bool inter, bool bwd, int blocks, cu
   }
 }
 
-// Launches; the number of blocks (negative) for the backward.
+// Launches; *rows: rows of partials that the backward writes for each side.
 template <typename T>
-int run(Args a, int dtype, bool inter, bool bwd, cudaStream_t s) {
+int run(Args a, int dtype, bool inter, bool bwd, int* partial_rows, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);  // channels of a lane, in two pieces of 8 bytes
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; };
   bool vec = a.D % V == 0 && a.D / V <= 32 && a.R % V == 0 && (a.R == 0 || (al(a.cos) && al(a.sin)));
@@ -558,17 +557,28 @@ int run(Args a, int dtype, bool inter, bool bwd, cudaStream_t s) {
   while (lanes * V < a.D) lanes *= 2;
   // Heads per group: several amortise the token's angles and the weights and
   // keep more loads in flight; one where several would leave SMs without work.
-  const int hpg = vec && rows * lanes >= 4ll * 148 * 2048 ? kManyHeads : 1;
+  const int hpg = vec && rows * lanes >= 4ll * 148 * 2048 ? (bwd ? kManyHeadsBwd : kManyHeads) : 1;
   for (int i = 0; i < 2; ++i) a.side[i].chunks = (a.side[i].heads + hpg - 1) / hpg;
-  const int64_t need = vec ? (a.T * (a.side[0].chunks + a.side[1].chunks) * lanes + kThreads - 1) / kThreads
-                           : (rows + kThreads / 32 - 1) / (kThreads / 32);
-  if (!bwd && need >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "norm_rotate: too many rows");
-  const int blocks = bwd ? (int)std::min<int64_t>(need, kBwdBlocks) : (int)need;
-  if (vec && hpg > 1) launch_lanes<T, kManyHeads>(a, lanes, inter, bwd, blocks, s);
-  else if (vec) launch_lanes<T, 1>(a, lanes, inter, bwd, blocks, s);
-  else if (bwd) backward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
+  if (bwd) {
+    // vec: tokens over x, chunks of heads over y; else rows over x, sides over y
+    const int per_block = vec ? kThreads / lanes : kThreads / 32;
+    for (int i = 0; i < 2; ++i) a.side[i].blocks_y = vec ? std::min(a.side[i].chunks, kMaxBwdY) : 1;
+    const int y = a.side[0].blocks_y + a.side[1].blocks_y;
+    const int64_t x = vec ? (a.T + per_block - 1) / per_block : (rows + per_block - 1) / per_block;
+    const dim3 blocks((unsigned)std::min<int64_t>(x, std::max(1, kBwdBlocks / y)), y);
+    for (int i = 0; i < 2; ++i) partial_rows[i] = (int)blocks.x * a.side[i].blocks_y;
+    if (vec && hpg > 1) launch_lanes<T, kManyHeadsBwd>(a, lanes, inter, true, blocks, s);
+    else if (vec) launch_lanes<T, 1>(a, lanes, inter, true, blocks, s);
+    else backward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
+    return UPLIFT_LA_OK;
+  }
+  const int64_t x = vec ? (a.T * lanes + kThreads - 1) / kThreads : (rows + kThreads / 32 - 1) / (kThreads / 32);
+  if (x >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "norm_rotate: too many rows");
+  const dim3 blocks((unsigned)x, vec ? a.side[0].chunks + a.side[1].chunks : 1);
+  if (vec && hpg > 1) launch_lanes<T, kManyHeads>(a, lanes, inter, false, blocks, s);
+  else if (vec) launch_lanes<T, 1>(a, lanes, inter, false, blocks, s);
   else forward_any_kernel<T><<<blocks, kThreads, 0, s>>>(a, inter);
-  return bwd ? -blocks : UPLIFT_LA_OK;
+  return UPLIFT_LA_OK;
 }
 
 // Validates the arguments and fills `a`.
@@ -579,7 +589,7 @@ int prepare(const char* what, const uplift_tok_norm_rotate_args* in, bool bwd, A
     return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, dt);
   if (wt != UPLIFT_LA_F32 && wt != UPLIFT_LA_BF16 && wt != UPLIFT_LA_F16)
     return fail(UPLIFT_LA_ERR_ARG, "%s: unknown weight dtype %d", what, wt);
-  if (in->T < 0 || in->T >= (1ll << 31) || in->P < 0 || in->Hq < 1 || in->Hk < 1 || in->Hq > 65536 || in->Hk > 65536)
+  if (in->T < 0 || in->T >= (1ll << 31) || in->P < 0 || in->Hq < 1 || in->Hk < 1 || in->Hq > 32767 || in->Hk > 32767)
     return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes T=%lld P=%lld Hq=%d Hk=%d", what, (long long)in->T,
                 (long long)in->P, in->Hq, in->Hk);
   if (in->D < 1 || in->D > UPLIFT_TOK_MAX_NORM_DIM)
@@ -616,10 +626,10 @@ int prepare(const char* what, const uplift_tok_norm_rotate_args* in, bool bwd, A
   return UPLIFT_LA_OK;
 }
 
-int run_dtype(const Args& a, int dtype, bool inter, bool bwd, cudaStream_t s) {
-  if (dtype == UPLIFT_LA_F32) return run<float>(a, dtype, inter, bwd, s);
-  if (dtype == UPLIFT_LA_BF16) return run<__nv_bfloat16>(a, dtype, inter, bwd, s);
-  return run<__half>(a, dtype, inter, bwd, s);
+int run_dtype(const Args& a, int dtype, bool inter, bool bwd, int* partial_rows, cudaStream_t s) {
+  if (dtype == UPLIFT_LA_F32) return run<float>(a, dtype, inter, bwd, partial_rows, s);
+  if (dtype == UPLIFT_LA_BF16) return run<__nv_bfloat16>(a, dtype, inter, bwd, partial_rows, s);
+  return run<__half>(a, dtype, inter, bwd, partial_rows, s);
 }
 
 }  // namespace nr
@@ -634,12 +644,12 @@ int uplift_tok_norm_rotate(const uplift_tok_norm_rotate_args* args, void* stream
   Args a;
   int rc = prepare("uplift_tok_norm_rotate", args, false, &a);
   if (rc != UPLIFT_LA_OK || args->T == 0) return rc;
-  rc = run_dtype(a, args->dtype, args->interleaved != 0, false, static_cast<cudaStream_t>(stream));
+  rc = run_dtype(a, args->dtype, args->interleaved != 0, false, nullptr, static_cast<cudaStream_t>(stream));
   return rc != UPLIFT_LA_OK ? rc : tok::launched("norm_rotate");
 }
 
 int64_t uplift_tok_norm_rotate_partial_floats(int D) {
-  return D < 1 ? 0 : 2ll * ula::tok::nr::kBwdBlocks * D;
+  return D < 1 ? 0 : (int64_t)ula::tok::nr::kBwdBlocks * D;
 }
 
 int uplift_tok_norm_rotate_backward(const uplift_tok_norm_rotate_args* args, void* stream) {
@@ -649,16 +659,25 @@ int uplift_tok_norm_rotate_backward(const uplift_tok_norm_rotate_args* args, voi
   int rc = prepare("uplift_tok_norm_rotate_backward", args, true, &a);
   if (rc != UPLIFT_LA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int blocks = 0;
+  int partial_rows[2] = {0, 0};
   if (args->T > 0) {
-    rc = run_dtype(a, args->dtype, args->interleaved != 0, true, s);
-    if (rc > 0) return rc;
-    blocks = -rc;
+    rc = run_dtype(a, args->dtype, args->interleaved != 0, true, partial_rows, s);
+    if (rc != UPLIFT_LA_OK) return rc;
     if ((rc = tok::launched("norm_rotate backward")) != UPLIFT_LA_OK) return rc;
   }
   if (args->dweights != nullptr) {
-    dweights_kernel<<<(2 * args->D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, s>>>(args->partial, args->dweights,
-                                                                                            blocks, args->D);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((args->D + 31) / 32), 2);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, dweights_kernel, (const float*)args->partial, args->dweights,
+                                             (int)args->weight_dtype, partial_rows[0], partial_rows[1], (int)args->D);
+    if (e != cudaSuccess) return fail(UPLIFT_LA_ERR_CUDA, "norm_rotate weight gradients launch: %s", cudaGetErrorString(e));
     return tok::launched("norm_rotate weight gradients");
   }
   return UPLIFT_LA_OK;

@@ -37,47 +37,62 @@ _NR_ARGS = struct.Struct("@q" + 6 * "Pqq" + 7 * "P" + "qq" + "iiii" + "f" + "iii
 _PA_ARGS = struct.Struct("@q" + 8 * "Pqq" + 6 * "P" + "qqq" + "iiii" + "f" + "iii")
 _NO_ROWS = (0, 0, 0)
 
-try:  # the stream's handle without making a Stream object (microseconds count in a decoding step)
-    _raw_stream = torch._C._cuda_getCurrentRawStream
+try:  # without making Stream and device objects: microseconds count in a decoding step
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 except AttributeError:  # pragma: no cover
+    _current_device = torch.cuda.current_device
+
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 
+_HERE = nullcontext()
+
 
 def _on(index: int):
-    """Context in which `index` is the current device."""
-    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+    """Context in which `index` (the device of CUDA tensors, so CUDA is initialised) is the current device."""
+    return _HERE if _current_device() == index else torch.cuda.device(index)
 
 
-def _device(what: str, named) -> int:
-    """The common CUDA device index of (name, tensor) pairs; raises where they differ or are not on CUDA."""
-    index = named[0][1].get_device()
-    for name, t in named:
+def _device(what: str, names: str, *tensors) -> int:
+    """The common CUDA device index of the tensors (None: left out); raises where they differ or are not on CUDA."""
+    index = tensors[0].get_device()
+    same = index >= 0
+    for t in tensors:
+        same = same and (t is None or t.get_device() == index)
+    if same:
+        return index
+    for name, t in zip(names.split(), tensors):
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"uplift_b200 {what} runs on CUDA (sm_100) tensors only; {name} is a "
                                f"{t.device} tensor (there is no CPU fallback)")
         if t.get_device() != index:
-            raise ValueError(f"{what}: tensors on different devices: {named[0][1].device} vs {t.device} ({name})")
-    return index
+            raise ValueError(f"{what}: tensors on different devices: {tensors[0].device} vs {t.device} ({name})")
+    raise AssertionError
 
 
-def _check_rows(what: str, named) -> None:
-    name0, first = named[0]
-    dtype, D = first.dtype, first.shape[-1]
+def _check_rows(what: str, names: str, *tensors) -> None:
+    first = tensors[0]
+    dtype, D = first.dtype, first.shape[-1] if first.dim() else 0
+    fine = dtype in _DTYPES
+    for t in tensors:
+        shape = t.shape
+        fine = fine and len(shape) == 3 and t.dtype is dtype and shape[2] == D and D > 0 and shape[1] > 0
+    if fine:
+        return
     if dtype not in _DTYPES:
         raise ValueError(f"{what}: unsupported dtype {dtype} (float32, bfloat16, float16)")
-    for name, t in named:
-        shape = t.shape
-        if len(shape) != 3:
-            raise ValueError(f"{what}: {name} must be [rows, heads, D], got {tuple(shape)}")
+    names = names.split()
+    for name, t in zip(names, tensors):
+        if t.dim() != 3:
+            raise ValueError(f"{what}: {name} must be [rows, heads, D], got {tuple(t.shape)}")
         if t.dtype is not dtype:
-            raise ValueError(f"{what}: {name} is {t.dtype}, {name0} is {dtype}")
-        if shape[2] != D:
-            raise ValueError(f"{what}: {name} has head dimension {shape[2]}, {name0} has {D}")
-        if shape[1] < 1 or D < 1:
-            raise ValueError(f"{what}: {name} has no heads or channels: {tuple(shape)}")
+            raise ValueError(f"{what}: {name} is {t.dtype}, {names[0]} is {dtype}")
+        if t.shape[2] != D:
+            raise ValueError(f"{what}: {name} has head dimension {t.shape[2]}, {names[0]} has {D}")
+        if t.shape[1] < 1 or D < 1:
+            raise ValueError(f"{what}: {name} has no heads or channels: {tuple(t.shape)}")
 
 
 def _rows(t: torch.Tensor):
@@ -111,7 +126,7 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 def _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions):
     """Checks the arguments: (device index, weights' type)."""
     what = "norm_rotate"
-    _check_rows(what, (("q", q), ("k", k)))
+    _check_rows(what, "q k", q, k)
     T, _, D = q.shape
     if k.shape[0] != T:
         raise ValueError(f"{what}: q has {T} tokens, k has {k.shape[0]}")
@@ -139,13 +154,21 @@ def _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions):
     elif positions.shape != (T,) or (positions.dtype is not torch.int32 and positions.dtype is not torch.int64):
         raise ValueError(f"{what}: positions must be int32 or int64 [{T}], got {tuple(positions.shape)} "
                          f"{positions.dtype}")
-    index = _device(what, (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos),
-                           ("sin", sin), ("positions", positions)))
+    index = _device(what, "q k q_weight k_weight cos sin positions", q, k, q_weight, k_weight, cos, sin, positions)
     return index, (_native.F32 if wdt is None else _DTYPES[wdt])
 
 
 def _c(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.contiguous()
+
+
+def _weight_dtype(q_weight, k_weight) -> torch.dtype:
+    return q_weight.dtype if q_weight is not None else k_weight.dtype if k_weight is not None else torch.float32
+
+
+@functools.lru_cache(maxsize=None)
+def _partial_floats(D: int) -> int:
+    return _native.load().uplift_tok_norm_rotate_partial_floats(D)
 
 
 def norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
@@ -172,7 +195,7 @@ def norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6
 
 def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
                              interleaved=False, need_weights=True):
-    """Launch uplift_tok_norm_rotate_backward: (dq, dk, dweights [2, D] fp32; empty when not needed)."""
+    """Launch uplift_tok_norm_rotate_backward: (dq, dk, dweights [2, D] in the weights' type; empty when not needed)."""
     index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
     T, Hq, D = q.shape
     P, half = cos.shape
@@ -185,8 +208,8 @@ def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positio
         rh, gk = _rows(gk.to(q.dtype))
         rdq, dq = _new_rows(q)
         rdk, dk = _new_rows(k)
-        dw = torch.empty((2, D) if need_weights else (0,), dtype=torch.float32, device=q.device)
-        partial = dw.new_empty(lib.uplift_tok_norm_rotate_partial_floats(D)) if need_weights else None
+        dw = torch.empty((2, D) if need_weights else (0,), dtype=_weight_dtype(q_weight, k_weight), device=q.device)
+        partial = torch.empty(_partial_floats(D), dtype=torch.float32, device=q.device) if need_weights else None
         rc = lib.uplift_tok_norm_rotate_backward(
             _NR_ARGS.pack(_NR_ARGS.size, *rq, *rk, *rg, *rh, *rdq, *rdk, _ptr(q_weight), _ptr(k_weight),
                           cos.data_ptr(), sin.data_ptr(), _ptr(positions), dw.data_ptr() if need_weights else 0,
@@ -198,27 +221,27 @@ def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positio
     return dq, dk, dw
 
 
-def _norm_rotate_grads(ctx_needs, dq, dk, dw, q_weight, k_weight):
-    nq, nk, nqw, nkw = ctx_needs
-    return (dq if nq else None, dk if nk else None, dw[0].to(q_weight.dtype) if nqw else None,
-            dw[1].to(k_weight.dtype) if nkw else None)
-
-
 class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.eps, ctx.interleaved = eps, interleaved
+        ctx.set_materialize_grads(False)
         return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
-        needs = ctx.needs_input_grad[:4]
-        dq, dk, dw = norm_rotate_backward_raw(gq, gk, q, k, qw, kw, cos, sin, positions, ctx.eps, ctx.interleaved,
-                                              need_weights=needs[2] or needs[3])
-        return (*_norm_rotate_grads(needs, dq, dk, dw, qw, kw), None, None, None, None, None)
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        nq, nk, nqw, nkw = ctx.needs_input_grad[:4]
+        if gq is None:  # an output that is not used
+            gq = torch.zeros_like(q)
+        if gk is None:
+            gk = torch.zeros_like(k)
+        dq, dk, dw = norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, ctx.eps,
+                                              ctx.interleaved, need_weights=nqw or nkw)
+        return (dq if nq else None, dk if nk else None, dw[0] if nqw else None, dw[1] if nkw else None, None, None,
+                None, None, None)
 
 
 @torch.library.custom_op("uplift_b200::norm_rotate", mutates_args=())
@@ -247,7 +270,7 @@ def _norm_rotate_backward_op(gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor
 @_norm_rotate_backward_op.register_fake
 def _(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, need_weights):
     return (q.new_empty(q.shape), k.new_empty(k.shape),
-            q.new_empty((2, q.shape[2]) if need_weights else (0,), dtype=torch.float32))
+            q.new_empty((2, q.shape[2]) if need_weights else (0,), dtype=_weight_dtype(q_weight, k_weight)))
 
 
 def _nr_setup_context(ctx, inputs, output):
@@ -258,10 +281,12 @@ def _nr_setup_context(ctx, inputs, output):
 
 def _nr_backward(ctx, gq, gk):
     q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
-    needs = ctx.needs_input_grad[:4]
+    nq, nk, nqw, nkw = ctx.needs_input_grad[:4]
     dq, dk, dw = torch.ops.uplift_b200.norm_rotate_backward(gq, gk, q, k, qw, kw, cos, sin, positions, ctx.eps,
-                                                            ctx.interleaved, needs[2] or needs[3])
-    return (*_norm_rotate_grads(needs, dq, dk, dw, qw, kw), None, None, None, None, None)
+                                                            ctx.interleaved, nqw or nkw)
+    # the op's outputs must not alias each other, so the rows of dw are copied
+    return (dq if nq else None, dk if nk else None, dw[0].clone() if nqw else None, dw[1].clone() if nkw else None,
+            None, None, None, None, None)
 
 
 torch.library.register_autograd("uplift_b200::norm_rotate", _nr_backward, setup_context=_nr_setup_context)
@@ -303,7 +328,7 @@ def _starts(what: str, name: str, t: torch.Tensor, entries: int) -> None:
 def _attention_args(q, k, v, cu_q, cu_k, used_k, scale):
     """Checks the arguments: the device index."""
     what = "packed_attention"
-    _check_rows(what, (("q", q), ("k", k), ("v", v)))
+    _check_rows(what, "q k v", q, k, v)
     if k.shape != v.shape:
         raise ValueError(f"{what}: k is {tuple(k.shape)}, v is {tuple(v.shape)}")
     _, Hq, D = q.shape
@@ -318,7 +343,7 @@ def _attention_args(q, k, v, cu_q, cu_k, used_k, scale):
         _starts(what, "used_k", used_k, n - 1)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
-    return _device(what, (("q", q), ("k", k), ("v", v), ("cu_q", cu_q), ("cu_k", cu_k), ("used_k", used_k)))
+    return _device(what, "q k v cu_q cu_k used_k", q, k, v, cu_q, cu_k, used_k)
 
 
 @functools.lru_cache(maxsize=256)
@@ -387,11 +412,14 @@ class _PackedAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, used_k)
         ctx.causal, ctx.scale = causal, scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 8
         q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
         grads = packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal, ctx.scale)
         return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
