@@ -2,11 +2,11 @@
 // bf16 / fp16, D <= 128.
 //
 // An item is 256 query rows of one head of one sequence (two tiles of
-// M = 128), which walks the key tiles (128 keys) that its rows see:
+// M = 128), which walks the key tiles (64 keys) that its rows see:
 //
-//   S_t[128 x 128] = Q_t . K_j^T                    (tcgen05, fp32 in TMEM)
+//   S_t[128 x 64] = Q_t . K_j^T                     (tcgen05, fp32 in TMEM)
 //   m = max(m, rowmax S), P = exp2((S - m) scale log2 e), l += rowsum P
-//   O_t[128 x D]  += P . V_j                        (P from TMEM, V MN-major)
+//   O_t[128 x D] += P . V_j                         (P from TMEM, V MN-major)
 //
 // with the running maximum m and sum l in the registers of the thread that
 // owns the row (TMEM lane = query row), so that one pass over K and V
@@ -18,11 +18,14 @@
 //
 // Roles (384 threads, one persistent CTA per SM): warps 0-3 and 4-7 one
 // softmax group per tile (a thread per row); warp 8 looks the items up and
-// issues the TMA loads; warp 9 issues the MMAs.  The two tiles share each
-// K / V tile in shared memory and alternate: while one group computes its
-// exponentials the tensor cores work for the other.  P is rounded to the
-// storage type in place of S (half of its columns) -- the tensor cores
-// multiply 16-bit operands; the sum l uses the unrounded weights.
+// issues the TMA loads; warps 9 and 10 issue the MMAs of a tile each, so that
+// the waits of one overlap the products of the other.  Each tile has two score
+// buffers in TMEM, so the scores of key tile j + 1 are there when a group is
+// done with tile j: a group never waits for the tensor cores (with one
+// buffer of 128 keys a group stood still for two products per tile, and the
+// long prompt took 1.21 ms).  P is rounded to the storage type in place of S
+// (half of its columns) -- the tensor cores multiply 16-bit operands; the sum
+// l uses the unrounded weights.
 //
 // Scores that a row does not see -- behind its sequence's end, where a tile
 // holds rows of the next sequence, or behind the causal edge -- are set to
@@ -51,30 +54,27 @@ namespace fwd {
 
 constexpr int kM = 128;            // query rows of a tile
 constexpr int kItemRows = 2 * kM;
-constexpr int kN = 128;            // keys of a tile
-constexpr int kChunkBytes = 128 * 128;  // 128 rows x 64 channels
+constexpr int kN = 64;             // keys of a tile
+constexpr int kQChunk = kM * 128, kKvChunk = kN * 128;  // 64 channels of a tile
 constexpr int kThreads = 384;
 constexpr int kTmemCols = 512;
 constexpr int kItems = 2;          // ring of looked-up items
 constexpr uint64_t kTimeoutNs = 2000000000ull;
-// Registers of the softmax groups and of the other warps after the split:
-// 2 x 128 x 208 + 128 x 88 = 384 x 168, what the CTA is launched with.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;    // log2 of the growth of the maximum that O is rescaled for
 
 template <int DP>
 struct Cfg {
   static constexpr int kChunks = DP / 64;
-  static constexpr int kQBytes = kChunks * kChunkBytes;  // one query tile
-  static constexpr int kSlotBytes = kChunks * kChunkBytes;
-  static constexpr int kSlots = DP == 128 ? 4 : 8;       // K and V tiles in turn
+  static constexpr int kQBytes = kChunks * kQChunk;  // one query tile
+  static constexpr int kSlotBytes = kChunks * kKvChunk;
+  static constexpr int kSlots = 8;                   // K and V tiles
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kQBytes;
   static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;
   static constexpr int kStageBytes = 32 * 128;           // a warp's 32 rows x 64 channels
   static constexpr int kOffBar = kOffStage + 8 * kStageBytes;
-  static constexpr int kNumBars = 2 + 2 * kSlots + 3 * 2 + 2 * kItems + 1;
+  static constexpr int kNumBars = 2 + 2 * kSlots + 4 + 4 + 4 + 2 * kItems + 2;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffItems = kOffMisc + 32;
   static constexpr int kSmem = kOffItems + kItems * 48 + 1024;  // + base alignment slack
@@ -103,12 +103,16 @@ struct Params {
   unsigned int* host_status;
 };
 
-// Bounded wait, inline: a kernel that splits its registers between warps
-// cannot call functions.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
                                           const WaitLimit& limit) {
-  return mbar_wait_inline(b, parity, abort_flag, where, limit, &g_tok_fwd_status);
+  if (mbar_try(b, parity)) return true;  // completed phase: no call into the bounded slow path
+  return mbar_wait_status(b, parity, abort_flag, where, limit, &g_tok_fwd_status);
 }
+
+// Position of K_j and V_j of an item with `tiles` key tiles in the order in
+// which they are loaded: K_0, K_1, V_0, K_2, V_1, K_3, ..
+__device__ __forceinline__ uint32_t k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
+__device__ __forceinline__ uint32_t v_pos(int j, int tiles) { return min(2 * j + 2, 2 * tiles - 1); }
 
 template <typename T>
 __device__ __forceinline__ uint32_t nonfinite_probe(uint32_t acc, uint32_t x);  // acc stays 0 in both halves iff x is finite
@@ -124,23 +128,17 @@ __device__ __forceinline__ uint32_t nonfinite_probe<__half>(uint32_t acc, uint32
   return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// Replaces infinities and NaN in row r of a V tile by zero; true if there were any.
+// The part of V row tid % 64 of a tile that thread tid of a group looks
+// through: every second 16-byte piece of each chunk of 64 channels.
 template <typename T, int CHUNKS>
-__device__ __forceinline__ void clean_row(uint8_t* tile, int r) {
-#pragma unroll 1
-  for (int i = 0; i < CHUNKS * 64; ++i) {
-    T* e = reinterpret_cast<T*>(tile + (i >> 6) * kChunkBytes + r * 128 + (((((i & 63) >> 3) ^ (r & 7)) << 4)) + (i & 7) * 2);
-    if (!isfinite(St<T>::f(*e))) *e = St<T>::t(0.f);
-  }
-}
-template <typename T, int CHUNKS>
-__device__ __forceinline__ bool row_is_finite(const uint8_t* tile, int r) {
+__device__ __forceinline__ bool row_is_finite(const uint8_t* tile, int tid) {
+  const int r = tid & 63;
   uint32_t acc = 0;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll 4
-    for (int i = 0; i < 8; ++i) {  // pieces in an order that spreads the lanes over the banks
-      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kChunkBytes + r * 128 + ((i ^ (r & 7)) << 4));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kKvChunk + r * 128 + (((2 * i + (tid >> 6)) ^ (r & 7)) << 4));
       acc = nonfinite_probe<T>(acc, v.x);
       acc = nonfinite_probe<T>(acc, v.y);
       acc = nonfinite_probe<T>(acc, v.z);
@@ -150,11 +148,21 @@ __device__ __forceinline__ bool row_is_finite(const uint8_t* tile, int r) {
   const float2 f = St<T>::unpack(acc);
   return f.x == 0.f && f.y == 0.f;
 }
+// Replaces infinities and NaN in it by zero.
+template <typename T, int CHUNKS>
+__device__ __noinline__ void clean_row(uint8_t* tile, int tid) {
+  const int r = tid & 63;
+  for (int i = 0; i < CHUNKS * 32; ++i) {
+    const int piece = 2 * ((i >> 3) & 3) + (tid >> 6);
+    T* e = reinterpret_cast<T*>(tile + (i >> 5) * kKvChunk + r * 128 + ((piece ^ (r & 7)) << 4) + (i & 7) * 2);
+    if (!isfinite(St<T>::f(*e))) *e = St<T>::t(0.f);
+  }
+}
 
 // Adds the infinities and NaN of the rows j0 .. j1 - 1 of v (`channels`
 // channels of them) to a staged output row.
 template <typename T>
-__device__ __forceinline__ void add_nonfinite(uint8_t* row, int lane, const T* v, int64_t stride, int j0, int j1, int channels) {
+__device__ __noinline__ void add_nonfinite(uint8_t* row, int lane, const T* v, int64_t stride, int j0, int j1, int channels) {
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
 #pragma unroll 1
@@ -167,17 +175,8 @@ __device__ __forceinline__ void add_nonfinite(uint8_t* row, int lane, const T* v
   }
 }
 
-// Scores from column lim on are not seen.
 template <int N>
-__device__ __forceinline__ void cut(float* f, int lim) {
-  if (lim < N) {
-#pragma unroll
-    for (int c = 0; c < N; ++c) f[c] = c < lim ? f[c] : -INFINITY;
-  }
-}
-template <int N>
-__device__ __forceinline__ float row_max(float* f, int lim) {
-  cut<N>(f, lim);
+__device__ __forceinline__ float row_max(const float* f) {
   float mx[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
   for (int c = 4; c < N; c += 4) {
@@ -202,36 +201,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   uint64_t* q_empty = q_full + 1;             // the item's score MMAs are done
   uint64_t* kv_full = q_empty + 1;            // [kSlots]
   uint64_t* kv_empty = kv_full + C::kSlots;   // [kSlots]
-  uint64_t* s_full = kv_empty + C::kSlots;    // [2] scores of a tile
-  uint64_t* p_full = s_full + 2;              // [2] weights of a tile
-  uint64_t* o_full = p_full + 2;              // [2] an item's output
+  uint64_t* s_full = kv_empty + C::kSlots;    // [2][2] scores: query tile, buffer
+  uint64_t* p_full = s_full + 4;              // [2][2] weights
+  uint64_t* o_done = p_full + 4;              // [2] a product with V is complete
+  uint64_t* o_full = o_done + 2;              // [2] an item's last product is complete
   uint64_t* item_full = o_full + 2;           // [kItems]
   uint64_t* item_empty = item_full + kItems;  // [kItems]
-  uint64_t* drain = item_empty + kItems;
+  uint64_t* drain = item_empty + kItems;      // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
   volatile int* v_cleaned = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 16);
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
 
   const int tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);  // both MMA warps
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);  // 4 warps
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 9);  // 8 softmax warps, MMA
+      mbar_init(&item_empty[i], 10);  // 8 softmax warps, 2 MMA warps
     }
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     abort_flag[0] = 0;
     abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
     *v_cleaned = 0;
@@ -244,13 +248,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  auto t_s = [&](int t) { return tmem + t * kN; };            // scores, then weights of tile t
-  auto t_o = [&](int t) { return tmem + 2 * kN + t * DP; };   // output of tile t
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  auto t_s = [&](int t, uint32_t b) { return tmem + (2 * t + b) * kN; };  // scores, then weights of tile t
+  auto t_o = [&](int t) { return tmem + 4 * kN + t * DP; };               // output of tile t
   const WaitLimit tmo{p.timeout_ns, p.host_status};
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ---------------------------------------------------------- producer
       if (lane == 0) {
@@ -305,23 +308,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               for (int t = 0; t < qt; ++t) {
 #pragma unroll
                 for (int c = 0; c < C::kChunks; ++c)
-                  load_rows(sQ + t * C::kQBytes + c * kChunkBytes, &p.qmap, q_full, 64 * c, it.h, it.row + t * kM);
+                  load_rows(sQ + t * C::kQBytes + c * kQChunk, &p.qmap, q_full, 64 * c, it.h, it.row + t * kM);
               }
             }
             ++nq;
             const int hk = it.h / p.group;
+            auto load = [&](const CUtensorMap* map, int j) {
+              const int s = g % C::kSlots;
+              ok = ok && mbar_wait(&kv_empty[s], ((g / C::kSlots) & 1) ^ 1, abort_flag, 1, tmo);
+              ++g;
+              if (!ok) return;
+              mbar_expect_tx(&kv_full[s], C::kSlotBytes);
+#pragma unroll
+              for (int c = 0; c < C::kChunks; ++c)
+                load_rows(sKV + s * C::kSlotBytes + c * kKvChunk, map, &kv_full[s], 64 * c, hk, it.k0 + j * kN);
+            };
+            load(&p.kmap, 0);
+            if (tiles_k > 1) load(&p.kmap, 1);
             for (int j = 0; j < tiles_k && ok; ++j) {
-#pragma unroll
-              for (int w = 0; w < 2; ++w, ++g) {  // K_j, V_j
-                const int s = g % C::kSlots;
-                ok = ok && mbar_wait(&kv_empty[s], ((g / C::kSlots) & 1) ^ 1, abort_flag, 1, tmo);
-                if (!ok) break;
-                mbar_expect_tx(&kv_full[s], C::kSlotBytes);
-#pragma unroll
-                for (int c = 0; c < C::kChunks; ++c)
-                  load_rows(sKV + s * C::kSlotBytes + c * kChunkBytes, w == 0 ? &p.kmap : &p.vmap, &kv_full[s], 64 * c, hk,
-                            it.k0 + j * kN);
-              }
+              load(&p.vmap, j);
+              if (j + 2 < tiles_k) load(&p.kmap, j + 2);
             }
           }
         }
@@ -332,85 +338,100 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const uint64_t t0 = gtimer();
         while (gtimer() - t0 < 200000ull) {}
       }
-    } else if (warp == 9 && lane == 0) {
-      // -------------------------------------------------------- MMA issuer
+    } else if (warp < 11) {
+      // ------------------------------------------- MMA issuer of a query tile
+      const int t = warp - 9;
       constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
       constexpr uint32_t kIdO = idesc_f16(St<T>::kFmt, 1, kM, DP);
       const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
-      const uint32_t aQ = su32(sQ), aKV = su32(sKV);
+      // descriptors: the start address counts 16 bytes in their lowest bits
+      const uint64_t dq = mdesc(su32(sQ) + t * C::kQBytes, 16, 1024, kLayoutSw128);
+      const uint64_t dk = mdesc(su32(sKV), 16, 1024, kLayoutSw128), dv = mdesc(su32(sKV), kKvChunk, 1024, kLayoutSw128);
+      const uint32_t o = t_o(t);
       bool ok = true;
-      uint32_t g = 0, nq = 0;
-      uint32_t np[2] = {0, 0};
-      auto scores = [&](int t, uint32_t slot) {
-        const uint32_t a = aQ + t * C::kQBytes, b = aKV + slot * C::kSlotBytes;
-        for (int ks = 0; ks < ksteps; ++ks) {
-          const uint32_t off = (ks >> 2) * kChunkBytes + 32 * (ks & 3);
-          tc_mma(t_s(t), mdesc(a + off, 16, 1024, kLayoutSw128), mdesc(b + off, 16, 1024, kLayoutSw128), kIdS, ks > 0);
+      uint32_t g = 0, nq = 0, ns = 0;  // ns: key tiles of this query tile so far
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, 2, tmo));
+      };
+      auto ready = [&](uint32_t pos) { return wait(&kv_full[pos % C::kSlots], (pos / C::kSlots) & 1); };
+      // scores of key tile n (counted over items) with the K tile at `pos`;
+      // a tile that this query tile does not see is only given back
+      auto scores = [&](uint32_t n, uint32_t pos, bool seen, bool last) {
+        tc_fence_after();
+        if (elect_one()) {
+          if (seen) {
+            const uint64_t k = dk + (pos % C::kSlots) * (C::kSlotBytes >> 4);
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+              if (ks < ksteps)
+                tc_mma(t_s(t, n & 1), dq + (((ks >> 2) * kQChunk + 32 * (ks & 3)) >> 4),
+                       k + (((ks >> 2) * kKvChunk + 32 * (ks & 3)) >> 4), kIdS, ks > 0);
+            tc_commit(&s_full[2 * t + (n & 1)]);
+            if (last) tc_commit(q_empty);
+          }
+          tc_commit(&kv_empty[pos % C::kSlots]);
         }
-        tc_commit(&s_full[t]);
+        __syncwarp();
       };
       for (int n = 0; ok; ++n) {
         const int islot = n % kItems;
-        ok = mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 2, tmo);
+        ok = wait(&item_full[islot], (n / kItems) & 1);
         if (!ok) break;
-        const int rows = items[islot].n;
-        const int nt[2] = {items[islot].nt[0], items[islot].nt[1]};
-        mbar_arrive(&item_empty[islot]);
+        const int rows = items[islot].n, mine = items[islot].nt[t], tiles = max(items[islot].nt[0], items[islot].nt[1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[islot]);
         if (rows == 0) break;
-        const int tiles = max(nt[0], nt[1]);
         if (tiles == 0) continue;
-        ok = mbar_wait(q_full, nq & 1, abort_flag, 2, tmo) &&
-             mbar_wait(&kv_full[g % C::kSlots], (g / C::kSlots) & 1, abort_flag, 2, tmo);
+        ok = wait(q_full, nq & 1);
         ++nq;
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (nt[t] > 0) scores(t, g % C::kSlots);
-        tc_commit(&kv_empty[g % C::kSlots]);
-        if (tiles == 1) tc_commit(q_empty);
+        if (ok && mine == 0 && lane == 0) mbar_arrive(q_empty);
+        for (int j = 0; j < min(2, tiles) && ok; ++j) {
+          ok = ready(g + j);
+          if (ok) scores(ns + j, g + j, j < mine, j + 1 == mine);
+        }
         for (int j = 0; j < tiles && ok; ++j) {
-          const uint32_t gv = g + 2 * j + 1, gk = gv + 1;  // V_j, K_j+1
-          const uint32_t sv = gv % C::kSlots, sk = gk % C::kSlots;
-          ok = mbar_wait(&kv_full[sv], (gv / C::kSlots) & 1, abort_flag, 2, tmo) &&
-               (j + 1 >= tiles || mbar_wait(&kv_full[sk], (gk / C::kSlots) & 1, abort_flag, 2, tmo));
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t] || !ok) continue;
-            ok = mbar_wait(&p_full[t], np[t] & 1, abort_flag, 2, tmo);
-            if (!ok) break;
-            ++np[t];
-            tc_fence_after();
-#pragma unroll
-            for (int ks = 0; ks < kN / 16; ++ks)
-              mma_tmem_a(t_o(t), t_s(t) + 8 * ks, mdesc(aKV + sv * C::kSlotBytes + 2048 * ks, kChunkBytes, 1024, kLayoutSw128),
-                         kIdO, (j > 0 || ks > 0) ? 1u : 0u);
-            if (j + 1 < nt[t]) scores(t, sk);
-            else tc_commit(&o_full[t]);
-          }
+          const uint32_t gv = g + v_pos(j, tiles);
+          ok = ready(gv) && (j >= mine || wait(&p_full[2 * t + ((ns + j) & 1)], ((ns + j) >> 1) & 1));
           if (!ok) break;
-          tc_commit(&kv_empty[sv]);
-          if (j + 1 < tiles) tc_commit(&kv_empty[sk]);
-          if (j + 2 == tiles) tc_commit(q_empty);
+          tc_fence_after();
+          if (elect_one()) {
+            if (j < mine) {
+              const uint64_t v = dv + (gv % C::kSlots) * (C::kSlotBytes >> 4);
+              const uint32_t w = t_s(t, (ns + j) & 1);
+#pragma unroll
+              for (int ks = 0; ks < kN / 16; ++ks)
+                mma_tmem_a(o, w + 8 * ks, v + ((2048 * ks) >> 4), kIdO, (j > 0 || ks > 0) ? 1u : 0u);
+              tc_commit(&o_done[t]);
+              if (j + 1 == mine) tc_commit(&o_full[t]);
+            }
+            tc_commit(&kv_empty[gv % C::kSlots]);
+          }
+          __syncwarp();
+          if (j + 2 < tiles) {
+            const uint32_t gk = g + k_pos(j + 2);
+            ok = ready(gk);
+            if (ok) scores(ns + j + 2, gk, j + 2 < mine, j + 3 == mine);
+          }
         }
         g += 2 * tiles;
+        ns += mine;
       }
       // all issued MMAs complete before TMEM can be released (this wait
       // ignores the abort flag: it must not be cut short by another role)
-      tc_commit(drain);
-      mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
+      if (elect_one()) tc_commit(&drain[t]);
+      __syncwarp();
+      mbar_wait(&drain[t], 0, abort_flag + 1, 2, tmo);
     }
   } else {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2;
     const int q = warp & 3;
     const int r = 32 * q + lane;  // row of the tile = TMEM lane
     const uint32_t lane_off = (uint32_t)(32 * q) << 16;
-    const uint32_t ts = t_s(t) + lane_off, to = t_o(t) + lane_off;
+    const uint32_t to = t_o(t) + lane_off;
     const float c2 = p.scale * kLog2e;
     uint8_t* stage = smem + C::kOffStage + warp * C::kStageBytes;
-    uint32_t ns = 0, no = 0, g = 0;
+    uint32_t ns = 0, no = 0, g = 0;  // key tiles and items of this query tile, K / V tiles before this item
     bool ok = true;
     for (int n = 0; ok; ++n) {
       const int islot = n % kItems;
@@ -429,37 +450,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + t * kM)) : it.nk) / kN;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < tiles; ++j, ++ns) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], ns & 1, abort_flag, 3, tmo));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (ns & 1)], (ns >> 1) & 1, abort_flag, 3, tmo));
         if (!ok) break;
         tc_fence_after();
-        // The row maximum, then the weights.  A thread holds 64 of its 128
-        // scores at a time: columns 64.. are read for the maximum and again
-        // for the weights (128 more cycles of TMEM reads per tile, hidden
-        // behind the exponentials), since all 128 with the packed weights
-        // and the addresses do not fit a thread's registers.
-        const int lim = j >= edge ? see - j * kN : kN;
-        uint32_t sa[64], sb[32];
-        float* fa = reinterpret_cast<float*>(sa);
-        float* fb = reinterpret_cast<float*>(sb);
-        float mj = -INFINITY;
+        const uint32_t ts = t_s(t, ns & 1) + lane_off;
+        uint32_t s[kN];
+        float* f = reinterpret_cast<float*>(s);
+        tc_ld32(ts, s);
+        tc_ld32(ts + 32, s + 32);
+        tc_wait_ld_regs(s);
+        tc_wait_ld_regs(s + 32);
+        if (j >= edge) {
+          const int lim = see - j * kN;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tc_ld32(ts + 64 + 32 * c, sb);
-          tc_wait_ld_regs(sb);
-          mj = fmaxf(mj, row_max<32>(fb, lim - 64 - 32 * c));
+          for (int c = 0; c < kN; ++c) f[c] = c < lim ? f[c] : -INFINITY;
         }
-        tc_ld32(ts, sa);
-        tc_ld32(ts + 32, sa + 32);
-        tc_wait_ld_regs(sa);
-        tc_wait_ld_regs(sa + 32);
-        mj = fmaxf(mj, row_max<64>(fa, lim));
+        const float mj = row_max<kN>(f);
         if (j == 0) {
           m = mj;
         } else {
           const bool grow = (mj - m) * c2 > kRescale;  // also from m = -inf
           if (__any_sync(0xffffffffu, grow)) {
-            // the score MMAs of this tile came after the product that last
-            // wrote O, so O is complete
+            // the last product that wrote O has to be complete (the one
+            // before it is: the scores of this tile came after it)
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (ns - 1) & 1, abort_flag, 3, tmo));
+            if (!ok) break;
+            tc_fence_after();
             const float a = grow ? ex2((m - mj) * c2) : 1.f;
             if (grow) m = mj;
             l *= a;
@@ -477,47 +493,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const float mc = m == -INFINITY ? 0.f : m * c2;
         const float2 c22 = make_float2(c2, c2), mc2 = make_float2(-mc, -mc);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // 32 scores -> weights in columns 16 h.. of the tile (the scores
-        // there have been read before)
-        auto weights = [&](const float* f, int h) {
+#pragma unroll
+        for (int h = 0; h < kN / 32; ++h) {
           uint32_t w[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float2 x = __ffma2_rn(make_float2(f[c], f[c + 1]), c22, mc2);
+            const float2 x = __ffma2_rn(make_float2(f[32 * h + c], f[32 * h + c + 1]), c22, mc2);
             const float2 y = make_float2(ex2(x.x), ex2(x.y));
             sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], y);
             w[c / 2] = St<T>::pack(y.x, y.y);
           }
           tmem_st16(ts + 16 * h, w);
-        };
-        tc_ld32(ts + 64, sb);
-        weights(fa, 0);
-        weights(fa + 32, 1);
-        tc_wait_ld_regs(sb);
-        tc_ld32(ts + 96, sa);
-        cut<32>(fb, lim - 64);
-        weights(fb, 2);
-        tc_wait_ld_regs(sa);
-        cut<32>(fa, lim - 96);
-        weights(fa, 3);
+        }
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         if (j >= edge) {
           // V tile j: infinities and NaN out (see the top of the file)
-          const uint32_t gv = g + 2 * j + 1;
+          const uint32_t gv = g + v_pos(j, all_tiles);
           uint8_t* tile = sKV + (gv % C::kSlots) * C::kSlotBytes;
           ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[gv % C::kSlots], (gv / C::kSlots) & 1, abort_flag, 3, tmo));
           if (!ok) break;
-          if (!row_is_finite<T, C::kChunks>(tile, r)) {
+          if (!row_is_finite<T, C::kChunks>(tile, tid & 127)) {
             *v_cleaned = 1;
             __threadfence_block();
-            clean_row<T, C::kChunks>(tile, r);
+            clean_row<T, C::kChunks>(tile, tid & 127);
             fence_proxy_async();
           }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + (ns & 1)]);
       }
       if (!ok) break;
       g += 2 * all_tiles;
@@ -525,8 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       // ---------------------------------------------------------- epilogue
       if (tiles > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1, abort_flag, 4, tmo));
-        if (!ok) break;
         ++no;
+        if (!ok) break;
         tc_fence_after();
       }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN

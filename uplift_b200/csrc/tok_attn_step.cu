@@ -42,10 +42,8 @@ constexpr int kKeys = 16;          // keys of a warp at a time
 constexpr int kRows = 8;           // query heads of an item
 constexpr int kMinChunk = kWarps * kKeys;
 constexpr int kMaxChunks = 128;    // of one token
-#ifndef ULA_STEP_CTAS
-#define ULA_STEP_CTAS 4
-#endif
-constexpr int kCtasPerSm = ULA_STEP_CTAS;
+constexpr int kCtasPerSm = 3;      // 168 registers a thread; with 4 (128) or 2 the large steps are 1.5 and 1.2 times slower
+constexpr int kManyKeys = 1024;    // keys of an item of a large problem
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;    // see tok_attn_fwd.cu
 
@@ -474,11 +472,11 @@ int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s) {
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)a.pk.T * p.chunks * a.Hq * a.D);
   p.scale = a.scale;
-  // Keys per item so that the items fill the SMs about four times, within 64
-  // (the four warps once) and 512 (where the join costs 3 % of the reads).
+  // Keys per item: the items of a small problem fill the SMs once, those of a
+  // large one have 1024 keys (the join costs 2 % of the reads; 512: 8 % slower).
   const int64_t pairs = a.pk.B > 0 ? (int64_t)a.pk.T * a.pk.S / a.pk.B * a.Hk * p.row_tiles : 0;
-  const int64_t len = pairs / ((int64_t)sms * kCtasPerSm * 4);
-  p.min_len = (int)std::min<int64_t>(512, std::max<int64_t>(kMinChunk, (len + kMinChunk - 1) / kMinChunk * kMinChunk));
+  const int64_t len = pairs / ((int64_t)sms * kCtasPerSm);
+  p.min_len = (int)std::min<int64_t>(kManyKeys, std::max<int64_t>(kMinChunk, (len + kMinChunk - 1) / kMinChunk * kMinChunk));
   if (a.dtype == UPLIFT_LA_BF16)
     return a.D <= 64 ? run<__nv_bfloat16, 64>(p, sms, s) : run<__nv_bfloat16, 128>(p, sms, s);
   return a.D <= 64 ? run<__half, 64>(p, sms, s) : run<__half, 128>(p, sms, s);

@@ -110,6 +110,20 @@ struct TileWalk {
   }
 };
 
+// ------------------------------------------------------------ MMA issue
+// One lane of a converged warp.  The MMA warp runs its loop with all lanes,
+// so that descriptors and TMEM addresses are uniform over the warp and stay
+// in uniform registers; only the instructions are issued by the elected lane.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(pred));
+  return pred != 0;
+}
+
 // ------------------------------------------------------------ TMEM
 // kind::f16 MMA with the A operand in TMEM (lane = row; a 32-bit column
 // holds two consecutive K elements).
