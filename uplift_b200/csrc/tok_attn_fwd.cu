@@ -16,16 +16,24 @@
 // or fp16, and the final division by l takes any common factor out), which
 // after the first tiles hardly ever happens.
 //
-// Roles (384 threads, one persistent CTA per SM): warps 0-3 and 4-7 one
-// softmax group per tile (a thread per row); warp 8 looks the items up and
-// issues the TMA loads; warps 9 and 10 issue the MMAs of a tile each, so that
-// the waits of one overlap the products of the other.  Each tile has two score
-// buffers in TMEM, so the scores of key tile j + 1 are there when a group is
-// done with tile j: a group never waits for the tensor cores (with one
-// buffer of 128 keys a group stood still for two products per tile, and the
-// long prompt took 1.21 ms).  P is rounded to the storage type in place of S
-// (half of its columns) -- the tensor cores multiply 16-bit operands; the sum
-// l uses the unrounded weights.
+// Roles (640 threads, one persistent CTA per SM): warps 0-7 and 8-15 the
+// softmax of a tile each, as two groups of four warps that take the key tiles
+// in turn (a thread per row); warp 16 looks the items up and issues the TMA
+// loads; warps 17 and 18 issue the MMAs of a tile each, so that the waits of
+// one overlap the products of the other.  Each tile has two score buffers in
+// TMEM, one per group, so the scores of the next key tile are there when a
+// group is done.  A warp alone gets one exponential every 15 cycles out of the
+// unit that could give one every 8, and none while it loads, compares and
+// stores: with one group per tile (two warps per SM quarter) the unit was
+// busy half of the time.  P is rounded to the storage type in place of S --
+// the tensor cores multiply 16-bit operands; the sum l uses the unrounded
+// weights.
+//
+// The maximum of a row is kept in shared memory.  A group decides on it for
+// key tile j (and rescales O, after the product of tile j - 1) only when the
+// other group has decided for tile j - 1, so weights and sums always agree
+// on it; the decision needs the scores' maximum alone and comes long before
+// the other group asks for it.
 //
 // Scores that a row does not see -- behind its sequence's end, where a tile
 // holds rows of the next sequence, or behind the causal edge -- are set to
@@ -56,7 +64,7 @@ constexpr int kM = 128;            // query rows of a tile
 constexpr int kItemRows = 2 * kM;
 constexpr int kN = 64;             // keys of a tile
 constexpr int kQChunk = kM * 128, kKvChunk = kN * 128;  // 64 channels of a tile
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
 constexpr int kTmemCols = 512;
 constexpr int kItems = 2;          // ring of looked-up items
 constexpr uint64_t kTimeoutNs = 2000000000ull;
@@ -73,11 +81,12 @@ struct Cfg {
   static constexpr int kOffKV = 2 * kQBytes;
   static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;
   static constexpr int kStageBytes = 32 * 128;           // a warp's 32 rows x 64 channels
-  static constexpr int kOffBar = kOffStage + 8 * kStageBytes;
+  static constexpr int kOffRows = kOffStage + 8 * kStageBytes;  // [query tile][row]: maximum and the key tile it is of
+  static constexpr int kOffBar = kOffRows + 2 * kM * 8;
   static constexpr int kNumBars = 2 + 2 * kSlots + 4 + 4 + 4 + 2 * kItems + 2;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffItems = kOffMisc + 32;
-  static constexpr int kSmem = kOffItems + kItems * 48 + 1024;  // + base alignment slack
+  static constexpr int kSmem = kOffItems + kItems * 32;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -159,14 +168,14 @@ __device__ __noinline__ void clean_row(uint8_t* tile, int tid) {
   }
 }
 
-// Adds the infinities and NaN of the rows j0 .. j1 - 1 of v (`channels`
-// channels of them) to a staged output row.
+// Adds the infinities and NaN of the rows j0 .. j1 - 1 of v (channels i0 ..
+// i1 - 1) to a staged output row.
 template <typename T>
-__device__ __noinline__ void add_nonfinite(uint8_t* row, int lane, const T* v, int64_t stride, int j0, int j1, int channels) {
+__device__ __noinline__ void add_nonfinite(uint8_t* row, int lane, const T* v, int64_t stride, int j0, int j1, int i0, int i1) {
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
 #pragma unroll 1
-    for (int i = 0; i < channels; ++i) {
+    for (int i = i0; i < i1; ++i) {
       const float x = St<T>::f(v[j * stride + i]);
       if (isfinite(x)) continue;
       T* e = reinterpret_cast<T*>(row + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2);
@@ -192,8 +201,11 @@ __device__ __forceinline__ float row_max(const float* f) {
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((su32(smem) & 1023u) != 0) {  // the swizzled tiles need it, and the declaration asks for it
+    if (threadIdx.x == 0) atomicCAS(&g_tok_fwd_status, 0u, 1u);
+    return;
+  }
   uint8_t* sQ = smem + C::kOffQ;
   uint8_t* sKV = smem + C::kOffKV;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -211,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
   volatile int* v_cleaned = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 16);
+  int* issuing = reinterpret_cast<int*>(smem + C::kOffMisc + 20);
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
 
   const int tid = threadIdx.x;
@@ -232,16 +245,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 10);  // 8 softmax warps, 2 MMA warps
+      mbar_init(&item_empty[i], 18);  // 16 softmax warps, 2 MMA warps
     }
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     abort_flag[0] = 0;
     abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
     *v_cleaned = 0;
+    *issuing = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -253,8 +267,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   auto t_o = [&](int t) { return tmem + 4 * kN + t * DP; };               // output of tile t
   const WaitLimit tmo{p.timeout_ns, p.host_status};
 
-  if (warp >= 8) {
-    if (warp == 8) {
+  if (warp >= 16) {
+    if (warp == 16) {
       // ---------------------------------------------------------- producer
       if (lane == 0) {
         prefetch_map(&p.qmap);
@@ -338,9 +352,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const uint64_t t0 = gtimer();
         while (gtimer() - t0 < 200000ull) {}
       }
-    } else if (warp < 11) {
+    } else if (warp < 19) {
       // ------------------------------------------- MMA issuer of a query tile
-      const int t = warp - 9;
+      const int t = warp - 17;
       constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
       constexpr uint32_t kIdO = idesc_f16(St<T>::kFmt, 1, kM, DP);
       const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
@@ -354,24 +368,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, 2, tmo));
       };
       auto ready = [&](uint32_t pos) { return wait(&kv_full[pos % C::kSlots], (pos / C::kSlots) & 1); };
-      // scores of key tile n (counted over items) with the K tile at `pos`;
-      // a tile that this query tile does not see is only given back
+      // (one lane) scores of key tile n, counted over items, with the K tile
+      // at `pos`; a tile that this query tile does not see is only given back
       auto scores = [&](uint32_t n, uint32_t pos, bool seen, bool last) {
-        tc_fence_after();
-        if (elect_one()) {
-          if (seen) {
-            const uint64_t k = dk + (pos % C::kSlots) * (C::kSlotBytes >> 4);
+        if (seen) {
+          const uint64_t k = dk + (pos % C::kSlots) * (C::kSlotBytes >> 4);
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks)
-              if (ks < ksteps)
-                tc_mma(t_s(t, n & 1), dq + (((ks >> 2) * kQChunk + 32 * (ks & 3)) >> 4),
-                       k + (((ks >> 2) * kKvChunk + 32 * (ks & 3)) >> 4), kIdS, ks > 0);
-            tc_commit(&s_full[2 * t + (n & 1)]);
-            if (last) tc_commit(q_empty);
-          }
-          tc_commit(&kv_empty[pos % C::kSlots]);
+          for (int ks = 0; ks < DP / 16; ++ks)
+            if (ks < ksteps)
+              tc_mma(t_s(t, n & 1), dq + (((ks >> 2) * kQChunk + 32 * (ks & 3)) >> 4),
+                     k + (((ks >> 2) * kKvChunk + 32 * (ks & 3)) >> 4), kIdS, ks > 0);
+          tc_commit(&s_full[2 * t + (n & 1)]);
+          if (last) tc_commit(q_empty);
         }
-        __syncwarp();
+        tc_commit(&kv_empty[pos % C::kSlots]);
       };
       for (int n = 0; ok; ++n) {
         const int islot = n % kItems;
@@ -387,31 +397,40 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         if (ok && mine == 0 && lane == 0) mbar_arrive(q_empty);
         for (int j = 0; j < min(2, tiles) && ok; ++j) {
           ok = ready(g + j);
-          if (ok) scores(ns + j, g + j, j < mine, j + 1 == mine);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) scores(ns + j, g + j, j < mine, j + 1 == mine);
+          __syncwarp();
         }
         for (int j = 0; j < tiles && ok; ++j) {
-          const uint32_t gv = g + v_pos(j, tiles);
-          ok = ready(gv) && (j >= mine || wait(&p_full[2 * t + ((ns + j) & 1)], ((ns + j) >> 1) & 1));
+          // V_j and K_j+2 are there long before the weights, which are waited
+          // for last: the products follow them at once
+          const uint32_t gv = g + v_pos(j, tiles), gk = g + k_pos(j + 2);
+          ok = ready(gv) && (j + 2 >= tiles || ready(gk)) &&
+               (j >= mine || wait(&p_full[2 * t + ((ns + j) & 1)], ((ns + j) >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
+            // One tile's products at a time: interleaved, both tiles' would
+            // end together, and the tensor cores wait while both groups work.
+            // (Only a matter of speed: after a while it goes on regardless.)
+            for (int spin = 0; atomicExch(issuing, 1) != 0 && spin < 4096; ++spin) {}
             if (j < mine) {
               const uint64_t v = dv + (gv % C::kSlots) * (C::kSlotBytes >> 4);
               const uint32_t w = t_s(t, (ns + j) & 1);
 #pragma unroll
               for (int ks = 0; ks < kN / 16; ++ks)
-                mma_tmem_a(o, w + 8 * ks, v + ((2048 * ks) >> 4), kIdO, (j > 0 || ks > 0) ? 1u : 0u);
+                mma_tmem_a(o, w + 8 * (ks & 1) + 32 * (ks >> 1), v + ((2048 * ks) >> 4), kIdO, (j > 0 || ks > 0) ? 1u : 0u);
+            }
+            if (j + 2 < tiles) scores(ns + j + 2, gk, j + 2 < mine, j + 3 == mine);
+            if (j < mine) {
               tc_commit(&o_done[t]);
               if (j + 1 == mine) tc_commit(&o_full[t]);
             }
             tc_commit(&kv_empty[gv % C::kSlots]);
+            atomicExch(issuing, 0);
           }
           __syncwarp();
-          if (j + 2 < tiles) {
-            const uint32_t gk = g + k_pos(j + 2);
-            ok = ready(gk);
-            if (ok) scores(ns + j + 2, gk, j + 2 < mine, j + 3 == mine);
-          }
         }
         g += 2 * tiles;
         ns += mine;
@@ -424,19 +443,47 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
   } else {
     // ------------------------------------------------------------ softmax
-    const int t = warp >> 2;
-    const int q = warp & 3;
-    const int r = 32 * q + lane;  // row of the tile = TMEM lane
+    const int t = warp >> 3, group = (warp >> 2) & 1, q = warp & 3;
+    const int r = 32 * q + lane;     // row of the tile = TMEM lane
+    const int pair = 1 + 4 * t + q;  // named barrier of the two warps with the same rows
+    volatile uint64_t* decided = reinterpret_cast<volatile uint64_t*>(smem + C::kOffRows) + t * kM + r;
     const uint32_t lane_off = (uint32_t)(32 * q) << 16;
-    const uint32_t to = t_o(t) + lane_off;
+    const uint32_t ts = t_s(t, group) + lane_off, to = t_o(t) + lane_off;
     const float c2 = p.scale * kLog2e;
-    uint8_t* stage = smem + C::kOffStage + warp * C::kStageBytes;
+    uint8_t* stage = smem + C::kOffStage + (4 * t + q) * C::kStageBytes;
     uint32_t ns = 0, no = 0, g = 0;  // key tiles and items of this query tile, K / V tiles before this item
+    // A wait that ran out sets ok = false and ends the steps; the warps of a
+    // pair tell each other at the item's pair barriers.
     bool ok = true;
-    for (int n = 0; ok; ++n) {
+    auto wait = [&](uint64_t* bar, uint32_t parity, unsigned where) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where, tmo));
+    };
+    // The row's maximum and the number of the key tile that it was decided
+    // for, in one word: the thread of the other group sees both at once.
+    auto decide = [&](float m, uint32_t step) { *decided = ((uint64_t)(step + 1) << 32) | __float_as_uint(m); };
+    auto decision = [&](uint32_t step, float* m) {
+      uint64_t t0 = 0;
+      bool got = false;
+      for (uint32_t it = 1;; ++it) {
+        const uint64_t v = *decided;
+        got = (uint32_t)(v >> 32) == step + 1;
+        *m = __uint_as_float((uint32_t)v);
+        if (__all_sync(0xffffffffu, got)) return true;
+        if ((it & 63u) == 0) {
+          if (t0 == 0) t0 = gtimer();
+          const bool late = gtimer() - t0 > tmo.ns;
+          if (__any_sync(0xffffffffu, late || *abort_flag)) {
+            if (late) give_up(abort_flag, 3, tmo, &g_tok_fwd_status);
+            return false;
+          }
+        }
+      }
+    };
+    *decided = 0;
+    for (int n = 0;; ++n) {
       const int islot = n % kItems;
-      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 3, tmo));
-      if (!ok) break;
+      ok = ok && wait(&item_full[islot], (n / kItems) & 1, 3);
+      if (bar_any(pair, 64, !ok)) break;
       Item it;
       it.row = items[islot].row; it.n = items[islot].n; it.h = items[islot].h; it.k0 = items[islot].k0;
       it.nk = items[islot].nk; it.see = items[islot].see;
@@ -448,37 +495,50 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int see = p.pk.causal ? max(0, min(it.nk, it.see + t * kM + r)) : it.nk;  // keys this row sees
       // tiles from edge on hold keys that the tile's first row does not see
       const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + t * kM)) : it.nk) / kN;
-      float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < tiles; ++j, ++ns) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (ns & 1)], (ns >> 1) & 1, abort_flag, 3, tmo));
+      float m = -INFINITY, l = 0.f;  // l: of this group's key tiles, for the maximum m
+      // l for a new maximum
+      auto adopt = [&](float mn) {
+        if (mn != m) l *= ex2((m - mn) * c2);
+        m = mn;
+      };
+      for (int j = (ns & 1) == (uint32_t)group ? 0 : 1; j < tiles; j += 2) {
+        const uint32_t nn = ns + j;
+        ok = wait(&s_full[2 * t + group], (nn >> 1) & 1, 3);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ts = t_s(t, ns & 1) + lane_off;
-        uint32_t s[kN];
+        const int lim = j >= edge ? see - j * kN : kN;  // columns from lim on are not seen
+        uint32_t s[32];
         float* f = reinterpret_cast<float*>(s);
-        tc_ld32(ts, s);
-        tc_ld32(ts + 32, s + 32);
-        tc_wait_ld_regs(s);
-        tc_wait_ld_regs(s + 32);
-        if (j >= edge) {
-          const int lim = see - j * kN;
+        auto cut = [&](int first) {
+          if (j >= edge) {
 #pragma unroll
-          for (int c = 0; c < kN; ++c) f[c] = c < lim ? f[c] : -INFINITY;
-        }
-        const float mj = row_max<kN>(f);
+            for (int c = 0; c < 32; ++c) f[c] = first + c < lim ? f[c] : -INFINITY;
+          }
+        };
+        tc_ld32(ts, s);
+        tc_wait_ld_regs(s);
+        cut(0);
+        float mj = row_max<32>(f);
+        tc_ld32(ts + 32, s);
+        tc_wait_ld_regs(s);
+        cut(32);
+        mj = fmaxf(mj, row_max<32>(f));
         if (j == 0) {
           m = mj;
         } else {
+          float before;
+          ok = decision(nn - 1, &before);
+          if (!ok) break;
+          adopt(before);
           const bool grow = (mj - m) * c2 > kRescale;  // also from m = -inf
           if (__any_sync(0xffffffffu, grow)) {
             // the last product that wrote O has to be complete (the one
             // before it is: the scores of this tile came after it)
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (ns - 1) & 1, abort_flag, 3, tmo));
+            ok = wait(&o_done[t], (nn - 1) & 1, 3);
             if (!ok) break;
             tc_fence_after();
             const float a = grow ? ex2((m - mj) * c2) : 1.f;
-            if (grow) m = mj;
-            l *= a;
+            if (grow) adopt(mj);
 #pragma unroll 1
             for (int c = 0; c < DP; c += 16) {
               uint32_t o[16];
@@ -490,27 +550,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
           }
         }
+        decide(m, nn);
         const float mc = m == -INFINITY ? 0.f : m * c2;
         const float2 c22 = make_float2(c2, c2), mc2 = make_float2(-mc, -mc);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int h = 0; h < kN / 32; ++h) {
+        auto weights = [&](uint32_t dst) {  // over scores that have been read
           uint32_t w[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float2 x = __ffma2_rn(make_float2(f[32 * h + c], f[32 * h + c + 1]), c22, mc2);
+            const float2 x = __ffma2_rn(make_float2(f[c], f[c + 1]), c22, mc2);
             const float2 y = make_float2(ex2(x.x), ex2(x.y));
             sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], y);
             w[c / 2] = St<T>::pack(y.x, y.y);
           }
-          tmem_st16(ts + 16 * h, w);
-        }
+          tmem_st16(dst, w);
+        };
+        weights(ts + 32);
+        tc_ld32(ts, s);  // the first half once more: 64 scores and their weights at a time do not fit the registers
+        tc_wait_ld_regs(s);
+        cut(0);
+        weights(ts);
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         if (j >= edge) {
-          // V tile j: infinities and NaN out (see the top of the file)
+          // V tile j: infinities and NaN out (see above)
           const uint32_t gv = g + v_pos(j, all_tiles);
           uint8_t* tile = sKV + (gv % C::kSlots) * C::kSlotBytes;
-          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[gv % C::kSlots], (gv / C::kSlots) & 1, abort_flag, 3, tmo));
+          ok = wait(&kv_full[gv % C::kSlots], (gv / C::kSlots) & 1, 3);
           if (!ok) break;
           if (!row_is_finite<T, C::kChunks>(tile, tid & 127)) {
             *v_cleaned = 1;
@@ -522,67 +587,71 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + (ns & 1)]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + group]);
       }
-      if (!ok) break;
+      ns += tiles;
       g += 2 * all_tiles;
       if (rows <= 0) continue;
       // ---------------------------------------------------------- epilogue
       if (tiles > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1, abort_flag, 4, tmo));
+        float last;
+        ok = ok && decision(ns - 1, &last) && wait(&o_full[t], no & 1, 4);
         ++no;
-        if (!ok) break;
         tc_fence_after();
+        if (ok) adopt(last);
       }
+      if (bar_any(pair, 64, !ok)) break;
+      // both have the final maximum: its word serves to exchange the sums
+      reinterpret_cast<volatile float*>(decided)[group] = l;
+      named_bar(pair, 64);
+      l += reinterpret_cast<volatile float*>(decided)[1 - group];
+      named_bar(pair, 64);
+      if (group == 0) *decided = 0;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
-      if (p.lse != nullptr && r < rows)
+      if (p.lse != nullptr && r < rows && group == 0)
         p.lse[(int64_t)it.h * p.pk.T + it.row + t * kM + r] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
-      const int wrows = min(32, rows - 32 * q);  // of this warp
+      const int wrows = min(32, rows - 32 * q);  // of this warp's rows
       const bool fix = *v_cleaned != 0;
+      // 64 channels at a time, half of them by each warp of the pair
 #pragma unroll 1
       for (int c = 0; c < C::kChunks; ++c) {
         if (64 * c >= p.D) break;
-        uint32_t o[64];
-        if (tiles > 0) {
-          tc_ld32(to + 64 * c, o);
-          tc_ld32(to + 64 * c + 32, o + 32);
-          tc_wait_ld_regs(o);
-          tc_wait_ld_regs(o + 32);
-        }
-        if (lane == 0) bulk_wait_read0();  // the staging buffer is free
-        __syncwarp();
         uint8_t* row = stage + lane * 128;
+        uint32_t o[32];
+        if (tiles > 0) tc_ld32(to + 64 * c + 32 * group, o);
+        if (group == 0 && lane == 0) bulk_wait_read0();  // the staging buffer is free
+        named_bar(pair, 64);
+        if (tiles > 0) tc_wait_ld_regs(o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4; ++e) {
           float x[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = inv == 0.f ? 0.f : __uint_as_float(o[8 * e + i]) * inv;
-          *reinterpret_cast<uint4*>(row + ((e ^ (lane & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(row + (((4 * group + e) ^ (lane & 7)) << 4)) =
               make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
         }
         if (fix && tiles > 0) {
           // add the values taken out of the tiles on the edge of this item
           const int e0 = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN * kN;
           add_nonfinite<T>(row, lane, static_cast<const T*>(p.v.p) + (int64_t)it.k0 * p.v.t + (it.h / p.group) * p.v.h + 64 * c,
-                           p.v.t, e0, see, min(64, p.D - 64 * c));
+                           p.v.t, e0, see, 32 * group, min(32 * group + 32, p.D - 64 * c));
         }
         fence_proxy_async();
-        __syncwarp();
+        named_bar(pair, 64);
         const int row0 = it.row + t * kM + 32 * q;
         if (wrows == 32) {
-          if (lane == 0) {
+          if (group == 0 && lane == 0) {
             tma_store(&p.omap, stage, 64 * c, it.h, row0, 0);
             bulk_commit();
           }
         } else {  // the rows behind the sequence are not ours
-          for (int e = lane; e < wrows * 8; e += 32) {
+          for (int e = 32 * group + lane; e < wrows * 8; e += 64) {
             const int rr = e >> 3, piece = e & 7;
             if (64 * c + 8 * piece < p.D)
               *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(p.out.p)) + (int64_t)(row0 + rr) * p.out.t +
                                         (int64_t)it.h * p.out.h + 64 * c + 8 * piece) =
                   *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
           }
-          __syncwarp();
         }
       }
       tc_fence_before();  // O has been read: the next item's first product (after p_full) may overwrite it
@@ -595,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       hi = max(lo, e.x + e.y);
     }
     const int64_t gap = (int64_t)lo + (p.pk.T - hi);
-    for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < gap * p.Hq; i += (int64_t)gridDim.x * 8) {
+    for (int64_t i = (int64_t)blockIdx.x * 16 + warp; i < gap * p.Hq; i += (int64_t)gridDim.x * 16) {
       const int64_t k = i / p.Hq;
       const int h = (int)(i - k * p.Hq);
       const int64_t row = k < lo ? k : hi + (k - lo);
@@ -608,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }

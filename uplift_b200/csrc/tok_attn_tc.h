@@ -44,6 +44,16 @@ inline int read_status(unsigned int& symbol, bool clear) {
 }
 
 // ------------------------------------------------------------ waits
+// Ends the CTA's work: every bounded wait returns false from now on.
+__device__ __forceinline__ void give_up(volatile int* abort_flag, unsigned where, const WaitLimit& limit,
+                                        unsigned int* status) {
+  *abort_flag = 1;
+  atomicCAS(status, 0u, where);
+  if (limit.host_word != nullptr) {
+    *reinterpret_cast<volatile unsigned int*>(limit.host_word) = where;
+    __threadfence_system();
+  }
+}
 // mbar_wait_status of la_tc_common.h as inline code.
 __device__ __forceinline__ bool mbar_wait_inline(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
                                                  const WaitLimit& limit, unsigned int* status) {
@@ -58,17 +68,26 @@ __device__ __forceinline__ bool mbar_wait_inline(uint64_t* b, uint32_t parity, v
       break;
     }
     if (gtimer() - t0 > limit.ns) {
-      *abort_flag = 1;
-      atomicCAS(status, 0u, where);
-      if (limit.host_word != nullptr) {
-        *reinterpret_cast<volatile unsigned int*>(limit.host_word) = where;
-        __threadfence_system();
-      }
+      give_up(abort_flag, where, limit, status);
       ok = false;
       break;
     }
   }
   return ok;
+}
+
+// Named barrier of n threads that tells all of them whether any had `pred`.
+__device__ __forceinline__ bool bar_any(int id, int n, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
 }
 
 // ------------------------------------------------------------ sequences
