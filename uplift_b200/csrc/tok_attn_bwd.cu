@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     bool ok = true;
     uint32_t g = 0, nx = 0;
     for (int n = 0;; ++n) {
-      const int64_t i = (int64_t)blockIdx.x + (int64_t)n * gridDim.x;
+      const int64_t i = dealt(n);
       int b = 0, local = 0, tiles = 0;
       const int64_t tile = i / p.heads;
       const bool more = tile < (1ll << 31) && walk.find(p.pk, KEYS, kM, (int)tile, &b, &local, &tiles);
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
         const int shift = s.nk - s.nq;  // causal: query i sees keys <= i + shift
         if (KEYS) {
           const int seg = segment(p.pk.cu_k, b, p.pk.S).y;
-          const int j0 = local * kM;  // the first keys are seen by most queries
+          const int j0 = local * kM;
           it.row = s.k0 + j0;
           it.n = min(kM, seg - j0);
           it.live = max(0, min(it.n, s.nk - j0));
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
           it.ny = it.live > 0 ? max(0, s.nq - i0) : 0;
           it.off = j0 - shift - i0;
         } else {
-          const int i0 = (p.pk.causal ? tiles - 1 - local : local) * kM;  // the last queries see most keys
+          const int i0 = local * kM;
           it.row = s.q0 + i0;
           it.n = min(kM, s.nq - i0);
           it.live = it.n;

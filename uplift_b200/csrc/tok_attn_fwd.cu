@@ -283,15 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       uint32_t g = 0;  // K / V slot uses
       uint32_t nq = 0;  // items with loads
       for (int n = 0;; ++n) {
-        const int64_t i = (int64_t)blockIdx.x + (int64_t)n * gridDim.x;
+        const int64_t i = dealt(n);
         int b = 0, local = 0, tiles = 0;
         const int64_t tile = i / p.Hq;
         const bool more = tile < (1ll << 31) && walk.find(p.pk, false, kItemRows, (int)tile, &b, &local, &tiles);
         Item it{};
         if (more) {
           const Seq s = sequence(p.pk, b);
-          // the rows that see most come first
-          const int i0 = (p.pk.causal ? tiles - 1 - local : local) * kItemRows;
+          const int i0 = local * kItemRows;
           it.row = s.q0 + i0;
           it.n = min(kItemRows, s.nq - i0);
           it.h = (int)(i - tile * p.Hq);

@@ -92,42 +92,74 @@ __device__ __forceinline__ bool bar_any(int id, int n, bool pred) {
 
 // ------------------------------------------------------------ sequences
 // Tile number -> (sequence, tile of the sequence), for numbers that only
-// grow: a warp looks at 32 sequences at a time and goes on from where the
-// last search ended.  `by_keys`: tiles of the key segments, else of the
-// queries.
+// grow: a warp looks at 32 sequences at a time (a lane each) and goes on from
+// where the last search ended.  `by_keys`: tiles of the key segments, else of
+// the queries.
+//
+// A causal query tile costs in proportion to its index, a causal key tile to
+// its distance from the end.  Among 32 sequences the costliest tiles come
+// first: level by level, from the longest sequence's last tile (first, by
+// keys) down, the tiles of equal cost of all sequences that have them.  Dealt
+// to the CTAs forth and back, that evens out their work without a counter.
 struct TileWalk {
   int b0 = 0;       // first sequence of the window
-  int before = 0;   // tiles before the window
+  int before = 0;   // tiles before the window (not causal) or the level
+  int n = -1;       // tiles of the lane's sequence; -1: not read yet
+  int level = 0;    // cost, in tiles, of the tiles at hand
   // all lanes; false: there is no such tile
   __device__ __forceinline__ bool find(const Packing& p, bool by_keys, int tile_rows, int tile, int* b, int* local,
                                        int* tiles) {
     const int lane = threadIdx.x & 31;
-    while (b0 < p.B) {
-      int n = 0;
-      if (b0 + lane < p.B)
-        n = ((by_keys ? segment(p.cu_k, b0 + lane, p.S).y : segment(p.cu_q, b0 + lane, p.T).y) + tile_rows - 1) /
-            tile_rows;
-      int sum = n;  // inclusive scan
+    for (;;) {
+      if (n < 0) {
+        if (b0 >= p.B) return false;
+        n = 0;
+        if (b0 + lane < p.B)
+          n = ((by_keys ? segment(p.cu_k, b0 + lane, p.S).y : segment(p.cu_q, b0 + lane, p.T).y) + tile_rows - 1) /
+              tile_rows;
+        level = __reduce_max_sync(0xffffffffu, n);
+      }
+      if (p.causal) {
+        while (level > 0) {
+          const unsigned have = __ballot_sync(0xffffffffu, n >= level);
+          const int cnt = __popc(have);
+          if (tile < before + cnt) {
+            const int l = __fns(have, 0, tile - before + 1);
+            *tiles = __shfl_sync(0xffffffffu, n, l);
+            *local = by_keys ? *tiles - level : level - 1;
+            *b = b0 + l;
+            return true;
+          }
+          before += cnt;
+          --level;
+        }
+      } else {
+        int sum = n;  // inclusive scan
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        const int total = __shfl_sync(0xffffffffu, sum, 31);
+        if (tile < before + total) {
+          const int l = __ffs(__ballot_sync(0xffffffffu, tile < before + sum)) - 1;
+          *tiles = __shfl_sync(0xffffffffu, n, l);
+          *local = tile - before - (__shfl_sync(0xffffffffu, sum, l) - *tiles);
+          *b = b0 + l;
+          return true;
+        }
+        before += total;
       }
-      const int total = __shfl_sync(0xffffffffu, sum, 31);
-      if (tile < before + total) {
-        const unsigned hit = __ballot_sync(0xffffffffu, tile < before + sum);
-        const int l = __ffs(hit) - 1;
-        *tiles = __shfl_sync(0xffffffffu, n, l);
-        *local = tile - before - (__shfl_sync(0xffffffffu, sum, l) - *tiles);
-        *b = b0 + l;
-        return true;
-      }
-      before += total;
       b0 += 32;
+      n = -1;
     }
-    return false;
   }
 };
+
+// Item number of a CTA's n-th turn: items are dealt forth and back.
+__device__ __forceinline__ int64_t dealt(int n) {
+  return (int64_t)n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
 
 // ------------------------------------------------------------ MMA issue
 // One lane of a converged warp.  The MMA warp runs its loop with all lanes,
