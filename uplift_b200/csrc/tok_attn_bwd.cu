@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
 
   const int tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     mbar_init(x_full, 1);
     mbar_init(x_empty, 1);
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   auto col_s = [&](uint32_t b) { return tmem + b * 2 * kN; };
   auto col_dp = [&](uint32_t b) { return tmem + b * 2 * kN + kN; };
   const uint32_t col_acc = tmem + C::kColAcc;
@@ -269,80 +269,87 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
-      constexpr uint32_t kIdA = idesc_f16(St<T>::kFmt, 1, kM, DP);
-      const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
-      const uint32_t aX = su32(sX), aY = su32(sY);
-      bool ok = true;
-      uint32_t g = 0, nx = 0;  // steps and items with steps so far
-      auto first = [&](uint32_t gs) {  // S and dP of step gs
-        const uint32_t y = aY + (gs % C::kStages) * 2 * C::kYBytes;
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t d = w == 0 ? col_s(gs & 1) : col_dp(gs & 1);
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const uint32_t c = ks >> 2, k = 32 * (ks & 3);
-            tc_mma(d, mdesc(aX + w * C::kXBytes + c * C::kXChunk + k, 16, 1024, kLayoutSw128),
-                   mdesc(y + w * C::kYBytes + c * C::kYChunk + k, 16, 1024, kLayoutSw128), kIdS, ks > 0);
-          }
+    constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
+    constexpr uint32_t kIdA = idesc_f16(St<T>::kFmt, 1, kM, DP);
+    const int ksteps = (p.D + 15) / 16;  // channels behind D are zero
+    // descriptors: the start address counts 16 bytes in their lowest bits
+    const uint64_t dx = mdesc(su32(sX), 16, 1024, kLayoutSw128), dy = mdesc(su32(sY), 16, 1024, kLayoutSw128);
+    const uint64_t dyt = mdesc(su32(sY), C::kYChunk, 1024, kLayoutSw128);
+    bool ok = true;
+    uint32_t g = 0, nx = 0;  // steps and items with steps so far
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, 2, tmo));
+    };
+    auto ready = [&](uint32_t gs) { return wait(&y_full[gs % C::kStages], (gs / C::kStages) & 1); };
+    auto first = [&](uint32_t gs) {  // (one lane) S and dP of step gs
+      const uint64_t y = dy + (gs % C::kStages) * (2 * C::kYBytes >> 4);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const uint32_t c = ks >> 2, k = 32 * (ks & 3);
+          if (ks < ksteps)
+            tc_mma(w == 0 ? col_s(gs & 1) : col_dp(gs & 1), dx + ((w * C::kXBytes + c * C::kXChunk + k) >> 4),
+                   y + ((w * C::kYBytes + c * C::kYChunk + k) >> 4), kIdS, ks > 0);
         }
-        tc_commit(&s_full[gs & 1]);
-      };
-      for (int n = 0; ok; ++n) {
-        const int islot = n % kItems;
-        ok = mbar_wait(&item_full[islot], (n / kItems) & 1, abort_flag, 2, tmo);
+      }
+      tc_commit(&s_full[gs & 1]);
+    };
+    for (int n = 0; ok; ++n) {
+      const int islot = n % kItems;
+      ok = wait(&item_full[islot], (n / kItems) & 1);
+      if (!ok) break;
+      const int rows = items[islot].n;
+      const int total = items[islot].steps * passes;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[islot]);
+      if (rows == 0) break;
+      if (total == 0) continue;
+      ok = wait(x_full, nx & 1);
+      // up to two steps of first products ahead of the second ones
+      for (int j = 0; j < min(2, total) && ok; ++j) {
+        ok = ready(g + j);
         if (!ok) break;
-        const int rows = items[islot].n;
-        const int total = items[islot].steps * passes;
-        mbar_arrive(&item_empty[islot]);
-        if (rows == 0) break;
-        if (total == 0) continue;
-        ok = mbar_wait(x_full, nx & 1, abort_flag, 2, tmo);
-        // up to two steps of first products ahead of the second ones
-        for (int j = 0; j < min(2, total) && ok; ++j) {
-          ok = mbar_wait(&y_full[(g + j) % C::kStages], ((g + j) / C::kStages) & 1, abort_flag, 2, tmo);
-          if (!ok) break;
-          tc_fence_after();
+        tc_fence_after();
+        if (elect_one()) {
           first(g + j);
+          if (j + 1 == total) tc_commit(x_empty);
         }
-        if (total <= 2) tc_commit(x_empty);
-        ok = ok && mbar_wait(acc_empty, (nx & 1) ^ 1, abort_flag, 2, tmo);
-        ++nx;
-        for (int j = 0; j < total && ok; ++j) {
-          const uint32_t gs = g + j, b = gs & 1;
-          ok = mbar_wait(&p_full[b], (gs >> 1) & 1, abort_flag, 2, tmo);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t y = aY + (gs % C::kStages) * 2 * C::kYBytes;
+        __syncwarp();
+      }
+      ok = ok && wait(acc_empty, (nx & 1) ^ 1);
+      ++nx;
+      for (int j = 0; j < total && ok; ++j) {
+        const uint32_t gs = g + j, b = gs & 1;
+        // the step after next is there long before P and dS, which are waited
+        // for last: the products follow them at once
+        ok = (j + 2 >= total || ready(gs + 2)) && wait(&p_full[b], (gs >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t y = dyt + (gs % C::kStages) * (2 * C::kYBytes >> 4);
           if (KEYS) {
 #pragma unroll
             for (int ks = 0; ks < kN / 16; ++ks)
-              mma_tmem_a(col_acc, col_s(b) + 8 * ks, mdesc(y + C::kYBytes + 2048 * ks, C::kYChunk, 1024, kLayoutSw128), kIdA,
-                         (j > 0 || ks > 0) ? 1u : 0u);
+              mma_tmem_a(col_acc, col_s(b) + 8 * ks, y + ((C::kYBytes + 2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int ks = 0; ks < kN / 16; ++ks)
-            mma_tmem_a(col_acc + (KEYS ? DP : 0), col_dp(b) + 8 * ks, mdesc(y + 2048 * ks, C::kYChunk, 1024, kLayoutSw128),
-                       kIdA, (j > 0 || ks > 0) ? 1u : 0u);
+            mma_tmem_a(col_acc + (KEYS ? DP : 0), col_dp(b) + 8 * ks, y + ((2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
           tc_commit(&y_empty[gs % C::kStages]);
-          if (j + 2 < total) {
-            const uint32_t gn = gs + 2;
-            ok = mbar_wait(&y_full[gn % C::kStages], (gn / C::kStages) & 1, abort_flag, 2, tmo);
-            if (!ok) break;
-            tc_fence_after();
-            first(gn);
-            if (j + 3 == total) tc_commit(x_empty);
-          }
+          if (j + 2 < total) first(gs + 2);
+          if (j + 3 == total) tc_commit(x_empty);
+          if (j + 1 == total) tc_commit(acc_full);
         }
-        if (!ok) break;
-        tc_commit(acc_full);
-        g += total;
+        __syncwarp();
       }
-      // all issued MMAs complete before TMEM can be released (this wait
-      // ignores the abort flag: it must not be cut short by another role)
-      tc_commit(drain);
-      mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
+      g += total;
     }
+    // all issued MMAs complete before TMEM can be released (this wait
+    // ignores the abort flag: it must not be cut short by another role)
+    if (elect_one()) tc_commit(drain);
+    __syncwarp();
+    mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
   } else if (warp == 10) {
     // ------------------------------------- lse and delta of the columns
     if (KEYS) {
