@@ -114,8 +114,9 @@ def _rows(t: torch.Tensor):
 
 def _new_rows(t: torch.Tensor):
     """A new contiguous tensor like t, as _rows gives it."""
-    n = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
-    return (n.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]), n
+    n = torch.empty_like(t, memory_format=torch.contiguous_format)
+    _, heads, D = t.shape
+    return (n.data_ptr(), heads * D, D), n
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -174,6 +175,10 @@ def _partial_floats(D: int) -> int:
 def norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
     """Launch uplift_tok_norm_rotate (no autograd)."""
     index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    return _norm_rotate(index, wt, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+def _norm_rotate(index, wt, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     T, Hq, D = q.shape
     P, half = cos.shape
     lib = _native.load()
@@ -197,6 +202,12 @@ def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positio
                              interleaved=False, need_weights=True):
     """Launch uplift_tok_norm_rotate_backward: (dq, dk, dweights [2, D] in the weights' type; empty when not needed)."""
     index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
+    return _norm_rotate_backward(index, wt, gq.to(q.dtype), gk.to(q.dtype), q, k, q_weight, k_weight, cos, sin,
+                                 positions, eps, interleaved, need_weights)
+
+
+def _norm_rotate_backward(index, wt, gq, gk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved,
+                          need_weights):
     T, Hq, D = q.shape
     P, half = cos.shape
     lib = _native.load()
@@ -204,8 +215,8 @@ def norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positio
     with _on(index):
         rq, q = _rows(q)
         rk, k = _rows(k)
-        rg, gq = _rows(gq.to(q.dtype))
-        rh, gk = _rows(gk.to(q.dtype))
+        rg, gq = _rows(gq)
+        rh, gk = _rows(gk)
         rdq, dq = _new_rows(q)
         rdk, dk = _new_rows(k)
         dw = torch.empty((2, D) if need_weights else (0,), dtype=_weight_dtype(q_weight, k_weight), device=q.device)
@@ -225,9 +236,10 @@ class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.checked = index, wt = _norm_rotate_args(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.eps, ctx.interleaved = eps, interleaved
         ctx.set_materialize_grads(False)
-        return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        return _norm_rotate(index, wt, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -238,8 +250,8 @@ class _NormRotate(torch.autograd.Function):
             gq = torch.zeros_like(q)
         if gk is None:
             gk = torch.zeros_like(k)
-        dq, dk, dw = norm_rotate_backward_raw(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, ctx.eps,
-                                              ctx.interleaved, need_weights=nqw or nkw)
+        dq, dk, dw = _norm_rotate_backward(*ctx.checked, gq, gk, q, k, q_weight, k_weight, cos, sin, positions,
+                                           ctx.eps, ctx.interleaved, nqw or nkw)
         return (dq if nq else None, dk if nk else None, dw[0] if nqw else None, dw[1] if nkw else None, None, None,
                 None, None, None)
 
@@ -313,7 +325,9 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
     eps, interleaved = float(eps), bool(interleaved)
     if torch.compiler.is_compiling():
         return torch.ops.uplift_b200.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                    (q_weight is not None and q_weight.requires_grad) or
+                                    (k_weight is not None and k_weight.requires_grad)):
         return _NormRotate.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     return norm_rotate_raw(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
@@ -382,12 +396,16 @@ def packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k=None,
     """Launch uplift_tok_attention_backward: (dq, dk, dv)."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
+    return _packed_attention_backward(index, g.to(q.dtype), q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale)
+
+
+def _packed_attention_backward(index, g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale):
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
     lib = _native.load()
     _native.host_status.raise_if_set()
     cu_q, cu_k, used_k, lse = cu_q.contiguous(), cu_k.contiguous(), _c(used_k), lse.contiguous()
     with _on(index):
-        rg, g = _rows(g.to(q.dtype))
+        rg, g = _rows(g)
         rq, q = _rows(q)
         rk, k = _rows(k)
         rv, v = _rows(v)
@@ -421,7 +439,8 @@ class _PackedAttention(torch.autograd.Function):
         if g is None:
             return (None,) * 8
         q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
-        grads = packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal, ctx.scale)
+        grads = _packed_attention_backward(q.get_device(), g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal,
+                                           ctx.scale)
         return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
 
 
