@@ -1,8 +1,10 @@
 // Attention over packed sequences on the tensor cores of B200 (sm_100a),
 // bf16 / fp16, D <= 128.
 //
-// An item is 256 query rows of one head of one sequence (two tiles of
-// M = 128), which walks the key tiles (64 keys) that its rows see:
+// An item is two tiles of 128 query rows (M = 128) of one sequence that read
+// the same key head: the same rows of two query heads where the group has an
+// even number of them, else 256 rows of one head.  It walks the key tiles (64
+// keys) that its rows see:
 //
 //   S_t[128 x 64] = Q_t . K_j^T                     (tcgen05, fp32 in TMEM)
 //   m = max(m, rowmax S), P = exp2((S - m) scale log2 e), l += rowsum P
@@ -61,7 +63,6 @@ namespace tok {
 namespace fwd {
 
 constexpr int kM = 128;            // query rows of a tile
-constexpr int kItemRows = 2 * kM;
 constexpr int kN = 64;             // keys of a tile
 constexpr int kQChunk = kM * 128, kKvChunk = kN * 128;  // 64 channels of a tile
 constexpr int kThreads = 640;
@@ -92,8 +93,8 @@ struct Cfg {
 
 struct Item {
   int row;        // first query row in the tensor
-  int n;          // its rows, 1..256; 0: no more items
-  int h;          // query head
+  int n;          // its rows, 1..128 (256 if one head); 0: no more items
+  int h;          // (first) query head
   int k0;         // first key row in the tensor
   int nk;         // keys of the sequence
   int see;        // keys that the first row sees (may be negative; each next row sees one more when causal)
@@ -107,6 +108,8 @@ struct Params {
   float* lse;
   Packing pk;
   int Hq, group, D;
+  int heads;     // query heads of an item: 1 or 2
+  int row_step;  // from the rows of the first query tile to those of the second: 128, or 0 with two heads
   float scale;
   uint64_t timeout_ns;
   unsigned int* host_status;
@@ -285,23 +288,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       for (int n = 0;; ++n) {
         const int64_t i = dealt(n);
         int b = 0, local = 0, tiles = 0;
-        const int64_t tile = i / p.Hq;
-        const bool more = tile < (1ll << 31) && walk.find(p.pk, false, kItemRows, (int)tile, &b, &local, &tiles);
+        const int per_tile = p.Hq / p.heads, item_rows = kM + p.row_step;
+        const int64_t tile = i / per_tile;
+        const bool more = tile < (1ll << 31) && walk.find(p.pk, false, item_rows, (int)tile, &b, &local, &tiles);
         Item it{};
         if (more) {
           const Seq s = sequence(p.pk, b);
-          const int i0 = local * kItemRows;
+          const int i0 = local * item_rows;
           it.row = s.q0 + i0;
-          it.n = min(kItemRows, s.nq - i0);
-          it.h = (int)(i - tile * p.Hq);
+          it.n = min(item_rows, s.nq - i0);
+          it.h = (int)(i - tile * per_tile) * p.heads;
           it.k0 = s.k0;
           it.nk = s.nk;
           it.see = p.pk.causal ? i0 + 1 + s.nk - s.nq : s.nk;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const int last = min(it.n, (t + 1) * kM) - 1;  // last row of the tile
+            const int last = min(it.n, t * p.row_step + kM) - 1;  // last row of the tile
             const int see = p.pk.causal ? max(0, min(s.nk, it.see + last)) : s.nk;
-            it.nt[t] = last >= t * kM ? (see + kN - 1) / kN : 0;
+            it.nt[t] = last >= t * p.row_step ? (see + kN - 1) / kN : 0;
           }
         }
         if (lane == 0) {
@@ -316,12 +320,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           if (ok && tiles_k > 0) {
             ok = mbar_wait(q_empty, (nq & 1) ^ 1, abort_flag, 1, tmo);
             if (ok) {
-              const int qt = it.n > kM ? 2 : 1;  // query tiles with rows
+              const int qt = p.heads > 1 || it.n > kM ? 2 : 1;  // query tiles with rows
               mbar_expect_tx(q_full, qt * C::kQBytes);
               for (int t = 0; t < qt; ++t) {
 #pragma unroll
                 for (int c = 0; c < C::kChunks; ++c)
-                  load_rows(sQ + t * C::kQBytes + c * kQChunk, &p.qmap, q_full, 64 * c, it.h, it.row + t * kM);
+                  load_rows(sQ + t * C::kQBytes + c * kQChunk, &p.qmap, q_full, 64 * c, it.h + t * (p.heads - 1), it.row + t * p.row_step);
               }
             }
             ++nq;
@@ -490,10 +494,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[islot]);
       if (it.n == 0) break;
-      const int rows = min(kM, it.n - t * kM);  // of this tile; may be <= 0
-      const int see = p.pk.causal ? max(0, min(it.nk, it.see + t * kM + r)) : it.nk;  // keys this row sees
+      it.h += t * (p.heads - 1);
+      const int first = t * p.row_step;            // first row of this tile
+      const int rows = min(kM, it.n - first);      // its rows; may be <= 0
+      const int see = p.pk.causal ? max(0, min(it.nk, it.see + first + r)) : it.nk;  // keys this row sees
       // tiles from edge on hold keys that the tile's first row does not see
-      const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + t * kM)) : it.nk) / kN;
+      const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + first)) : it.nk) / kN;
       float m = -INFINITY, l = 0.f;  // l: of this group's key tiles, for the maximum m
       // l for a new maximum
       auto adopt = [&](float mn) {
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       if (group == 0) *decided = 0;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
       if (p.lse != nullptr && r < rows && group == 0)
-        p.lse[(int64_t)it.h * p.pk.T + it.row + t * kM + r] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+        p.lse[(int64_t)it.h * p.pk.T + it.row + first + r] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
       const int wrows = min(32, rows - 32 * q);  // of this warp's rows
       const bool fix = *v_cleaned != 0;
       // 64 channels at a time, half of them by each warp of the pair
@@ -637,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         }
         fence_proxy_async();
         named_bar(pair, 64);
-        const int row0 = it.row + t * kM + 32 * q;
+        const int row0 = it.row + first + 32 * q;
         if (wrows == 32) {
           if (group == 0 && lane == 0) {
             tma_store(&p.omap, stage, 64 * c, it.h, row0, 0);
@@ -728,11 +734,13 @@ int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
   p.pk = a.pk;
   p.Hq = a.Hq;
   p.group = a.Hq / a.Hk;
+  p.heads = p.group % 2 == 0 ? 2 : 1;
+  p.row_step = p.heads == 2 ? 0 : kM;
   p.D = a.D;
   p.scale = a.scale;
   p.timeout_ns = tc_test_timeout_ns() != 0 ? tc_test_timeout_ns() : kTimeoutNs;
   p.host_status = host_status_word();
-  const int64_t most = ((int64_t)a.pk.T / kItemRows + a.pk.B) * a.Hq;  // items, at most
+  const int64_t most = ((int64_t)a.pk.T / (kM + p.row_step) + a.pk.B) * (a.Hq / p.heads);  // items, at most
   const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
   if (a.dtype == UPLIFT_LA_BF16)
     return a.D <= 64 ? launch<__nv_bfloat16, 64>(p, dev, grid, s) : launch<__nv_bfloat16, 128>(p, dev, grid, s);
