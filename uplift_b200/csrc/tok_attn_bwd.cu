@@ -24,10 +24,12 @@
 // while one group of warps forms P and dS of a step the tensor cores work on
 // the next.
 //
-// Roles (384 threads, one persistent CTA per SM): warps 0-3 and 4-7 the two
-// groups, taking steps in turn (a thread per row that stays) and storing the
-// results; warp 8 looks items up and issues TMA loads; warp 9 issues MMAs;
-// warp 10 (KEYS) fetches lse and delta of the queries that go by.
+// Roles (640 threads, one persistent CTA per SM): warps 0-7 and 8-15 form P
+// and dS of the steps in turn (two threads per row that stays, 32 columns
+// each) and store the results; warp 16 looks items up and issues TMA loads;
+// warp 17 issues MMAs, and warp 19 does its waiting, so that the tensor cores
+// are not idle for the length of two barrier waits per step; warp 18 (KEYS)
+// fetches lse and delta of the queries that go by.
 //
 // Rows that go by behind the end of their sequence belong to the next one:
 // their P and dS are set to zero and the rows in shared memory too, since an
@@ -50,7 +52,7 @@ namespace bwd {
 
 constexpr int kM = 128;   // rows that stay
 constexpr int kN = 64;    // rows that go by in a step
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
 constexpr int kTmemCols = 512;
 constexpr int kItems = 2;
 constexpr int kAux = 4;   // ring of lse / delta
@@ -68,12 +70,12 @@ struct Cfg {
   static constexpr int kOffY = 2 * kXBytes;
   static constexpr int kOffStage = kOffY + kStages * 2 * kYBytes;
   static constexpr int kStageBytes = 32 * 128;                  // a warp's 32 rows x 64 channels
-  static constexpr int kOffAux = kOffStage + 8 * kStageBytes;
+  static constexpr int kOffAux = kOffStage + 16 * kStageBytes;
   static constexpr int kOffBar = kOffAux + kAux * 2 * kN * 4;
   static constexpr int kNumBars = 2 + 2 * kStages + 2 * kAux + 4 + 2 + 2 * kItems + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffItems = kOffMisc + 32;
-  static constexpr int kSmem = kOffItems + kItems * 48 + 1024;  // + base alignment slack
+  static constexpr int kSmem = kOffItems + kItems * 32;
   static_assert(kSmem <= 232448, "shared memory");
   // TMEM columns: two buffers of S and dP, then the sums
   static constexpr int kColAcc = 4 * kN;
@@ -114,8 +116,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((su32(smem) & 1023u) != 0) {  // the swizzled tiles need it, and the declaration asks for it
+    if (threadIdx.x == 0) atomicCAS(&g_tok_bwd_status, 0u, 1u);
+    return;
+  }
   uint8_t* sX = smem + C::kOffX;
   uint8_t* sY = smem + C::kOffY;
   float* sAux = reinterpret_cast<float*>(smem + C::kOffAux);
@@ -135,6 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   uint64_t* drain = item_empty + kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  uint32_t* go = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 20);  // steps whose second products may begin
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
 
   const int tid = threadIdx.x;
@@ -148,24 +154,25 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     }
     for (int i = 0; i < kAux; ++i) {
       mbar_init(&a_full[i], 1);
-      mbar_init(&a_empty[i], 4);
+      mbar_init(&a_empty[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
+    mbar_init(acc_empty, 16);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], KEYS ? 10 : 9);  // 8 warps of the groups, MMA, lse / delta
+      mbar_init(&item_empty[i], KEYS ? 19 : 18);  // 16 warps of the groups, MMA, its forerunner, lse / delta
     }
     mbar_init(drain, 1);
     abort_flag[0] = 0;
     abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
+    *go = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -177,10 +184,13 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   auto col_dp = [&](uint32_t b) { return tmem + b * 2 * kN + kN; };
   const uint32_t col_acc = tmem + C::kColAcc;
   const WaitLimit tmo{p.timeout_ns, p.host_status};
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, 2, tmo));
+  };
   // heads that go by per item
   const int passes = KEYS ? p.group : 1;
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       prefetch_map(&p.x0);
@@ -267,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
       const uint64_t t0 = gtimer();
       while (gtimer() - t0 < 200000ull) {}
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ---------------------------------------------------------- MMA issuer
     constexpr uint32_t kIdS = idesc_f16(St<T>::kFmt, 0, kM, kN);
     constexpr uint32_t kIdA = idesc_f16(St<T>::kFmt, 1, kM, DP);
@@ -277,9 +287,6 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     const uint64_t dyt = mdesc(su32(sY), C::kYChunk, 1024, kLayoutSw128);
     bool ok = true;
     uint32_t g = 0, nx = 0;  // steps and items with steps so far
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, 2, tmo));
-    };
     auto ready = [&](uint32_t gs) { return wait(&y_full[gs % C::kStages], (gs / C::kStages) & 1); };
     auto first = [&](uint32_t gs) {  // (one lane) S and dP of step gs
       const uint64_t y = dy + (gs % C::kStages) * (2 * C::kYBytes >> 4);
@@ -321,9 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
       ++nx;
       for (int j = 0; j < total && ok; ++j) {
         const uint32_t gs = g + j, b = gs & 1;
-        // the step after next is there long before P and dS, which are waited
-        // for last: the products follow them at once
-        ok = (j + 2 >= total || ready(gs + 2)) && wait(&p_full[b], (gs >> 1) & 1);
+        ok = wait_raised(go, gs + 1, abort_flag, 2, tmo, &g_tok_bwd_status);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -331,11 +336,11 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
           if (KEYS) {
 #pragma unroll
             for (int ks = 0; ks < kN / 16; ++ks)
-              mma_tmem_a(col_acc, col_s(b) + 8 * ks, y + ((C::kYBytes + 2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
+              mma_tmem_a(col_acc, col_s(b) + 8 * (ks & 1) + 32 * (ks >> 1), y + ((C::kYBytes + 2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int ks = 0; ks < kN / 16; ++ks)
-            mma_tmem_a(col_acc + (KEYS ? DP : 0), col_dp(b) + 8 * ks, y + ((2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
+            mma_tmem_a(col_acc + (KEYS ? DP : 0), col_dp(b) + 8 * (ks & 1) + 32 * (ks >> 1), y + ((2048 * ks) >> 4), kIdA, (j > 0 || ks > 0) ? 1u : 0u);
           tc_commit(&y_empty[gs % C::kStages]);
           if (j + 2 < total) first(gs + 2);
           if (j + 3 == total) tc_commit(x_empty);
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     if (elect_one()) tc_commit(drain);
     __syncwarp();
     mbar_wait(drain, 0, abort_flag + 1, 2, tmo);
-  } else if (warp == 10) {
+  } else if (warp == 18) {
     // ------------------------------------- lse and delta of the columns
     if (KEYS) {
       bool ok = true;
@@ -389,10 +394,30 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
         }
       }
     }
-  } else if (warp < 8) {
+  } else if (warp == 19) {
+    // --------------------------------- forerunner of the MMA issuer: waits
+    // for what a step needs (P and dS, the tiles of the step after next) and
+    // raises a counter
+    bool ok = true;
+    uint32_t g = 0;
+    for (int n = 0; ok; ++n) {
+      const int islot = n % kItems;
+      ok = wait(&item_full[islot], (n / kItems) & 1);
+      if (!ok) break;
+      const int rows = items[islot].n;
+      const int total = items[islot].steps * passes;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[islot]);
+      if (rows == 0) break;
+      for (int j = 0; j < total && ok; ++j, ++g) {
+        ok = (j + 2 >= total || wait(&y_full[(g + 2) % C::kStages], ((g + 2) / C::kStages) & 1)) &&
+             wait(&p_full[g & 1], (g >> 1) & 1);
+        if (ok && lane == 0) raise_to(go, g + 1);
+      }
+    }
+  } else {
     // ------------------------------------------------------------ P and dS
-    const int w = warp >> 2;
-    const int q = warp & 3;
+    const int w = warp >> 3, half = (warp >> 2) & 1, q = warp & 3;
     const int r = 32 * q + lane;  // row that stays = TMEM lane
     const uint32_t lane_off = (uint32_t)(32 * q) << 16;
     const float c2 = p.scale * kLog2e;
@@ -436,23 +461,24 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
           else hi = min(hi, r + it.off - j * kN);
         }
         const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kN);
-        const uint32_t ts = col_s(w) + lane_off, td = col_dp(w) + lane_off;
+        constexpr int kCols = kN / 2;  // of this thread: columns kCols * half ..
+        const uint32_t ts = col_s(w) + kCols * half + lane_off, td = col_dp(w) + kCols * half + lane_off;
 #pragma unroll
-        for (int c = 0; c < kN; c += 32) {
-          uint32_t s[32], d[32];
-          tc_ld32(ts + c, s);
-          tc_ld32(td + c, d);
-          tc_wait_ld_regs(s);
-          tc_wait_ld_regs(d);
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t s[16], d[16];
+          tc_ld16(ts + c, s);
+          tc_ld16(td + c, d);
+          tc_wait_ld_regs16(s);
+          tc_wait_ld_regs16(d);
           float* fs = reinterpret_cast<float*>(s);
           float* fd = reinterpret_cast<float*>(d);
           const float2 c22 = make_float2(c2, c2);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
+          for (int e = 0; e < 16; e += 4) {
             float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndelta, ndelta, ndelta, ndelta);
             if (KEYS) {
-              nl = *reinterpret_cast<const float4*>(aux + c + e);
-              nd = *reinterpret_cast<const float4*>(aux + kN + c + e);
+              nl = *reinterpret_cast<const float4*>(aux + kCols * half + c + e);
+              nd = *reinterpret_cast<const float4*>(aux + kN + kCols * half + c + e);
             }
             const float2 x0 = __ffma2_rn(make_float2(fs[e], fs[e + 1]), c22, make_float2(nl.x, nl.y));
             const float2 x1 = __ffma2_rn(make_float2(fs[e + 2], fs[e + 3]), c22, make_float2(nl.z, nl.w));
@@ -464,27 +490,28 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
           }
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const bool seen = c + e >= lo && c + e < hi;
+            for (int e = 0; e < 16; ++e) {
+              const int col = kCols * half + c + e;
+              const bool seen = col >= lo && col < hi;
               fs[e] = seen ? fs[e] : 0.f;
               fd[e] = seen ? fd[e] : 0.f;
             }
           }
-          uint32_t ps[16], ds[16];
+          uint32_t ps[8], ds[8];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 8; ++e) {
             ps[e] = St<T>::pack(fs[2 * e], fs[2 * e + 1]);
             ds[e] = St<T>::pack(fd[2 * e], fd[2 * e + 1]);
           }
           // over columns that have been read
-          if (KEYS) tmem_st16(ts + c / 2, ps);
-          tmem_st16(td + c / 2, ds);
+          if (KEYS) tmem_st8(ts + c / 2, ps);
+          tmem_st8(td + c / 2, ds);
         }
         const int rows = it.ny - j * kN;  // of the tile that goes by
         if (rows < kN) {
           // rows of the next sequence: zero (both tiles, all channels)
           uint8_t* y = sY + (gs % C::kStages) * 2 * C::kYBytes;
-          for (int e = rows * 8 + (tid & 127); e < kN * 8; e += 128) {
+          for (int e = rows * 8 + (tid & 255); e < kN * 8; e += 256) {
 #pragma unroll
             for (int c = 0; c < 2 * C::kChunks; ++c)
               *reinterpret_cast<uint4*>(y + c * C::kYChunk + e * 16) = make_uint4(0, 0, 0, 0);
@@ -508,33 +535,34 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
         ++na;
         tc_fence_after();
       }
-      // KEYS: group 0 stores dV, group 1 dK; else each group every second chunk of dQ
+      // KEYS: warps 0-7 store dV, 8-15 dK, a chunk of 64 channels for each half;
+      // else the first halves store a chunk of dQ each
       const CUtensorMap* map = KEYS && w == 1 ? &p.o1 : &p.o0;
       const Rows& out = KEYS && w == 1 ? p.out1 : p.out0;
       const float f = KEYS && w == 0 ? 1.f : p.scale;
+      const int c = KEYS ? half : (half == 0 ? w : C::kChunks);
       const int wrows = min(32, it.n - 32 * q);
-#pragma unroll 1
-      for (int c = KEYS ? 0 : w; c < C::kChunks; c += KEYS ? 1 : 2) {
-        if (64 * c >= p.D) break;
-        uint32_t o[64];
-        if (total > 0) {
-          const uint32_t src = col_acc + lane_off + (KEYS && w == 1 ? DP : 0) + 64 * c;
-          tc_ld32(src, o);
-          tc_ld32(src + 32, o + 32);
-          tc_wait_ld_regs(o);
-          tc_wait_ld_regs(o + 32);
-        }
+      if (c < C::kChunks && 64 * c < p.D) {
+        const uint32_t src = col_acc + lane_off + (KEYS && w == 1 ? DP : 0) + 64 * c;
         const bool zero = total == 0 || r >= it.live;
         if (lane == 0) bulk_wait_read0();  // the staging buffer is free
         __syncwarp();
         uint8_t* row = stage + lane * 128;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          if (total > 0) {
+            tc_ld32(src + 32 * h, o);
+            tc_wait_ld_regs(o);
+          }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x[8];
+          for (int e = 0; e < 4; ++e) {
+            float x[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = zero ? 0.f : __uint_as_float(o[8 * e + i]) * f;
-          *reinterpret_cast<uint4*>(row + ((e ^ (lane & 7)) << 4)) =
-              make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
+            for (int i = 0; i < 8; ++i) x[i] = zero ? 0.f : __uint_as_float(o[8 * e + i]) * f;
+            *reinterpret_cast<uint4*>(row + (((4 * h + e) ^ (lane & 7)) << 4)) =
+                make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
+          }
         }
         fence_proxy_async();
         __syncwarp();
@@ -571,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
       hi = max(lo, e.x + e.y);
     }
     const int64_t gap = (int64_t)lo + (rows - hi);
-    for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < gap * p.heads; i += (int64_t)gridDim.x * 8) {
+    for (int64_t i = (int64_t)blockIdx.x * 16 + warp; i < gap * p.heads; i += (int64_t)gridDim.x * 16) {
       const int64_t k = i / p.heads;
       const int h = (int)(i - k * p.heads);
       const int64_t row = k < lo ? k : hi + (k - lo);
@@ -588,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }

@@ -76,6 +76,30 @@ __device__ __forceinline__ bool mbar_wait_inline(uint64_t* b, uint32_t parity, v
   return ok;
 }
 
+// A counter in shared memory that one thread raises and others wait for:
+// cheaper to look at than an mbarrier.
+__device__ __forceinline__ void raise_to(uint32_t* c, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(su32(c)), "r"(v) : "memory");
+}
+// Whole warp; false if the wait was given up.
+__device__ __forceinline__ bool wait_raised(uint32_t* c, uint32_t v, volatile int* abort_flag, unsigned where,
+                                            const WaitLimit& limit, unsigned int* status) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    uint32_t now;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(now) : "r"(su32(c)) : "memory");
+    if (__all_sync(0xffffffffu, (int32_t)(now - v) >= 0)) return true;
+    if ((it & 63u) == 0) {
+      if (t0 == 0) t0 = gtimer();
+      const bool late = gtimer() - t0 > limit.ns;
+      if (__any_sync(0xffffffffu, late || *abort_flag)) {
+        if (late) give_up(abort_flag, where, limit, status);
+        return false;
+      }
+    }
+  }
+}
+
 // Named barrier of n threads that tells all of them whether any had `pred`.
 __device__ __forceinline__ bool bar_any(int id, int n, bool pred) {
   uint32_t r;
@@ -205,6 +229,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
