@@ -102,7 +102,7 @@ typedef struct {
   uplift_tok_rows dq, dk, dv; /* backward only: the gradients, written whole: zero for rows of no sequence and keys that
                                  no query sees */
   float* lse;               /* [Hq, T]; forward: written unless NULL; backward: read */
-  float* delta;             /* backward only: workspace of T * Hq floats */
+  float* delta;             /* backward only: workspace of T * Hq + 16 floats */
   const int32_t* cu_q;      /* [B + 1] */
   const int32_t* cu_k;
   const int32_t* used_k;    /* [B] or NULL */

@@ -70,7 +70,7 @@ int prepare(const char* what, const uplift_tok_attention_args* in, bool bwd, Att
     *e.r = rows_of(*e.in, rows, heads, in->D);
     if ((rc = check_rows(what, e.name, *e.r, rows, heads, in->dtype)) != UPLIFT_LA_OK) return rc;
   }
-  if (bwd && in->T > 0 && (in->lse == nullptr || in->delta == nullptr))
+  if (bwd && ((in->T > 0 && in->lse == nullptr) || (in->T + in->S > 0 && in->delta == nullptr)))
     return fail(UPLIFT_LA_ERR_ARG, "%s: null lse or delta", what);
   a->lse = in->lse;
   a->delta = in->delta;

@@ -23,7 +23,7 @@ struct AttnArgs {
   int dtype;
   // backward
   Rows dout, dq, dk, dv;
-  float* delta;  // [Hq][T]
+  float* delta;  // [Hq][T], then 16 words more
 };
 
 // bf16 / fp16 attention on the tensor cores (tok_attn_fwd.cu).

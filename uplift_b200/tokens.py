@@ -413,7 +413,7 @@ def _packed_attention_backward(index, g, q, k, v, out, lse, cu_q, cu_k, used_k, 
         rdq, dq = _new_rows(q)
         rdk, dk = _new_rows(k)
         rdv, dv = _new_rows(v)
-        delta = torch.empty_like(lse)
+        delta = torch.empty(Hq * T + 16, dtype=torch.float32, device=q.device)
         rc = lib.uplift_tok_attention_backward(
             _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *rg, *rdq, *rdk, *rdv, lse.data_ptr(), delta.data_ptr(),
                           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), 0, 0, T, S, cu_q.shape[0] - 1, Hq, Hk, D,
