@@ -98,6 +98,8 @@ typedef struct {
   uplift_tok_rows q;        /* [T, Hq, D] */
   uplift_tok_rows k, v;     /* [S, Hk, D] */
   uplift_tok_rows out;      /* [T, Hq, D] */
+  uplift_tok_rows out_lo;   /* [T, Hq, D] or data = NULL; 16-bit types only: what the rounding of out left (forward: written;
+                               backward: read, for gradients as exact as if out had not been rounded) */
   uplift_tok_rows dout;     /* backward only: gradient of out */
   uplift_tok_rows dq, dk, dv; /* backward only: the gradients, written whole: zero for rows of no sequence and keys that
                                  no query sees */

@@ -13,11 +13,11 @@ def lib():
 
 
 def _attn_args(kw):
-    a = dict(q=16, k=16, v=16, out=16, dout=16, dq=16, dk=16, dv=16, st=(128, 64), lse=16, delta=16, cu=16, ws=0,
+    a = dict(q=16, k=16, v=16, out=16, lo=0, dout=16, dq=16, dk=16, dv=16, st=(128, 64), lse=16, delta=16, cu=16, ws=0,
              ws_bytes=0, B=1, T=40, S=4, Hq=2, Hk=1, D=64, scale=0.125, causal=1, dtype=_native.BF16,
              size=tokens._PA_ARGS.size)
     a.update(kw)
-    rows = [x for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv") for x in (a[n], *a["st"])]
+    rows = [x for n in ("q", "k", "v", "out", "lo", "dout", "dq", "dk", "dv") for x in (a[n], *a["st"])]
     return tokens._PA_ARGS.pack(a["size"], *rows, a["lse"], a["delta"], a["cu"], a["cu"], 0, a["ws"], a["ws_bytes"],
                                 a["T"], a["S"], a["B"], a["Hq"], a["Hk"], a["D"], a["scale"], a["causal"], a["dtype"],
                                 0)
@@ -50,6 +50,7 @@ def _nr(lib, **kw):
     (dict(T=1 << 31), "ERR_SHAPE"), (dict(S=1 << 31), "ERR_SHAPE"), (dict(scale=0.0), "ERR_ARG"),
     (dict(scale=-1.0), "ERR_ARG"), (dict(scale=float("nan")), "ERR_ARG"), (dict(scale=float("inf")), "ERR_ARG"),
     (dict(q=0), "ERR_ARG"), (dict(out=0), "ERR_ARG"), (dict(cu=0), "ERR_ARG"), (dict(q=8), "ERR_LAYOUT"),
+    (dict(lo=8), "ERR_LAYOUT"),
     (dict(st=(132, 64)), "ERR_LAYOUT"), (dict(st=(128, 4)), "ERR_LAYOUT"), (dict(st=(0, 64)), "ERR_LAYOUT"),
     (dict(size=8), "ERR_ARG"),
 ])
@@ -154,8 +155,9 @@ def test_operators_are_traced_under_fake_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
         q, k, v = _qkv(dt=torch.bfloat16)
-        out, lse = torch.ops.uplift_b200.packed_attention(q, k, v, _cu(0, 4), _cu(0, 4), None, True, 0.25)
+        out, lse, lo = torch.ops.uplift_b200.packed_attention(q, k, v, _cu(0, 4), _cu(0, 4), None, True, 0.25)
         assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (2, 4) and lse.dtype == torch.float32
+        assert lo.shape == q.shape and lo.dtype == q.dtype
         a, b = torch.ops.uplift_b200.norm_rotate(q, k, None, None, torch.ones(4, 8), torch.ones(4, 8), None, 1e-6, False)
         assert a.shape == q.shape and b.shape == k.shape
 

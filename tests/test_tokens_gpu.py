@@ -227,6 +227,31 @@ def test_gradients_of_broadcast_outputs():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("lens", [(300, 150, 33), (3, 1, 4)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_gradients_that_cancel(dt, lens):
+    """Two equal keys, the second's value the first's with its halves exchanged, and equal halves in dO: the two
+    products dO . v are the same number, dS is zero, and what is left of dq and dk is the error of rowsum(dO O).
+    Were O taken as rounded, that error would be u |dO . O|; with the rounding's rest it is u u |dO . O|, plus that
+    of the two sums of D products in 32 bits (2^-23 an addition in the matrix unit)."""
+    gen = torch.Generator().manual_seed(23)
+    D, B = 64, len(lens)
+    T, u = sum(lens), torch.finfo(dt).eps / 2
+    q, g = rand(gen, T, 2, D, dt=dt), rand(gen, T, 2, D // 2, dt=dt).repeat(1, 1, 2)
+    k, v = rand(gen, B, 1, D, dt=dt).repeat_interleave(2, 0), rand(gen, B, 1, D, dt=dt)
+    v = torch.stack([v, v.roll(D // 2, -1)], 1).reshape(2 * B, 1, D)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = ops.packed_attention(*leaves, starts(list(lens)), starts([2] * B), causal=False)
+    dq, dk, _ = torch.autograd.grad(out, leaves, g)
+    seq = torch.repeat_interleave(torch.arange(B, device=DEV), torch.tensor(lens, device=DEV))
+    size = (g.abs() * v.view(B, 2, 1, D).abs().mean(1)[seq]).double().sum(-1)  # [T, 2], at least |dO| . |O|
+    err = D ** -0.5 * size * (u * u + 2 * D * 2.0 ** -23)  # of dS, for the two keys together
+    qmax, kmax = q.double().abs(), k.view(B, 2, 1, D)[seq, 0].double().abs()
+    assert (dq.double().abs() <= err[..., None] * kmax * (1 + 4 * u)).all()
+    most = torch.zeros(B, 1, D, dtype=torch.float64, device=DEV).index_add_(0, seq, (err[..., None] * qmax).sum(1, True))
+    assert (dk.double().abs() <= (most * (1 + 4 * u)).repeat_interleave(2, 0)).all()
+
+
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
 def test_results_do_not_change_between_runs(dt, D):
     gen = torch.Generator().manual_seed(12)

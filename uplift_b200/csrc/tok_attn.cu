@@ -63,6 +63,10 @@ int prepare(const char* what, const uplift_tok_attention_args* in, bool bwd, Att
       {"v", &in->v, &a->v, true, true},         {"out", &in->out, &a->out, false, true},
       {"dout", &in->dout, &a->dout, false, bwd}, {"dq", &in->dq, &a->dq, false, bwd},
       {"dk", &in->dk, &a->dk, true, bwd},       {"dv", &in->dv, &a->dv, true, bwd}};
+  if (in->out_lo.data != nullptr && in->dtype != UPLIFT_LA_F32) {
+    a->out_lo = rows_of(in->out_lo, in->T, in->Hq, in->D);
+    if ((rc = check_rows(what, "out_lo", a->out_lo, in->T, in->Hq, in->dtype)) != UPLIFT_LA_OK) return rc;
+  }
   for (const auto& e : all) {
     if (!e.used) continue;
     const int64_t rows = e.keys ? in->S : in->T;

@@ -16,6 +16,7 @@ struct Rows {  // [rows, heads, D], channel stride 1; strides in elements
 
 struct AttnArgs {
   Rows q, k, v, out;  // forward writes out
+  Rows out_lo;        // 16-bit out only: out before its rounding, less out; p null: not wanted, not known
   float* lse;         // [Hq][T] or null
   Packing pk;
   int Hq, Hk, D;

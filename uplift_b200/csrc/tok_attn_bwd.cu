@@ -632,10 +632,12 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   }
 }
 
-// delta = rowsum(dO O): eight lanes per row, 16 bytes each at a time.
+// delta = rowsum(dO O): eight lanes per row, 16 bytes each at a time.  O is
+// taken as out + out_lo: the rounding of out alone would be the largest error
+// of dS in rows that see few keys.
 // Also sets the item counters of the passes that follow to zero.
 template <typename T>
-__global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, float* delta, int* counters, int T_, int Hq, int D) {
+__global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo, float* delta, int* counters, int T_, int Hq, int D) {
   if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const int64_t item = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
   const int l = threadIdx.x & 7;
@@ -653,6 +655,15 @@ __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, float* 
       for (int i = 0; i < 4; ++i) {
         const float2 x = St<T>::unpack(ua[i]), y = St<T>::unpack(ub[i]);
         sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+      }
+      if (lo.p != nullptr) {
+        const uint4 d = *reinterpret_cast<const uint4*>(static_cast<const T*>(lo.p) + t * lo.t + (int64_t)h * lo.h + c);
+        const uint32_t ud[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = St<T>::unpack(ua[i]), y = St<T>::unpack(ud[i]);
+          sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+        }
       }
     }
   }
@@ -697,8 +708,8 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
   int* counters = reinterpret_cast<int*>(a.delta + (int64_t)T * a.Hq);
   const int64_t blocks = std::max<int64_t>(1, ((int64_t)T * a.Hq + 31) / 32);
   if (blocks >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "attention backward: too many rows");
-  if (bf16) delta_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.delta, counters, T, a.Hq, a.D);
-  else delta_kernel<__half><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.delta, counters, T, a.Hq, a.D);
+  if (bf16) delta_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, T, a.Hq, a.D);
+  else delta_kernel<__half><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, T, a.Hq, a.D);
   if ((rc = launched("attention backward")) != UPLIFT_LA_OK) return rc;
   if (T > 0) {
     // queries stay; without keys no box is loaded and the maps stay empty

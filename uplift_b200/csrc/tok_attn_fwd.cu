@@ -103,8 +103,8 @@ struct Item {
 
 struct Params {
   CUtensorMap qmap, kmap, vmap;  // boxes {64, 1, 128, 1}
-  CUtensorMap omap;              // box {64, 1, 32, 1}
-  Rows v, out;
+  CUtensorMap omap, lmap;        // out, out_lo; box {64, 1, 32, 1}
+  Rows v, out, out_lo;           // out_lo.p: null if not wanted
   float* lse;
   Packing pk;
   int Hq, group, D;
@@ -201,7 +201,8 @@ __device__ __forceinline__ float row_max(const float* f) {
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
-template <typename T, int DP>
+// LO: out_lo is written as well (on its own for the registers that it takes).
+template <typename T, int DP, bool LO>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -624,38 +625,50 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         uint8_t* row = stage + lane * 128;
         uint32_t o[32];
         if (tiles > 0) tc_ld32(to + 64 * c + 32 * group, o);
-        if (group == 0 && lane == 0) bulk_wait_read0();  // the staging buffer is free
-        named_bar(pair, 64);
         if (tiles > 0) tc_wait_ld_regs(o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = inv == 0.f ? 0.f : __uint_as_float(o[8 * e + i]) * inv;
-          *reinterpret_cast<uint4*>(row + (((4 * group + e) ^ (lane & 7)) << 4)) =
-              make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
-        }
-        if (fix && tiles > 0) {
-          // add the values taken out of the tiles on the edge of this item
-          const int e0 = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN * kN;
-          add_nonfinite<T>(row, lane, static_cast<const T*>(p.v.p) + (int64_t)it.k0 * p.v.t + (it.h / p.group) * p.v.h + 64 * c,
-                           p.v.t, e0, see, 32 * group, min(32 * group + 32, p.D - 64 * c));
-        }
-        fence_proxy_async();
-        named_bar(pair, 64);
         const int row0 = it.row + first + 32 * q;
-        if (wrows == 32) {
-          if (group == 0 && lane == 0) {
-            tma_store(&p.omap, stage, 64 * c, it.h, row0, 0);
-            bulk_commit();
+        // out, then (for the gradients) what its rounding left
+#pragma unroll 1
+        for (int part = 0; part < (LO ? 2 : 1); ++part) {
+          if (group == 0 && lane == 0) bulk_wait_read0();  // the staging buffer is free
+          named_bar(pair, 64);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float2 x = make_float2(__uint_as_float(o[8 * e + 2 * i]) * inv, __uint_as_float(o[8 * e + 2 * i + 1]) * inv);
+              if (inv == 0.f) x = make_float2(0.f, 0.f);
+              y[i] = St<T>::pack(x.x, x.y);
+              if (LO && part == 1) {
+                const float2 hi = St<T>::unpack(y[i]);
+                y[i] = St<T>::pack(isfinite(hi.x) ? x.x - hi.x : 0.f, isfinite(hi.y) ? x.y - hi.y : 0.f);
+              }
+            }
+            *reinterpret_cast<uint4*>(row + (((4 * group + e) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
           }
-        } else {  // the rows behind the sequence are not ours
-          for (int e = 32 * group + lane; e < wrows * 8; e += 64) {
-            const int rr = e >> 3, piece = e & 7;
-            if (64 * c + 8 * piece < p.D)
-              *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(p.out.p)) + (int64_t)(row0 + rr) * p.out.t +
-                                        (int64_t)it.h * p.out.h + 64 * c + 8 * piece) =
-                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          if (fix && tiles > 0 && part == 0) {
+            // add the values taken out of the tiles on the edge of this item
+            const int e0 = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN * kN;
+            add_nonfinite<T>(row, lane, static_cast<const T*>(p.v.p) + (int64_t)it.k0 * p.v.t + (it.h / p.group) * p.v.h + 64 * c,
+                             p.v.t, e0, see, 32 * group, min(32 * group + 32, p.D - 64 * c));
+          }
+          fence_proxy_async();
+          named_bar(pair, 64);
+          if (wrows == 32) {
+            if (group == 0 && lane == 0) {
+              tma_store(!LO || part == 0 ? &p.omap : &p.lmap, stage, 64 * c, it.h, row0, 0);
+              bulk_commit();
+            }
+          } else {  // the rows behind the sequence are not ours
+            const Rows& out = !LO || part == 0 ? p.out : p.out_lo;
+            for (int e = 32 * group + lane; e < wrows * 8; e += 64) {
+              const int rr = e >> 3, piece = e & 7;
+              if (64 * c + 8 * piece < p.D)
+                *reinterpret_cast<uint4*>(static_cast<T*>(const_cast<void*>(out.p)) + (int64_t)(row0 + rr) * out.t +
+                                          (int64_t)it.h * out.h + 64 * c + 8 * piece) =
+                    *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+            }
           }
         }
       }
@@ -675,6 +688,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int64_t row = k < lo ? k : hi + (k - lo);
       T* o = static_cast<T*>(const_cast<void*>(p.out.p)) + row * p.out.t + (int64_t)h * p.out.h;
       for (int e = lane * 8; e < p.D; e += 256) *reinterpret_cast<uint4*>(o + e) = make_uint4(0, 0, 0, 0);
+      if constexpr (LO) {
+        T* ol = static_cast<T*>(const_cast<void*>(p.out_lo.p)) + row * p.out_lo.t + (int64_t)h * p.out_lo.h;
+        for (int e = lane * 8; e < p.D; e += 256) *reinterpret_cast<uint4*>(ol + e) = make_uint4(0, 0, 0, 0);
+      }
       if (p.lse != nullptr && lane == 0) p.lse[(int64_t)h * p.pk.T + row] = -INFINITY;
     }
     if (lane == 0) bulk_wait_all();
@@ -688,13 +705,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool LO>
 int launch(const Params& p, int dev, int grid, cudaStream_t s) {
   static std::atomic<bool> configured[64] = {};
-  const int rc = opt_in_smem(attention_kernel<T, DP>, Cfg<DP>::kSmem, configured, dev);
+  const int rc = opt_in_smem(attention_kernel<T, DP, LO>, Cfg<DP>::kSmem, configured, dev);
   if (rc != UPLIFT_LA_OK) return rc;
-  attention_kernel<T, DP><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(p);
+  attention_kernel<T, DP, LO><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(p);
   return launched("attention");
+}
+
+template <typename T>
+int launch(const Params& p, int dev, int grid, cudaStream_t s) {
+  if (p.out_lo.p != nullptr) return p.D <= 64 ? launch<T, 64, true>(p, dev, grid, s) : launch<T, 128, true>(p, dev, grid, s);
+  return p.D <= 64 ? launch<T, 64, false>(p, dev, grid, s) : launch<T, 128, false>(p, dev, grid, s);
 }
 
 }  // namespace fwd
@@ -727,9 +750,11 @@ int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
   if (rc == UPLIFT_LA_OK && a.pk.S > 0) rc = make_row_map(&p.kmap, a.dtype, a.k, a.pk.S, a.Hk, a.D, kN);
   if (rc == UPLIFT_LA_OK && a.pk.S > 0) rc = make_row_map(&p.vmap, a.dtype, a.v, a.pk.S, a.Hk, a.D, kN);
   if (rc == UPLIFT_LA_OK) rc = make_row_map(&p.omap, a.dtype, a.out, a.pk.T, a.Hq, a.D, 32);
+  if (rc == UPLIFT_LA_OK && a.out_lo.p != nullptr) rc = make_row_map(&p.lmap, a.dtype, a.out_lo, a.pk.T, a.Hq, a.D, 32);
   if (rc != UPLIFT_LA_OK) return rc;
   p.v = a.v;
   p.out = a.out;
+  p.out_lo = a.out_lo;
   p.lse = a.lse;
   p.pk = a.pk;
   p.Hq = a.Hq;
@@ -742,9 +767,7 @@ int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
   p.host_status = host_status_word();
   const int64_t most = ((int64_t)a.pk.T / (kM + p.row_step) + a.pk.B) * (a.Hq / p.heads);  // items, at most
   const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
-  if (a.dtype == UPLIFT_LA_BF16)
-    return a.D <= 64 ? launch<__nv_bfloat16, 64>(p, dev, grid, s) : launch<__nv_bfloat16, 128>(p, dev, grid, s);
-  return a.D <= 64 ? launch<__half, 64>(p, dev, grid, s) : launch<__half, 128>(p, dev, grid, s);
+  return a.dtype == UPLIFT_LA_BF16 ? launch<__nv_bfloat16>(p, dev, grid, s) : launch<__half>(p, dev, grid, s);
 }
 
 int attn_fwd_device_status(bool clear) { return read_status(g_tok_fwd_status, clear); }

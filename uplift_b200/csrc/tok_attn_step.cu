@@ -48,7 +48,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;    // see tok_attn_fwd.cu
 
 struct Params {
-  Rows q, k, v, out;
+  Rows q, k, v, out, out_lo;  // out_lo.p: null if not wanted
   float* lse;
   float* part_o;   // [T][chunks][Hq][D]
   float2* part_ml; // [T][chunks][Hq]: maximum (of scale S log2 e) and sum
@@ -93,6 +93,19 @@ __device__ __forceinline__ float keys_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 8);
   return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
+// Four channels of a result; out_lo: what the rounding left.
+template <typename T>
+__device__ __forceinline__ void store_out(const Params& p, int64_t row, int h, int c, float4 x) {
+  const uint32_t y[2] = {St<T>::pack(x.x, x.y), St<T>::pack(x.z, x.w)};
+  *reinterpret_cast<uint2*>(static_cast<T*>(const_cast<void*>(p.out.p)) + row * p.out.t + (int64_t)h * p.out.h + c) =
+      make_uint2(y[0], y[1]);
+  if (p.out_lo.p == nullptr) return;
+  const float2 a = St<T>::unpack(y[0]), b = St<T>::unpack(y[1]);
+  *reinterpret_cast<uint2*>(static_cast<T*>(const_cast<void*>(p.out_lo.p)) + row * p.out_lo.t + (int64_t)h * p.out_lo.h + c) =
+      make_uint2(St<T>::pack(isfinite(a.x) ? x.x - a.x : 0.f, isfinite(a.y) ? x.y - a.y : 0.f),
+                 St<T>::pack(isfinite(b.x) ? x.z - b.x : 0.f, isfinite(b.y) ? x.w - b.y : 0.f));
+}
+
 // Loads that are not kept in L1: every byte is used once.
 __device__ __forceinline__ uint4 load16(const void* p) {
   uint4 v;
@@ -326,8 +339,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
       if (last) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         if (sum == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<uint2*>(static_cast<T*>(const_cast<void*>(p.out.p)) + row * p.out.t + (int64_t)h * p.out.h + c) =
-            make_uint2(St<T>::pack(o.x * inv, o.y * inv), St<T>::pack(o.z * inv, o.w * inv));
+        store_out<T>(p, row, h, c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
         if (c == 0 && p.lse != nullptr)
           p.lse[(int64_t)h * p.pk.T + row] = sum == 0.f ? -INFINITY : mm / kLog2e + logf(sum);
       } else {
@@ -412,8 +424,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (sum == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < p.D)
-    *reinterpret_cast<uint2*>(static_cast<T*>(const_cast<void*>(p.out.p)) + row * p.out.t + (int64_t)h * p.out.h + c) =
-        make_uint2(St<T>::pack(o.x * inv, o.y * inv), St<T>::pack(o.z * inv, o.w * inv));
+    store_out<T>(p, row, h, c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   if (lane == 0 && p.lse != nullptr)
     p.lse[(int64_t)h * p.pk.T + row] = sum == 0.f ? -INFINITY : mm / kLog2e + logf(sum);
 }
@@ -463,7 +474,7 @@ int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s) {
   const int rc = sm_count(&dev, &sms);
   if (rc != UPLIFT_LA_OK) return rc;
   Params p = {};
-  p.q = a.q; p.k = a.k; p.v = a.v; p.out = a.out;
+  p.q = a.q; p.k = a.k; p.v = a.v; p.out = a.out; p.out_lo = a.out_lo;
   p.lse = a.lse;
   p.pk = a.pk;
   p.Hq = a.Hq; p.Hk = a.Hk; p.group = a.Hq / a.Hk; p.D = a.D;

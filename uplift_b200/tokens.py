@@ -34,7 +34,7 @@ _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float
 
 # the argument structs of include/uplift_tokens.h (a token tensor: pointer, row stride, head stride)
 _NR_ARGS = struct.Struct("@q" + 6 * "Pqq" + 7 * "P" + "qq" + "iiii" + "f" + "iiiii")
-_PA_ARGS = struct.Struct("@q" + 8 * "Pqq" + 6 * "P" + "qqq" + "iiii" + "f" + "iii")
+_PA_ARGS = struct.Struct("@q" + 9 * "Pqq" + 6 * "P" + "qqq" + "iiii" + "f" + "iii")
 _NO_ROWS = (0, 0, 0)
 
 try:  # without making Stream and device objects: microseconds count in a decoding step
@@ -365,8 +365,9 @@ def _workspace_bytes(B, T, S, Hq, Hk, D, dtype) -> int:
     return _native.load().uplift_tok_attention_workspace(B, T, S, Hq, Hk, D, dtype)
 
 
-def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=None, need_lse=False):
-    """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, None when not needed)."""
+def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=None, need_lse=False, need_lo=False):
+    """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, out_lo: what the rounding of a
+    16-bit out left); lse and out_lo are None when not needed."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
@@ -381,25 +382,26 @@ def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=No
         rk, k = _rows(k)
         rv, v = _rows(v)
         ro, out = _new_rows(q)
+        rl, lo = _new_rows(q) if need_lo and q.dtype is not torch.float32 else (_NO_ROWS, None)
         lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device) if need_lse else None
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.uplift_tok_attention_forward(
-            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, _ptr(lse), 0,
+            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *rl, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, _ptr(lse), 0,
                           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), _ptr(ws), nbytes, T, S, B, Hq, Hk, D,
                           scale, causal, dt, 0), _raw_stream(index))
     if rc:
         _native.check(rc, "uplift_tok_attention_forward")
-    return out, lse
+    return out, lse, lo
 
 
-def packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k=None, causal=True, scale=None):
+def packed_attention_backward_raw(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k=None, causal=True, scale=None):
     """Launch uplift_tok_attention_backward: (dq, dk, dv)."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
-    return _packed_attention_backward(index, g.to(q.dtype), q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale)
+    return _packed_attention_backward(index, g.to(q.dtype), q, k, v, out, lse, lo, cu_q, cu_k, used_k, causal, scale)
 
 
-def _packed_attention_backward(index, g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale):
+def _packed_attention_backward(index, g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, causal, scale):
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
     lib = _native.load()
     _native.host_status.raise_if_set()
@@ -410,12 +412,13 @@ def _packed_attention_backward(index, g, q, k, v, out, lse, cu_q, cu_k, used_k, 
         rk, k = _rows(k)
         rv, v = _rows(v)
         ro, out = _rows(out)
+        rl, lo = _rows(lo) if lo is not None else (_NO_ROWS, None)
         rdq, dq = _new_rows(q)
         rdk, dk = _new_rows(k)
         rdv, dv = _new_rows(v)
         delta = torch.empty(Hq * T + 16, dtype=torch.float32, device=q.device)
         rc = lib.uplift_tok_attention_backward(
-            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *rg, *rdq, *rdk, *rdv, lse.data_ptr(), delta.data_ptr(),
+            _PA_ARGS.pack(_PA_ARGS.size, *rq, *rk, *rv, *ro, *rl, *rg, *rdq, *rdk, *rdv, lse.data_ptr(), delta.data_ptr(),
                           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(used_k), 0, 0, T, S, cu_q.shape[0] - 1, Hq, Hk, D,
                           scale, causal, _DTYPES[q.dtype], 0), _raw_stream(index))
     if rc:
@@ -426,8 +429,8 @@ def _packed_attention_backward(index, g, q, k, v, out, lse, cu_q, cu_k, used_k, 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, used_k, causal, scale):
-        out, lse = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, used_k)
+        out, lse, lo = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True, need_lo=True)
+        ctx.save_for_backward(q, k, v, out, lse, lo, cu_q, cu_k, used_k)
         ctx.causal, ctx.scale = causal, scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -438,8 +441,8 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 8
-        q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
-        grads = _packed_attention_backward(q.get_device(), g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal,
+        q, k, v, out, lse, lo, cu_q, cu_k, used_k = ctx.saved_tensors
+        grads = _packed_attention_backward(q.get_device(), g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, ctx.causal,
                                            ctx.scale)
         return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
 
@@ -447,38 +450,41 @@ class _PackedAttention(torch.autograd.Function):
 @torch.library.custom_op("uplift_b200::packed_attention", mutates_args=())
 def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
                          used_k: Optional[torch.Tensor], causal: bool,
-                         scale: float) -> tuple[torch.Tensor, torch.Tensor]:
-    return packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True)
+                         scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out, lse, lo = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True, need_lo=True)
+    return out, lse, lo if lo is not None else out.new_empty(0)
 
 
 @_packed_attention_op.register_fake
 def _(q, k, v, cu_q, cu_k, used_k, causal, scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+    return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32),
+            q.new_empty(0 if q.dtype is torch.float32 else q.shape))
 
 
 @torch.library.custom_op("uplift_b200::packed_attention_backward", mutates_args=())
 def _packed_attention_backward_op(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                                  out: torch.Tensor, lse: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
-                                  used_k: Optional[torch.Tensor], causal: bool,
+                                  out: torch.Tensor, lse: torch.Tensor, lo: torch.Tensor, cu_q: torch.Tensor,
+                                  cu_k: torch.Tensor, used_k: Optional[torch.Tensor], causal: bool,
                                   scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return packed_attention_backward_raw(g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale)
+    return packed_attention_backward_raw(g, q, k, v, out, lse, lo if lo.dim() == 3 else None, cu_q, cu_k, used_k,
+                                         causal, scale)
 
 
 @_packed_attention_backward_op.register_fake
-def _(g, q, k, v, out, lse, cu_q, cu_k, used_k, causal, scale):
+def _(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, causal, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 def _pa_setup_context(ctx, inputs, output):
     q, k, v, cu_q, cu_k, used_k, causal, scale = inputs
-    out, lse = output
-    ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, used_k)
+    out, lse, lo = output
+    ctx.save_for_backward(q, k, v, out, lse, lo, cu_q, cu_k, used_k)
     ctx.causal, ctx.scale = causal, scale
 
 
-def _pa_backward(ctx, g, _):
-    q, k, v, out, lse, cu_q, cu_k, used_k = ctx.saved_tensors
-    grads = torch.ops.uplift_b200.packed_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, used_k, ctx.causal,
+def _pa_backward(ctx, g, _lse, _lo):
+    q, k, v, out, lse, lo, cu_q, cu_k, used_k = ctx.saved_tensors
+    grads = torch.ops.uplift_b200.packed_attention_backward(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, ctx.causal,
                                                             ctx.scale)
     return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
 
@@ -509,10 +515,10 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
         cu_k = cu_q
     scale, causal = (float(scale) if scale is not None else q.shape[-1] ** -0.5), bool(causal)
     if torch.compiler.is_compiling():
-        out, lse = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale)
+        out, lse, _ = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale)
         lse = lse.detach()
     elif torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, used_k, causal, scale)
     else:
-        out, lse = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=return_lse)
+        out, lse, _ = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=return_lse)
     return (out, lse) if return_lse else out
