@@ -63,6 +63,8 @@ def test_attention_entry_refuses(lib, kw, code):
     (dict(dtype=-1), "ERR_ARG"), (dict(lse=0), "ERR_ARG"), (dict(delta=0), "ERR_ARG"),
     (dict(dout=0), "ERR_ARG"), (dict(out=0), "ERR_ARG"), (dict(v=24), "ERR_LAYOUT"),
     (dict(D=129), "ERR_SHAPE"), (dict(Hq=5, Hk=2), "ERR_SHAPE"), (dict(cu=0), "ERR_ARG"),
+    # more items than a 32-bit counter holds: one per sequence, 128 rows and head
+    (dict(B=1 << 26, T=1 << 26, Hq=32, Hk=1), "ERR_SHAPE"), (dict(B=1 << 26, S=1 << 26, Hq=32, Hk=32), "ERR_SHAPE"),
 ])
 def test_attention_backward_entry_refuses(lib, kw, code):
     assert _attn_bwd(lib, **kw) == getattr(_native, code)
@@ -155,7 +157,7 @@ def test_operators_are_traced_under_fake_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
         q, k, v = _qkv(dt=torch.bfloat16)
-        out, lse, lo = torch.ops.uplift_b200.packed_attention(q, k, v, _cu(0, 4), _cu(0, 4), None, True, 0.25)
+        out, lse, lo = torch.ops.uplift_b200.packed_attention(q, k, v, _cu(0, 4), _cu(0, 4), None, True, 0.25, True, True)
         assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (2, 4) and lse.dtype == torch.float32
         assert lo.shape == q.shape and lo.dtype == q.dtype
         a, b = torch.ops.uplift_b200.norm_rotate(q, k, None, None, torch.ones(4, 8), torch.ones(4, 8), None, 1e-6, False)

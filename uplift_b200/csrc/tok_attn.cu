@@ -5,6 +5,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "tok_attn.h"
 
 namespace ula {
@@ -76,6 +78,11 @@ int prepare(const char* what, const uplift_tok_attention_args* in, bool bwd, Att
   }
   if (bwd && ((in->T > 0 && in->lse == nullptr) || (in->T + in->S > 0 && in->delta == nullptr)))
     return fail(UPLIFT_LA_ERR_ARG, "%s: null lse or delta", what);
+  // the items of a pass of the gradients are counted in 32 bits
+  auto items = [&](int64_t rows, int heads) { return (rows / 128 + std::min<int64_t>(rows, in->B)) * heads; };
+  if (bwd && in->dtype != UPLIFT_LA_F32 && std::max(items(in->T, in->Hq), items(in->S, in->Hk)) >= (1ll << 31) - 65536)
+    return fail(UPLIFT_LA_ERR_SHAPE, "%s: too many sequences: B=%d T=%lld S=%lld Hq=%d Hk=%d", what, in->B,
+                (long long)in->T, (long long)in->S, in->Hq, in->Hk);
   a->lse = in->lse;
   a->delta = in->delta;
   a->pk = Packing{in->cu_q, in->cu_k, in->used_k, in->B, (int)in->T, (int)in->S, in->causal != 0};

@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           it.h = (int)(i - tile * per_tile) * p.heads;
           it.k0 = s.k0;
           it.nk = s.nk;
-          it.see = p.pk.causal ? i0 + 1 + s.nk - s.nq : s.nk;
+          it.see = p.pk.causal ? i0 + 1 - s.nq + s.nk : s.nk;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int last = min(it.n, t * p.row_step + kM) - 1;  // last row of the tile

@@ -56,14 +56,35 @@ struct Params {
   int Hq, Hk, group, D;
   int row_tiles;   // ceil(group / 8)
   int chunks;      // at most, per token
-  int min_len;     // least keys of a chunk
+  float share;     // of the pairs of one head, that an item takes to fill the SMs once; 0: items of kManyKeys
   float scale;
 };
 
-// Keys of a chunk of a sequence, a multiple of kMinChunk.
-__device__ __forceinline__ int chunk_len(const Params& p, int nk) {
-  const int even = (nk + p.chunks - 1) / p.chunks;
-  return max(p.min_len, (even + kMinChunk - 1) / kMinChunk * kMinChunk);
+// Query-key pairs of a small batch (whole warp); 0 for a large one.
+__device__ __forceinline__ float pairs_of(const Params& p) {
+  if (p.pk.B > 32 || p.share == 0.f) return 0.f;
+  float n = 0.f;
+  if ((int)(threadIdx.x & 31) < p.pk.B) {
+    const Seq s = sequence(p.pk, threadIdx.x & 31);
+    n = (float)s.nq * (float)s.nk;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+
+// Keys of a chunk of a sequence, a multiple of kMinChunk.  The items of a
+// small problem fill the SMs once, those of a large one (half as many tokens
+// times key heads as CTAs) have 1024 keys: the join costs 2 % of the reads
+// (512: 8 % slower).  What counts are the keys there are, not the cache's
+// room (4 tokens with 1000 keys each, 32 on 8 heads of 128, in room for 32768:
+// 14.4 us, by the room 26.8; in room for 1000: 13.0 and 12.4).  Batches of
+// more than 32 sequences are taken to be like the one at hand.
+__device__ __forceinline__ int chunk_len(const Params& p, float pairs, int nk) {
+  if (p.pk.B > 32) pairs = (float)p.pk.T * (float)nk;
+  const int fill = p.share == 0.f ? kManyKeys : (int)fminf((float)kManyKeys, pairs * p.share);
+  const int even = (nk + p.chunks - 1) / p.chunks;  // the workspace holds that many
+  return (max(max(fill, even), 1) + kMinChunk - 1) / kMinChunk * kMinChunk;
 }
 
 template <typename T> struct Mma;
@@ -131,8 +152,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 
 // Units of a sequence: one per query token and chunk of its keys.
 struct UnitWalk {
+  float pairs;
   int b0 = 0;
   int64_t before = 0;
+  __device__ __forceinline__ explicit UnitWalk(const Params& p) : pairs(pairs_of(p)) {}
   __device__ __forceinline__ bool find(const Params& p, int64_t unit, Seq* s, int* len, int* local) {
     const int lane = threadIdx.x & 31;
     while (b0 < p.pk.B) {
@@ -141,7 +164,7 @@ struct UnitWalk {
       int64_t n = 0;
       if (b0 + lane < p.pk.B) {
         mine = sequence(p.pk, b0 + lane);
-        l = chunk_len(p, mine.nk);
+        l = chunk_len(p, pairs, mine.nk);
         n = (int64_t)mine.nq * ((mine.nk + l - 1) / l);
       }
       int64_t sum = n;
@@ -180,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const float c2 = p.scale * kLog2e;
-  UnitWalk walk;
+  UnitWalk walk(p);
   const int per_unit = p.Hk * p.row_tiles;
   for (int64_t i = blockIdx.x;; i += gridDim.x) {
     Seq s;
@@ -374,10 +397,11 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const bool live = item < (int64_t)p.pk.T * p.Hq;
   const int64_t row = live ? item / p.Hq : 0;
   const int h = (int)(item - row * p.Hq);
+  const float pairs = pairs_of(p);
   if (live && p.pk.B > 0) {
     const Seq s = sequence(p.pk, sequence_of(p.pk.cu_q, p.pk.B, (int)row));
     if (row >= s.q0 && row < s.q0 + s.nq) {
-      const int see = keys_seen(s, (int)row - s.q0, p.pk.causal), len = chunk_len(p, s.nk);
+      const int see = keys_seen(s, (int)row - s.q0, p.pk.causal), len = chunk_len(p, pairs, s.nk);
       chunks = (see + len - 1) / len;
     }
   }
@@ -483,11 +507,8 @@ int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s) {
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)a.pk.T * p.chunks * a.Hq * a.D);
   p.scale = a.scale;
-  // Keys per item: the items of a small problem fill the SMs once, those of a
-  // large one have 1024 keys (the join costs 2 % of the reads; 512: 8 % slower).
-  const int64_t pairs = a.pk.B > 0 ? (int64_t)a.pk.T * a.pk.S / a.pk.B * a.Hk * p.row_tiles : 0;
-  const int64_t len = pairs / ((int64_t)sms * kCtasPerSm);
-  p.min_len = (int)std::min<int64_t>(kManyKeys, std::max<int64_t>(kMinChunk, (len + kMinChunk - 1) / kMinChunk * kMinChunk));
+  const int64_t units = (int64_t)a.pk.T * a.Hk * p.row_tiles, slots = (int64_t)sms * kCtasPerSm;
+  p.share = 2 * units >= slots ? 0.f : (float)(a.Hk * p.row_tiles) / (float)slots;
   if (a.dtype == UPLIFT_LA_BF16)
     return a.D <= 64 ? run<__nv_bfloat16, 64>(p, sms, s) : run<__nv_bfloat16, 128>(p, sms, s);
   return a.D <= 64 ? run<__half, 64>(p, sms, s) : run<__half, 128>(p, sms, s);

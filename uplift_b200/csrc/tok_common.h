@@ -73,7 +73,7 @@ __device__ __forceinline__ Seq sequence(const Packing& p, int b) {
 
 // Number of keys that query i of the sequence sees.
 __device__ __forceinline__ int keys_seen(const Seq& s, int i, int causal) {
-  return causal ? max(0, min(s.nk, i + 1 + s.nk - s.nq)) : s.nk;
+  return causal ? max(0, min(s.nk, i + 1 - s.nq + s.nk)) : s.nk;
 }
 
 // Dynamic shared memory above 48 KB is an opt-in per function and device;

@@ -16,7 +16,10 @@ float16; views into a fused projection output are read in place.  Both are
 differentiable (gradients are deterministic) and registered as torch custom
 ops, so torch.compile traces them.  Launches go to the current stream of the
 tensors' device; workspaces come from torch's allocator, so calls on several
-streams and in captured graphs share nothing.
+streams and in captured graphs share nothing.  As with every differentiable
+call, capture a backward pass into a CUDA graph only when no result of an
+eager call on the same leaves is alive: their gradients would be summed on the
+stream of that call, which is not being captured.
 """
 from __future__ import annotations
 
@@ -318,7 +321,7 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
     position leaves the token unrotated (class tokens); one beyond the table
     makes its rotated channels NaN.  Pairs are (i, i + R/2), or (2i, 2i + 1)
     when interleaved.  Arithmetic in fp32, one rounding per result.
-    Differentiable in q, k and the weights; the tables are constants.
+    Differentiable in q, k and the weights (once); the tables are constants.
     """
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("norm_rotate: cos and sin are constants and must not require gradients")
@@ -449,16 +452,17 @@ class _PackedAttention(torch.autograd.Function):
 
 @torch.library.custom_op("uplift_b200::packed_attention", mutates_args=())
 def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
-                         used_k: Optional[torch.Tensor], causal: bool,
-                         scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    out, lse, lo = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=True, need_lo=True)
-    return out, lse, lo if lo is not None else out.new_empty(0)
+                         used_k: Optional[torch.Tensor], causal: bool, scale: float, need_lse: bool,
+                         need_lo: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out, lse, lo = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse, need_lo)
+    return (out, lse if lse is not None else out.new_empty(0, dtype=torch.float32),
+            lo if lo is not None else out.new_empty(0))
 
 
 @_packed_attention_op.register_fake
-def _(q, k, v, cu_q, cu_k, used_k, causal, scale):
-    return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32),
-            q.new_empty(0 if q.dtype is torch.float32 else q.shape))
+def _(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse, need_lo):
+    return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]) if need_lse else 0, dtype=torch.float32),
+            q.new_empty(q.shape if need_lo and q.dtype is not torch.float32 else 0))
 
 
 @torch.library.custom_op("uplift_b200::packed_attention_backward", mutates_args=())
@@ -476,7 +480,7 @@ def _(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, causal, scale):
 
 
 def _pa_setup_context(ctx, inputs, output):
-    q, k, v, cu_q, cu_k, used_k, causal, scale = inputs
+    q, k, v, cu_q, cu_k, used_k, causal, scale, _, _ = inputs
     out, lse, lo = output
     ctx.save_for_backward(q, k, v, out, lse, lo, cu_q, cu_k, used_k)
     ctx.causal, ctx.scale = causal, scale
@@ -486,7 +490,7 @@ def _pa_backward(ctx, g, _lse, _lo):
     q, k, v, out, lse, lo, cu_q, cu_k, used_k = ctx.saved_tensors
     grads = torch.ops.uplift_b200.packed_attention_backward(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k, ctx.causal,
                                                             ctx.scale)
-    return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+    return (*(d if n else None for d, n in zip(grads, ctx.needs_input_grad)), *(None,) * 7)
 
 
 torch.library.register_autograd("uplift_b200::packed_attention", _pa_backward, setup_context=_pa_setup_context)
@@ -507,17 +511,19 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
     get zeros (lse -inf) and gradients zero.
 
     With return_lse also returns log(sum_j exp(scale q_i . k_j)), fp32
-    [Hq, T], a constant for autograd.  Differentiable in q, k, v.
+    [Hq, T], a constant for autograd.  Differentiable in q, k, v (once).
     """
     if cu_k is None:
         if q.shape[0] != k.shape[0]:
             raise ValueError(f"packed_attention: q has {q.shape[0]} rows and k has {k.shape[0]}: pass cu_k")
         cu_k = cu_q
     scale, causal = (float(scale) if scale is not None else q.shape[-1] ** -0.5), bool(causal)
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if torch.compiler.is_compiling():
-        out, lse, _ = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale)
+        out, lse, _ = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale,
+                                                             train or return_lse, train)
         lse = lse.detach()
-    elif torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    elif train:
         out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, used_k, causal, scale)
     else:
         out, lse, _ = packed_attention_raw(q, k, v, cu_q, cu_k, used_k, causal, scale, need_lse=return_lse)
