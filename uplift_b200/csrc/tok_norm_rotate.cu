@@ -557,7 +557,10 @@ int run(Args a, int dtype, bool inter, bool bwd, int* partial_rows, cudaStream_t
   while (lanes * V < a.D) lanes *= 2;
   // Heads per group: several amortise the token's angles and the weights and
   // keep more loads in flight; one where several would leave SMs without work.
-  const int hpg = vec && rows * lanes >= 4ll * 148 * 2048 ? (bwd ? kManyHeadsBwd : kManyHeads) : 1;
+  // 32 + 8 heads of 128 in bf16, forward and backward, several / one (us): 128
+  // tokens 3.2 / 2.5 and 3.7 / 4.1, 512: 4.8 / 4.9 and 6.7 / 7.2, 1024: 6.3 / 8.1
+  // and 9.1 / 11.4, 8192: 28 / 50 and 54 / 89.
+  const int hpg = vec && rows * lanes >= 148ll * 2048 ? (bwd ? kManyHeadsBwd : kManyHeads) : 1;
   for (int i = 0; i < 2; ++i) a.side[i].chunks = (a.side[i].heads + hpg - 1) / hpg;
   if (bwd) {
     // vec: tokens over x, chunks of heads over y; else rows over x, sides over y
