@@ -62,7 +62,7 @@ HEADS = {"mha": (3, 3), "group": (4, 2), "one key head": (5, 1)}
 @pytest.mark.parametrize("pack", PACKS)
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dt,D", [(BF16, 64), (BF16, 128), (F16, 64), (F16, 128), (BF16, 8), (BF16, 80), (F16, 104),
-                                  (F32, 64), (F32, 33)])
+                                  (F32, 64), (F32, 33), (F32, 128), (F32, 100)])
 def test_attention_packs(pack, causal, dt, D):
     gen = torch.Generator().manual_seed(hash((len(pack), causal, D)) & 0xffff)
     n_q, n_k = zip(*PACKS[pack])
@@ -99,16 +99,38 @@ def test_a_few_tokens_on_long_histories(causal):
     run_attention(q, k, v, starts(n_q), starts(n_k), None, causal, gen=gen)
 
 
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_in_segments_with_room(dt, D, causal):
+    """Rows of a key segment behind used_k, NaN here, reach nothing, and their gradients are zero."""
+    gen = torch.Generator().manual_seed(31)
+    n_q, n_k, seg = [40, 70, 3], [55, 130, 0], [64, 150, 9]
+    q, k, v = qkv(gen, sum(n_q), sum(seg), 4, 2, D, dt)
+    used = torch.tensor(n_k, dtype=torch.int32, device=DEV)
+    room = torch.cat([torch.arange(s, device=DEV) >= n for s, n in zip(seg, n_k)])
+    g = rand(gen, *q.shape, dt=dt)
+    ref = R.attention(q, k, v, starts(n_q), starts(seg), used, causal, None, g, dt)
+    k[room], v[room] = math.nan, math.inf
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.packed_attention(*leaves, starts(n_q), starts(seg), used_k=used, causal=causal)
+    R.check(out, ref["out"], ref["out_tol"], "out")
+    for n, d in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, g)):
+        R.check(d, ref[n], ref[n + "_tol"], n)
+        if n != "dq":
+            assert not d[room].any()
+
+
 def test_one_token_on_a_very_long_history():
     gen = torch.Generator().manual_seed(4)
     q, k, v = qkv(gen, 1, 70001, 4, 1, 128, BF16)
     run_attention(q, k, v, starts([1]), starts([70001]), None, True, grads=False, gen=gen)
 
 
-def test_many_sequences():
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_many_sequences(dt):
     gen = torch.Generator().manual_seed(5)
     n = [(i * 7) % 23 for i in range(700)]
-    q, k, v = qkv(gen, sum(n), sum(n), 2, 2, 64, BF16)
+    q, k, v = qkv(gen, sum(n), sum(n), 2, 2, 64, dt)
     run_attention(q, k, v, starts(n), starts(n), None, True, gen=gen)
 
 
