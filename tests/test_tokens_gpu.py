@@ -120,6 +120,36 @@ def test_gradients_in_segments_with_room(dt, D, causal):
             assert not d[room].any()
 
 
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (BF16, 40)])
+@pytest.mark.parametrize("Hq,Hk", [(3, 3), (8, 2), (6, 2), (10, 1), (24, 2)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_few_tokens_per_sequence(dt, D, Hq, Hk, causal):
+    """Rows of several tokens in one tile, tiles that end inside a token, edges inside the last keys."""
+    gen = torch.Generator().manual_seed(33)
+    n_q, n_k = [3, 1, 2, 0, 3, 1, 2, 3, 2], [300, 0, 2, 5, 1, 1025, 64, 65, 63]
+    q, k, v = qkv(gen, sum(n_q), sum(n_k), Hq, Hk, D, dt)
+    run_attention(q, k, v, starts(n_q), starts(n_k), None, causal, gen=gen)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_later_tokens_do_not_reach_earlier_ones_of_a_step(dt, D, at):
+    gen = torch.Generator().manual_seed(35)
+    q, k, v = qkv(gen, 6, 205, 4, 2, D, dt)
+    cu, cu_k = starts([3, 3]), starts([102, 103])
+    clean = ops.packed_attention(q, k, v, cu, cu_k)
+    k, v = k.clone(), v.clone()
+    for end in (102, 205):
+        v[end - 3 + at:end, 0, 3] = math.inf
+        v[end - 3 + at, 1, 5] = math.nan
+    out = ops.packed_attention(q, k, v, cu, cu_k)
+    for b in range(2):
+        assert torch.equal(out[3 * b:3 * b + at], clean[3 * b:3 * b + at])
+        seen = out[3 * b + at:3 * b + 3]
+        assert not bool(seen[:, :2, 3].isfinite().any()) and bool(seen[:, 2:, 5].isnan().all())
+        assert bool(seen[:, :, 6].isfinite().all())
+
+
 def test_one_token_on_a_very_long_history():
     gen = torch.Generator().manual_seed(4)
     q, k, v = qkv(gen, 1, 70001, 4, 1, 128, BF16)

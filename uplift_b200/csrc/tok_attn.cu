@@ -104,7 +104,7 @@ extern "C" {
 
 int64_t uplift_tok_attention_workspace(int B, int64_t T, int64_t S, int Hq, int Hk, int D, int dtype) {
   using namespace ula::tok;
-  if (T < 1 || Hk < 1 || Hq < Hk || D < 1 || !attn_step_applies(B, T, dtype)) return 0;
+  if (T < 1 || Hk < 1 || Hq < Hk || D < 1 || !attn_step_applies(B, T, Hq / Hk, dtype)) return 0;
   return attn_step_workspace(T, Hq, Hk, D);
 }
 
@@ -117,7 +117,7 @@ int uplift_tok_attention_forward(const uplift_tok_attention_args* args, void* st
   if (rc != UPLIFT_LA_OK || args->T == 0) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.dtype == UPLIFT_LA_F32) return attn_simt_forward(a, s);
-  if (!attn_step_applies(a.pk.B, a.pk.T, a.dtype)) return attn_tc_forward(a, s);
+  if (!attn_step_applies(a.pk.B, a.pk.T, a.Hq / a.Hk, a.dtype)) return attn_tc_forward(a, s);
   const int64_t need = attn_step_workspace(a.pk.T, a.Hq, a.Hk, a.D);
   if (args->workspace == nullptr || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15u) != 0)
     return fail(UPLIFT_LA_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);

@@ -35,7 +35,7 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s);
 int attn_bwd_device_status(bool clear);
 
 // The form for a few queries per sequence (tok_attn_step.cu).
-bool attn_step_applies(int B, int64_t T, int dtype);
+bool attn_step_applies(int B, int64_t T, int group, int dtype);
 int64_t attn_step_workspace(int64_t T, int Hq, int Hk, int D);  // bytes
 int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s);
 

@@ -3,9 +3,11 @@
 //
 // Each key and value is read once and meets only the Hq / Hk queries of its
 // group, so HBM bounds it: the kernel is built to keep loads in flight with
-// few instructions.  The keys of a query token are cut into chunks; an item
-// is one chunk for one token and (up to) eight query heads of a group, which
-// are the N of mma.m16n8k16 (fewer are padded, more make further items).  The
+// few instructions.  The keys of a sequence are cut into chunks; an item is
+// one chunk for (up to) eight query rows -- the heads of a group, token after
+// token -- which are the N of mma.m16n8k16 (fewer are padded, more make
+// further items, so several tokens read the keys once as long as they and
+// their heads are eight).  The
 // CTA's four warps take 16 keys in turn, each with its own running maximum
 // and sum, and everything is transposed, so that the few heads are the short
 // side of the products:
@@ -29,6 +31,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "tok_attn_tc.h"
 
@@ -39,7 +42,7 @@ namespace step {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;          // keys of a warp at a time
-constexpr int kRows = 8;           // query heads of an item
+constexpr int kRows = 8;           // query rows of an item
 constexpr int kMinChunk = kWarps * kKeys;
 constexpr int kMaxChunks = 128;    // of one token
 constexpr int kCtasPerSm = 3;      // 168 registers a thread; with 4 (128) or 2 the large steps are 1.5 and 1.2 times slower
@@ -54,19 +57,21 @@ struct Params {
   float2* part_ml; // [T][chunks][Hq]: maximum (of scale S log2 e) and sum
   Packing pk;
   int Hq, Hk, group, D;
-  int row_tiles;   // ceil(group / 8)
+  float units;     // row tiles of a key head over all sequences, about
   int chunks;      // at most, per token
   float share;     // of the pairs of one head, that an item takes to fill the SMs once; 0: items of kManyKeys
   float scale;
 };
 
-// Query-key pairs of a small batch (whole warp); 0 for a large one.
+__device__ __forceinline__ int row_tiles(const Params& p, int nq) { return (nq * p.group + kRows - 1) / kRows; }
+
+// Row tiles times keys of a small batch (whole warp); 0 for a large one.
 __device__ __forceinline__ float pairs_of(const Params& p) {
   if (p.pk.B > 32 || p.share == 0.f) return 0.f;
   float n = 0.f;
   if ((int)(threadIdx.x & 31) < p.pk.B) {
     const Seq s = sequence(p.pk, threadIdx.x & 31);
-    n = (float)s.nq * (float)s.nk;
+    n = (float)row_tiles(p, s.nq) * (float)s.nk;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
@@ -81,7 +86,7 @@ __device__ __forceinline__ float pairs_of(const Params& p) {
 // 14.4 us, by the room 26.8; in room for 1000: 13.0 and 12.4).  Batches of
 // more than 32 sequences are taken to be like the one at hand.
 __device__ __forceinline__ int chunk_len(const Params& p, float pairs, int nk) {
-  if (p.pk.B > 32) pairs = (float)p.pk.T * (float)nk;
+  if (p.pk.B > 32) pairs = p.units * (float)nk;
   const int fill = p.share == 0.f ? kManyKeys : (int)fminf((float)kManyKeys, pairs * p.share);
   const int even = (nk + p.chunks - 1) / p.chunks;  // the workspace holds that many
   return (max(max(fill, even), 1) + kMinChunk - 1) / kMinChunk * kMinChunk;
@@ -150,7 +155,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return d;
 }
 
-// Units of a sequence: one per query token and chunk of its keys.
+// Units of a sequence: one per row tile and chunk of its keys.
 struct UnitWalk {
   float pairs;
   int b0 = 0;
@@ -165,7 +170,7 @@ struct UnitWalk {
       if (b0 + lane < p.pk.B) {
         mine = sequence(p.pk, b0 + lane);
         l = chunk_len(p, pairs, mine.nk);
-        n = (int64_t)mine.nq * ((mine.nk + l - 1) / l);
+        n = (int64_t)row_tiles(p, mine.nq) * ((mine.nk + l - 1) / l);
       }
       int64_t sum = n;
 #pragma unroll
@@ -204,27 +209,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
   const int g = lane >> 2, t = lane & 3;
   const float c2 = p.scale * kLog2e;
   UnitWalk walk(p);
-  const int per_unit = p.Hk * p.row_tiles;
   for (int64_t i = blockIdx.x;; i += gridDim.x) {
     Seq s;
     int len, local;
-    const int64_t unit = i / per_unit;
+    const int64_t unit = i / p.Hk;
     if (!walk.find(p, unit, &s, &len, &local)) break;
-    const int sub = (int)(i - unit * per_unit);
-    const int hk = sub / p.row_tiles, h0 = hk * p.group + (sub - hk * p.row_tiles) * kRows;
-    const int rows = min(kRows, (hk + 1) * p.group - h0);
+    const int hk = (int)(i - unit * p.Hk);
     const int chunks = (s.nk + len - 1) / len;
-    const int tok = local / chunks, chunk = local - tok * chunks;
-    const int see = keys_seen(s, tok, p.pk.causal);
-    const int j0 = chunk * len, j1 = min(see, j0 + len);
-    if (j0 >= j1) continue;  // this token sees none of the chunk (the whole CTA skips it)
-    const int64_t row = s.q0 + tok;
-    // Q^T: head g, 8 channels of each block of 32
+    const int tile = local / chunks, chunk = local - tile * chunks;
+    // rows f0 .. of the nq x group of the sequence: token f / group, head f % group
+    const int f0 = tile * kRows, rows = min(kRows, s.nq * p.group - f0);
+    auto token = [&](int r) { return (f0 + min(r, rows - 1)) / p.group; };
+    auto head = [&](int r) { return hk * p.group + (f0 + r) % p.group; };
+    const int first_tok = token(0), last_tok = token(rows - 1);
+    const int j0 = chunk * len, j1 = min(keys_seen(s, last_tok, p.pk.causal), j0 + len);
+    if (j0 >= j1) continue;  // these rows see none of the chunk (the whole CTA skips it)
+    // keys that all of the rows see, and those of rows 2t, 2t + 1
+    const int every = min(keys_seen(s, first_tok, p.pk.causal), j1);
+    const int lim[2] = {min(keys_seen(s, token(2 * t), p.pk.causal), j1), min(keys_seen(s, token(2 * t + 1), p.pk.causal), j1)};
+    const int gtok = token(g);
+    // Q^T: row g, 8 channels of each block of 32
     uint32_t qb[KB][4];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
       const int c = 32 * b + 8 * t;
-      const uint4 v = load16_if(static_cast<const T*>(p.q.p) + row * p.q.t + (int64_t)(h0 + g) * p.q.h + c, g < rows && c < p.D);
+      const uint4 v = load16_if(static_cast<const T*>(p.q.p) + (int64_t)(s.q0 + gtok) * p.q.t + (int64_t)head(g) * p.q.h + c, g < rows && c < p.D);
       qb[b][0] = v.x; qb[b][1] = v.y; qb[b][2] = v.z; qb[b][3] = v.w;
     }
     // keys j + g, j + 8 + g of K, and j + 2t, + 2t + 1, + 2t + 8, + 2t + 9 of V
@@ -260,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
       }
       vp += v_step;
     };
-    float acc[VB][4][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2t, 2t + 1
+    float acc[VB][4][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows 2t, 2t + 1
 #pragma unroll
     for (int b = 0; b < VB; ++b) {
 #pragma unroll
@@ -270,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
 #pragma unroll 1
     for (; j < j1; j += kMinChunk) {
       load_v(j);
-      float sc[4] = {0.f, 0.f, 0.f, 0.f};  // key g: heads 2t, 2t + 1; key g + 8: the same
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};  // key g: rows 2t, 2t + 1; key g + 8: the same
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
         const uint32_t a0[4] = {kr[b][0].x, kr[b][1].x, kr[b][0].y, kr[b][1].y};
@@ -279,9 +288,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
         Mma<T>::run(sc, a1, qb[b][2], qb[b][3]);
       }
       if (j + kMinChunk < j1) load_k(j + kMinChunk);
-      if (j + kKeys > j1) {
-        if (j + g >= j1) sc[0] = sc[1] = -INFINITY;
-        if (j + g + 8 >= j1) sc[2] = sc[3] = -INFINITY;
+      const bool part = j + kKeys > every;
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + g + 8 * (e >> 1) >= lim[e & 1]) sc[e] = -INFINITY;
       }
       const float mx[2] = {fmaxf(sc[0], sc[2]) * c2, fmaxf(sc[1], sc[3]) * c2};
       if (__any_sync(0xffffffffu, mx[0] - m[0] > kRescale || mx[1] - m[1] > kRescale)) {  // also from m = -inf
@@ -307,18 +318,45 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
       for (int e = 0; e < 4; ++e) w[e] = ex2(fmaf(sc[e], c2, mm[e & 1]));
       l[0] += w[0] + w[2];
       l[1] += w[1] + w[3];
-      const uint32_t p0 = transpose8x8(St<T>::pack(w[0], w[1]));  // head g, keys 2t, 2t + 1
+      const uint32_t p0 = transpose8x8(St<T>::pack(w[0], w[1]));  // row g, keys 2t, 2t + 1
       const uint32_t p1 = transpose8x8(St<T>::pack(w[2], w[3]));  // keys 2t + 8, 2t + 9
+      auto add = [&](auto all, bool keep0, bool keep1) {  // to all rows, or to those of 2t, 2t + 1 that are kept
 #pragma unroll
-      for (int b = 0; b < VB; ++b) {
-        const uint32_t x[4][4] = {{vr[b][0].x, vr[b][0].y, vr[b][0].z, vr[b][0].w}, {vr[b][1].x, vr[b][1].y, vr[b][1].z, vr[b][1].w},
-                                  {vr[b][2].x, vr[b][2].y, vr[b][2].z, vr[b][2].w}, {vr[b][3].x, vr[b][3].y, vr[b][3].z, vr[b][3].w}};
+        for (int b = 0; b < VB; ++b) {
+          const uint32_t x[4][4] = {{vr[b][0].x, vr[b][0].y, vr[b][0].z, vr[b][0].w}, {vr[b][1].x, vr[b][1].y, vr[b][1].z, vr[b][1].w},
+                                    {vr[b][2].x, vr[b][2].y, vr[b][2].z, vr[b][2].w}, {vr[b][3].x, vr[b][3].y, vr[b][3].z, vr[b][3].w}};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // rows g, g + 8 of the tile: channels 8g + 2e, 8g + 2e + 1
-          const uint32_t a[4] = {__byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[0][e], x[1][e], 0x7632),
-                                 __byte_perm(x[2][e], x[3][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x7632)};
-          Mma<T>::run(acc[b][e], a, p0, p1);
+          for (int e = 0; e < 4; ++e) {  // rows g, g + 8 of the tile: channels 8g + 2e, 8g + 2e + 1
+            const uint32_t a[4] = {__byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[0][e], x[1][e], 0x7632),
+                                   __byte_perm(x[2][e], x[3][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x7632)};
+            if constexpr (decltype(all)::value) {
+              Mma<T>::run(acc[b][e], a, p0, p1);
+            } else {
+              float d[4] = {acc[b][e][0], acc[b][e][1], acc[b][e][2], acc[b][e][3]};
+              Mma<T>::run(d, a, p0, p1);
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (u & 1 ? keep1 : keep0) acc[b][e][u] = d[u];
+            }
+          }
         }
+      };
+      if (part && every < j1) {
+        // A value that a token does not see may be an infinity or NaN: from
+        // the last token back, each with the values that it sees.
+#pragma unroll 1
+        for (int tok = last_tok; tok >= first_tok; --tok) {
+          const int see = keys_seen(s, tok, p.pk.causal);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (j + 2 * t + (e & 1) + 8 * (e >> 1) < see) continue;
+#pragma unroll
+            for (int b = 0; b < VB; ++b) vr[b][e] = make_uint4(0, 0, 0, 0);
+          }
+          add(std::false_type{}, token(2 * t) == tok, token(2 * t + 1) == tok);
+        }
+      } else {
+        add(std::true_type{}, true, true);
       }
     }
     // join the warps
@@ -339,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
       }
     }
     __syncthreads();
-    const bool last = see <= len;  // the token's only chunk
     for (int e = threadIdx.x; e < rows * (DP / 4); e += kThreads) {
       const int rr = e / (DP / 4), c = (e - rr * (DP / 4)) * 4;
       if (c >= p.D) continue;
@@ -358,8 +395,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const Param
         sum = fmaf(lw, ff, sum);
         o.x = fmaf(x.x, ff, o.x); o.y = fmaf(x.y, ff, o.y); o.z = fmaf(x.z, ff, o.z); o.w = fmaf(x.w, ff, o.w);
       }
-      const int h = h0 + rr;
-      if (last) {
+      const int h = head(rr), tok = token(rr);
+      const int64_t row = s.q0 + tok;
+      const int see = keys_seen(s, tok, p.pk.causal);
+      if (j0 >= see) continue;  // the join does not look for it
+      if (see <= len) {  // the token's only chunk
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         if (sum == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
         store_out<T>(p, row, h, c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -462,7 +502,7 @@ int chunks_for(int64_t T, int group, int Hk) {
 
 template <typename T, int DP>
 int run(const Params& p, int sms, cudaStream_t s) {
-  const int64_t most = (int64_t)p.pk.T * p.chunks * p.Hk * p.row_tiles;
+  const int64_t most = ((int64_t)p.pk.T * p.group / kRows + p.pk.B) * p.chunks * p.Hk;
   const int grid = (int)std::min<int64_t>(most, (int64_t)sms * kCtasPerSm);
   if (p.D == DP) chunk_kernel<T, DP, true><<<grid, kThreads, 0, s>>>(p);
   else chunk_kernel<T, DP, false><<<grid, kThreads, 0, s>>>(p);
@@ -484,9 +524,14 @@ int run(const Params& p, int sms, cudaStream_t s) {
 
 }  // namespace step
 
-// Few queries per sequence: the keys are read for each query token, so this
-// form is for batches with at most a few tokens per sequence.
-bool attn_step_applies(int B, int64_t T, int dtype) { return dtype != UPLIFT_LA_F32 && T <= 4ll * B && T <= 65536; }
+// Few queries per sequence: the keys are read once for every eight rows, where
+// the tiles of tok_attn_fwd.cu are mostly empty.  16 sequences, this form / that
+// one (us): 32 heads on 8, 8192 keys: 1 token 97 / 278, 4: 148 / 280, 8: 241 / 283,
+// 16: 454 / 286; 1000 keys: 8 tokens 52 / 52; 8 heads on 8, 2000 keys: 8 tokens
+// 36 / 42, 16: 56 / 42; 32 heads on 1, 2000 keys: 4 tokens 47 / 83.
+bool attn_step_applies(int B, int64_t T, int group, int dtype) {
+  return dtype != UPLIFT_LA_F32 && T <= 8ll * B && T <= 65536 && T * group < (1ll << 31) - 64;
+}
 
 int64_t attn_step_workspace(int64_t T, int Hq, int Hk, int D) {
   return T * step::chunks_for(T, Hq / Hk, Hk) * Hq * (D + 2) * 4;
@@ -502,13 +547,14 @@ int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s) {
   p.lse = a.lse;
   p.pk = a.pk;
   p.Hq = a.Hq; p.Hk = a.Hk; p.group = a.Hq / a.Hk; p.D = a.D;
-  p.row_tiles = (p.group + kRows - 1) / kRows;
+  const int64_t tiles = std::max<int64_t>(std::min<int64_t>(a.pk.B, a.pk.T), ((int64_t)a.pk.T * p.group + kRows - 1) / kRows);
+  p.units = (float)tiles;
   p.chunks = chunks_for(a.pk.T, p.group, a.Hk);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)a.pk.T * p.chunks * a.Hq * a.D);
   p.scale = a.scale;
-  const int64_t units = (int64_t)a.pk.T * a.Hk * p.row_tiles, slots = (int64_t)sms * kCtasPerSm;
-  p.share = 2 * units >= slots ? 0.f : (float)(a.Hk * p.row_tiles) / (float)slots;
+  const int64_t slots = (int64_t)sms * kCtasPerSm;
+  p.share = 2 * tiles * a.Hk >= slots ? 0.f : (float)a.Hk / (float)slots;
   if (a.dtype == UPLIFT_LA_BF16)
     return a.D <= 64 ? run<__nv_bfloat16, 64>(p, sms, s) : run<__nv_bfloat16, 128>(p, sms, s);
   return a.D <= 64 ? run<__half, 64>(p, sms, s) : run<__half, 128>(p, sms, s);
