@@ -247,7 +247,7 @@ int uplift_la_set_kernel_policy(int policy);
 #define UPLIFT_LA_KERNEL_TENSOR_CORE_GUIDE_RESIZE 7  /* both fusions */
 int uplift_la_last_kernel(void);
 
-/* Device status word of the tensor-core kernels: 0 when every launch so far
+/* Device status word of the tensor-core kernels (uplift_tokens.h's too): 0 when every launch so far
  * completed its pipeline, else the role (1 producer, 2 MMA, 3 softmax or
  * split, 4 epilogue) whose bounded wait expired first.  Synchronises with
  * the device; `clear` resets the word.  Returns -1 if the read failed. */

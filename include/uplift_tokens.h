@@ -5,8 +5,8 @@
  * position rotation that feeds it.
  *
  * Token tensors are [rows, heads, D] with channel stride 1, given as
- * uplift_tok_rows: views into a fused projection output work.  Sequences are packed: sequence b owns the rows
- * cu[b] .. cu[b + 1] - 1 of its tensor; cu is a device array of B + 1
+ * uplift_tok_rows: views into a fused projection output work.  Sequences are
+ * packed: sequence b owns the rows cu[b] .. cu[b + 1] - 1 of its tensor; cu is a device array of B + 1
  * ascending int32 values.  Row numbers read from device arrays are clamped
  * to the tensors, so no content of these arrays makes a kernel leave them.
  *
@@ -15,7 +15,8 @@
  * storage type.  The entry points allocate nothing, never synchronise, are
  * deterministic (no floating-point atomics) and can be captured into CUDA
  * graphs; each returns UPLIFT_LA_OK or an error code (message in
- * uplift_la_last_error()).
+ * uplift_la_last_error()).  A tensor-core launch whose bounded wait ran out is
+ * reported by uplift_la_device_status() and the registered host status word.
  */
 #ifndef UPLIFT_TOKENS_H_
 #define UPLIFT_TOKENS_H_
@@ -98,8 +99,8 @@ typedef struct {
   uplift_tok_rows q;        /* [T, Hq, D] */
   uplift_tok_rows k, v;     /* [S, Hk, D] */
   uplift_tok_rows out;      /* [T, Hq, D] */
-  uplift_tok_rows out_lo;   /* [T, Hq, D] or data = NULL; 16-bit types only: what the rounding of out left (forward: written;
-                               backward: read, for gradients as exact as if out had not been rounded) */
+  uplift_tok_rows out_lo;   /* [T, Hq, D] or data = NULL; 16-bit types only: what the rounding of out left
+                               (forward: written; backward: read, so that the gradients do not carry it) */
   uplift_tok_rows dout;     /* backward only: gradient of out */
   uplift_tok_rows dq, dk, dv; /* backward only: the gradients, written whole: zero for rows of no sequence and keys that
                                  no query sees */

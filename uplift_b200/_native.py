@@ -250,7 +250,7 @@ class HostStatus:
             self._word.value = 0
             load().uplift_la_device_status(1)  # clear the device copy too (error path: synchronises)
             raise ExpiredWaitError(
-                f"a Local Attender tensor-core launch on this process gave up after a bounded wait "
+                f"a tensor-core launch (Local Attender or attention) on this process gave up after a bounded wait "
                 f"(role: {ROLES.get(code, code)}); its output is incomplete and must not be used")
 
 

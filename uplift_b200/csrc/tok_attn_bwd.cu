@@ -34,6 +34,13 @@
 // Rows that go by behind the end of their sequence belong to the next one:
 // their P and dS are set to zero and the rows in shared memory too, since an
 // infinity or NaN in them would turn the products into NaN.
+//
+// Bound by the chain of a step: scores and dP (tensor cores), P and dS (the
+// warps), products with them (tensor cores), with two steps in flight, which
+// TMEM allows.  Six documents of 300 to 2500 tokens, 32 heads on 8 of 128,
+// bf16, causal: dQ 157 us (720 TFLOP/s), dK and dV 186 us (810), 0.44 and 0.49 of a
+// large library product.  16 images of 1025, 6 heads of 64, fp16: 66 and 88 us (a
+// step of training 245 us; with one thread per row 266).
 
 #include <math.h>
 #include <string.h>
@@ -634,7 +641,8 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
 
 // delta = rowsum(dO O): eight lanes per row, 16 bytes each at a time.  O is
 // taken as out + out_lo: the rounding of out alone would be the largest error
-// of dS in rows that see few keys.
+// of dS in rows that see few keys.  Bound by HBM: 29 us for the three tensors
+// of 5986 tokens of 32 heads of 128 in bf16 (147 MB, 5.1 TB/s).
 // Also sets the item counters of the passes that follow to zero.
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo, float* delta, int* counters, int T_, int Hq, int D) {

@@ -26,6 +26,11 @@
 // grow by more than 2^8.  The warps' results are joined in shared memory; the
 // chunks' results go to a workspace and a second kernel joins them, unless
 // the token has one chunk only.
+//
+// 64 tokens on up to 8192 keys each (762 MB), 32 heads on 8 of 128, bf16: 135
+// us, 5.6 TB/s, 0.86 of a copy; on 8192 keys each 333 us, 6.45 TB/s, 0.99.  4
+// tokens on up to 1500 keys: 13 us on the device for both kernels, where the
+// reads take 3: launches and the length of one chunk.
 
 #include <math.h>
 

