@@ -592,3 +592,79 @@ def test_rows_beyond_32_bit_offsets():
     ref = R.attention(q, tail, tail, starts([1, 0, 2]), starts([100, 0, 100]), None, True, None, None, BF16)
     R.check(small, ref["out"], ref["out_tol"], "small")
     R.check(got, ref["out"], ref["out_tol"], "large")
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_one_tensor_in_three_places(dt):
+    """q, k and v are the same leaf: its gradient is the sum of the three."""
+    gen = torch.Generator().manual_seed(41)
+    x, g = rand(gen, 150, 2, 64, dt=dt, scale=1.2), rand(gen, 150, 2, 64, dt=dt)
+    cu = starts([70, 80])
+    three = [x.clone().requires_grad_() for _ in range(3)]
+    apart = torch.autograd.grad(ops.packed_attention(*three, cu), three, g)
+    x.requires_grad_()
+    (together,) = torch.autograd.grad(ops.packed_attention(x, x, x, cu), x, g)
+    # two additions in the storage type, each off by half a step
+    size = sum(d.double().abs() for d in apart)
+    err = (together.double() - sum(d.double() for d in apart)).abs()
+    assert (err <= 2.1 * torch.finfo(dt).eps / 2 * size).all()
+
+
+def test_calls_from_several_threads_and_streams():
+    """Steps, prompts and gradients at once, each thread on its stream: the results of the calls one by one."""
+    import threading
+    gen = torch.Generator().manual_seed(43)
+    jobs = []
+    for i, (lens, D, dt) in enumerate([([600, 77], 128, BF16), ([1] * 5, 64, F16), ([333], 64, F16), ([90, 200], 64, F32)]):
+        q, k, v = qkv(gen, sum(lens), sum(lens), 4, 2, D, dt)
+        jobs.append((q, k, v, starts(lens), rand(gen, *q.shape, dt=dt)))
+
+    def run(q, k, v, cu, g):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.packed_attention(*leaves, cu)
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+    alone = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong, streams = [], [torch.cuda.Stream() for _ in jobs]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                if not all(torch.equal(a, b) for a, b in zip(run(*jobs[i]), alone[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_two_graphs_at_once():
+    """Two captured steps and a captured prompt replayed together share no workspace."""
+    gen = torch.Generator().manual_seed(45)
+    runs = []
+    for n_q, n_k in (([1, 1, 1], [900, 1, 400]), ([2, 1, 1], [700, 50, 1300]), ([300, 20], [300, 20])):
+        q, k, v = qkv(gen, sum(n_q), sum(n_k), 8, 2, 64, BF16)
+        cu_q, cu_k = starts(n_q), starts(n_k)
+        exp = ops.packed_attention(q, k, v, cu_q, cu_k)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.packed_attention(q, k, v, cu_q, cu_k)
+        runs.append((graph, torch.cuda.Stream(), out, exp, (q, k, v, cu_q, cu_k)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, exp, _ in runs:
+        assert torch.equal(out, exp)
+
+
+def test_a_second_derivative_is_refused():
+    q = torch.randn(20, 2, 64, device=DEV, requires_grad=True)
+    out = ops.packed_attention(q, q, q, starts([20]))
+    (d,) = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice"):
+        d.sum().backward()
