@@ -635,15 +635,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       for (int c = 0; c < C::kChunks; ++c) {
         if (64 * c >= p.D) break;
         uint8_t* row = stage + lane * 128;
-        uint32_t o[32];
-        if (tiles > 0) tc_ld32(to + 64 * c + 32 * group, o);
-        if (tiles > 0) tc_wait_ld_regs(o);
         const int row0 = it.row + first + 32 * q;
         // out, then (for the gradients) what its rounding left
 #pragma unroll 1
         for (int part = 0; part < (LO ? 2 : 1); ++part) {
+          uint32_t o[32];
+          if (tiles > 0) tc_ld32(to + 64 * c + 32 * group, o);
           if (group == 0 && lane == 0) bulk_wait_read0();  // the staging buffer is free
           named_bar(pair, 64);
+          if (tiles > 0) tc_wait_ld_regs(o);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t y[4];
