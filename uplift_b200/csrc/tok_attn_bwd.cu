@@ -31,6 +31,11 @@
 // are not idle for the length of two barrier waits per step; warp 18 (KEYS)
 // fetches lse and delta of the queries that go by.
 //
+// The passes do not need each other.  dQ runs first; when all of its CTAs are
+// running (and delta is there, which they have waited for) the other may start,
+// so that its CTAs take the SMs as the first pass leaves them; it ends only
+// after the first has.
+//
 // Rows that go by behind the end of their sequence belong to the next one:
 // their P and dS are set to zero and the rows in shared memory too, since an
 // infinity or NaN in them would turn the products into NaN.
@@ -183,6 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (!KEYS) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // delta and the counters
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -631,6 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     if (lane == 0) bulk_wait_all();
   }
 
+  if (KEYS) asm volatile("griddepcontrol.wait;" ::: "memory");  // what follows this pass follows the other one too
   tc_fence_before();
   __syncthreads();
   if (warp == 17) {
@@ -646,6 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
 // Also sets the item counters of the passes that follow to zero.
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo, float* delta, int* counters, int T_, int Hq, int D) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const int64_t item = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
   const int l = threadIdx.x & 7;
@@ -680,18 +691,30 @@ __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo
   if (live && l == 0) delta[(int64_t)h * T_ + t] = sum;
 }
 
+// early: it may start before the kernel in front of it in the stream has ended.
 template <typename T, int DP, bool KEYS>
-int launch(const Params& p, int dev, int grid, cudaStream_t s) {
+int launch(const Params& p, int dev, int grid, bool early, cudaStream_t s) {
   static std::atomic<bool> configured[64] = {};
   const int rc = opt_in_smem(gradient_kernel<T, DP, KEYS>, Cfg<DP>::kSmem, configured, dev);
   if (rc != UPLIFT_LA_OK) return rc;
-  gradient_kernel<T, DP, KEYS><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<DP>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gradient_kernel<T, DP, KEYS>, p);
+  if (e != cudaSuccess) return fail(UPLIFT_LA_ERR_CUDA, "attention backward launch: %s", cudaGetErrorString(e));
   return launched("attention backward");
 }
 
 template <typename T, bool KEYS>
-int launch_d(const Params& p, int dev, int grid, cudaStream_t s) {
-  return p.D <= 64 ? launch<T, 64, KEYS>(p, dev, grid, s) : launch<T, 128, KEYS>(p, dev, grid, s);
+int launch_d(const Params& p, int dev, int grid, bool early, cudaStream_t s) {
+  return p.D <= 64 ? launch<T, 64, KEYS>(p, dev, grid, early, s) : launch<T, 128, KEYS>(p, dev, grid, early, s);
 }
 
 }  // namespace bwd
@@ -733,7 +756,7 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
     p.counter = counters;
     const int64_t most = ((int64_t)T / kM + a.pk.B) * a.Hq;
     const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
-    rc = bf16 ? launch_d<__nv_bfloat16, false>(p, dev, grid, s) : launch_d<__half, false>(p, dev, grid, s);
+    rc = bf16 ? launch_d<__nv_bfloat16, false>(p, dev, grid, true, s) : launch_d<__half, false>(p, dev, grid, true, s);
     if (rc != UPLIFT_LA_OK) return rc;
   }
   if (S > 0) {
@@ -751,7 +774,7 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
     p.counter = counters + 1;
     const int64_t most = ((int64_t)S / kM + a.pk.B) * a.Hk;
     const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
-    rc = bf16 ? launch_d<__nv_bfloat16, true>(p, dev, grid, s) : launch_d<__half, true>(p, dev, grid, s);
+    rc = bf16 ? launch_d<__nv_bfloat16, true>(p, dev, grid, T > 0, s) : launch_d<__half, true>(p, dev, grid, T > 0, s);
   }
   return rc;
 }
