@@ -92,6 +92,7 @@ def test_backward_and_step_workspaces(lib):
     assert lib.uplift_tok_norm_rotate_backward(_nr_args(dict(dq=0)), None) == _native.ERR_ARG
     need = lib.uplift_tok_attention_workspace(4, 4, 100, 8, 2, 64, _native.BF16)
     assert need > 0 and lib.uplift_tok_attention_workspace(4, 4, 100, 8, 2, 64, _native.F32) == 0
+    assert lib.uplift_tok_attention_workspace(4000, 4000, 100, 8, 2, 64, _native.BF16) == 0  # a chunk per token
     step = dict(B=4, T=4, S=100, Hq=8, Hk=2, st=(512, 64))
     assert _attn(lib, **step) == _native.ERR_ARG
     assert _attn(lib, ws=16, ws_bytes=need - 1, **step) == _native.ERR_ARG

@@ -99,6 +99,15 @@ def test_a_few_tokens_on_long_histories(causal):
     run_attention(q, k, v, starts(n_q), starts(n_k), None, causal, gen=gen)
 
 
+def test_a_step_of_many_sequences():
+    """So many that every token's keys are one chunk (no workspace), some without keys."""
+    gen = torch.Generator().manual_seed(47)
+    n_q, n_k = [1 + (i % 3 == 0) for i in range(500)], [(i * 13) % 90 for i in range(500)]
+    assert _native.load().uplift_tok_attention_workspace(500, sum(n_q), sum(n_k), 16, 8, 64, _native.BF16) == 0
+    q, k, v = qkv(gen, sum(n_q), sum(n_k), 16, 8, 64, BF16)
+    run_attention(q, k, v, starts(n_q), starts(n_k), None, True, grads=False, gen=gen)
+
+
 @pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 64), (F32, 128)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_gradients_in_segments_with_room(dt, D, causal):

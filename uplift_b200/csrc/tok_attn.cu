@@ -119,7 +119,8 @@ int uplift_tok_attention_forward(const uplift_tok_attention_args* args, void* st
   if (a.dtype == UPLIFT_LA_F32) return attn_simt_forward(a, s);
   if (!attn_step_applies(a.pk.B, a.pk.T, a.Hq / a.Hk, a.dtype)) return attn_tc_forward(a, s);
   const int64_t need = attn_step_workspace(a.pk.T, a.Hq, a.Hk, a.D);
-  if (args->workspace == nullptr || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15u) != 0)
+  if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(args->workspace) & 15u) != 0))
     return fail(UPLIFT_LA_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
   return attn_step_forward(a, args->workspace, s);
 }

@@ -539,7 +539,8 @@ bool attn_step_applies(int B, int64_t T, int group, int dtype) {
 }
 
 int64_t attn_step_workspace(int64_t T, int Hq, int Hk, int D) {
-  return T * step::chunks_for(T, Hq / Hk, Hk) * Hq * (D + 2) * 4;
+  const int chunks = step::chunks_for(T, Hq / Hk, Hk);
+  return chunks == 1 ? 0 : T * chunks * Hq * (D + 2) * 4;  // a token's only chunk is written at once
 }
 
 int attn_step_forward(const AttnArgs& a, void* workspace, cudaStream_t s) {
