@@ -88,7 +88,8 @@ int64_t uplift_tok_norm_rotate_partial_floats(int D);
  *
  * A query that sees no key gets out = 0 and lse = -inf, and so do rows of
  * no sequence.  What keys that a query does not see hold (NaN, infinities)
- * does not reach its output.
+ * does not reach its output or its gradient, nor does what that query and its
+ * dout hold reach the gradients of these keys.
  *
  * bf16 / fp16: D a multiple of 8; tensors 16-byte aligned, strides
  * multiples of 8 elements and row strides multiples of the head stride

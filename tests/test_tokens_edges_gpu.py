@@ -1,0 +1,103 @@
+"""The token-sequence operators where masks, types and forms meet: what a
+masked row may not reach in the gradients."""
+import math
+
+import pytest
+import torch
+
+import tokens_reference as R
+from uplift_b200 import _native, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib(cuda_lib):
+    yield
+    assert _native.device_status(clear=True) == 0  # no bounded wait ran out
+
+
+def starts(lens, first=0):
+    return torch.tensor([first] + [first + sum(lens[:i + 1]) for i in range(len(lens))], dtype=torch.int32, device=DEV)
+
+
+def rand(gen, *shape, dt=F32, scale=1.0):
+    return (torch.randn(*shape, generator=gen) * scale).to(DEV).to(dt)
+
+
+def qkv(gen, T, S, Hq, Hk, D, dt, scale=1.3):
+    return rand(gen, T, Hq, D, dt=dt, scale=scale), rand(gen, S, Hk, D, dt=dt, scale=scale), rand(gen, S, Hk, D, dt=dt)
+
+
+def attention_and_gradients(q, k, v, g, *args, **kw):
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    out = ops.packed_attention(*leaves, *args, **kw)
+    return (out.detach(), *torch.autograd.grad(out, leaves, g))
+
+
+# ------------------------------------------------- gradients behind the mask
+KINDS = [(BF16, 128), (F16, 64), (BF16, 80), (F32, 64)]
+
+
+@pytest.mark.parametrize("dt,D", KINDS)
+@pytest.mark.parametrize("Hq,Hk", [(2, 1), (3, 3), (4, 2)])
+@pytest.mark.parametrize("n_q,n_k", [(300, 300), (130, 333), (333, 130)])
+@pytest.mark.parametrize("at", [1, 63, 64, 100, 128])
+def test_later_keys_do_not_reach_gradients_of_earlier_queries(dt, D, Hq, Hk, n_q, n_k, at):
+    """Causal: NaN and infinities in keys and values from `at` on leave dq of the queries that see none of them as it
+    was (zero for those that see no key), and make that of the others NaN."""
+    gen = torch.Generator().manual_seed(51)
+    q, k, v = qkv(gen, n_q + 20, n_k + 20, Hq, Hk, D, dt)
+    g = rand(gen, *q.shape, dt=dt)
+    cu = starts([n_q, 20]), starts([n_k, 20])
+    out, dq, _, _ = attention_and_gradients(q, k, v, g, *cu)
+    k[at:n_k], v[at + 1:n_k] = math.nan, math.inf
+    got, got_dq, _, _ = attention_and_gradients(q, k, v, g, *cu)
+    hidden = torch.arange(n_q + 20, device=DEV) + n_k - n_q < at  # the last key that they see is before `at`
+    hidden[n_q:] = True  # the other sequence
+    assert torch.equal(got[hidden], out[hidden])
+    assert torch.equal(got_dq[hidden], dq[hidden])
+    assert bool(got_dq[~hidden].isnan().all())
+    if n_q > n_k:
+        assert not got_dq[:n_q - n_k].any()
+
+
+@pytest.mark.parametrize("dt,D", KINDS)
+@pytest.mark.parametrize("Hq,Hk", [(2, 1), (3, 3), (4, 2)])
+@pytest.mark.parametrize("n_q,n_k", [(300, 300), (130, 333), (333, 130)])
+@pytest.mark.parametrize("end", [1, 64, 100, 128])
+def test_earlier_queries_do_not_reach_gradients_of_later_keys(dt, D, Hq, Hk, n_q, n_k, end):
+    """Causal: NaN in the first `end` queries and infinities in their outputs' gradients leave dk and dv of the keys
+    that none of them sees as they were."""
+    gen = torch.Generator().manual_seed(53)
+    q, k, v = qkv(gen, n_q + 20, n_k + 20, Hq, Hk, D, dt)
+    g = rand(gen, *q.shape, dt=dt)
+    cu = starts([n_q, 20]), starts([n_k, 20])
+    _, _, dk, dv = attention_and_gradients(q, k, v, g, *cu)
+    q[:end:2], g[:end] = math.nan, math.inf
+    _, _, got_dk, got_dv = attention_and_gradients(q, k, v, g, *cu)
+    hidden = torch.arange(n_k + 20, device=DEV) > end - 1 + n_k - n_q
+    hidden[n_k:] = True
+    assert torch.equal(got_dk[hidden], dk[hidden]) and torch.equal(got_dv[hidden], dv[hidden])
+    assert not bool(got_dk[~hidden].isfinite().any()) and not bool(got_dv[~hidden].isfinite().any())
+
+
+@pytest.mark.parametrize("dt,D", KINDS)
+@pytest.mark.parametrize("row", [0, 70, 127, 128, 200, 299])
+def test_an_infinite_gradient_reaches_the_keys_that_its_query_sees(dt, D, row):
+    """One infinity in the outputs' gradient: its channel of dv is infinite for the keys that the query sees, and the
+    other channels are as they were; dk is not finite there."""
+    gen = torch.Generator().manual_seed(55)
+    q, k, v = qkv(gen, 300, 300, 4, 2, D, dt, scale=0.3)
+    g = rand(gen, *q.shape, dt=dt)
+    cu = starts([300])
+    _, _, dk, dv = attention_and_gradients(q, k, v, g, cu)
+    g[row, 1, 5] = -math.inf
+    _, dq, got_dk, got_dv = attention_and_gradients(q, k, v, g, cu)
+    assert bool((got_dv[:row + 1, 0, 5] == -math.inf).all()) and not bool(got_dk[:row + 1, 0].isfinite().any())
+    got_dv[:row + 1, 0, 5] = dv[:row + 1, 0, 5]
+    got_dk[:row + 1, 0] = dk[:row + 1, 0]
+    assert torch.equal(got_dv, dv) and torch.equal(got_dk, dk)
+    assert dq.isfinite().all(-1).sum() == 300 * 4 - 1

@@ -38,7 +38,11 @@
 //
 // Rows that go by behind the end of their sequence belong to the next one:
 // their P and dS are set to zero and the rows in shared memory too, since an
-// infinity or NaN in them would turn the products into NaN.
+// infinity or NaN in them would turn the products into NaN.  The same holds in
+// the steps on the causal edge, whose columns some of the rows that stay do not
+// see: the groups look the tiles through before the second products, replace
+// infinities and NaN by zero and put them back into the results of the rows
+// that do see them.
 //
 // Bound by the chain of a step: scores and dP (tensor cores), P and dS (the
 // warps), products with them (tensor cores), with two steps in flight, which
@@ -110,6 +114,7 @@ struct Params {
   CUtensorMap x0, x1;  // rows that stay: K, V or Q, dO; box {64, 1, 128}
   CUtensorMap y0, y1;  // rows that go by: Q, dO or K, V; box {64, 1, 64}
   CUtensorMap o0, o1;  // results: dV, dK or dQ; box {64, 1, 32}
+  Rows y[2];           // as y0, y1
   Rows out0, out1;
   const float* lse;
   const float* delta;
@@ -124,6 +129,51 @@ struct Params {
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
                                           const WaitLimit& limit) {
   return mbar_wait_inline(b, parity, abort_flag, where, limit, &g_tok_bwd_status);
+}
+
+// Makes the tiles of a step (Y0, Y1) fit for the second products: rows from
+// `rows` on become zero (both tiles, all channels); with `edge`, so do the
+// infinities and NaN of the tiles that are multiplied (Y0, and with KEYS Y1).
+// 256 threads, each its own 16-byte pieces.
+template <typename T, int CHUNKS, bool KEYS>
+__device__ __noinline__ void clean_step(uint8_t* y, int rows, bool edge, int tid, volatile int* cleaned) {
+#pragma unroll 1
+  for (int i = tid; i < 2 * CHUNKS * kN * 8; i += 256) {
+    uint4* piece = reinterpret_cast<uint4*>(y) + i;
+    if ((i & (kN * 8 - 1)) >= rows * 8) {
+      *piece = make_uint4(0, 0, 0, 0);
+    } else if (edge && (KEYS || i < CHUNKS * kN * 8)) {
+      const uint4 v = *piece;
+      uint32_t acc = nonfinite_probe<T>(nonfinite_probe<T>(nonfinite_probe<T>(nonfinite_probe<T>(0, v.x), v.y), v.z), v.w);
+      const float2 f = St<T>::unpack(acc);
+      if (f.x == 0.f && f.y == 0.f) continue;
+      *cleaned = 1;
+      T* e = reinterpret_cast<T*>(piece);
+      for (int k = 0; k < 8; ++k)
+        if (!isfinite(St<T>::f(e[k]))) e[k] = St<T>::t(0.f);
+    }
+  }
+  fence_proxy_async();
+}
+
+// Puts what was taken out of the rows y0 .. y1 - 1 of y (the channels
+// from `y` on) back into a staged row of results: weights are positive, so dV gets
+// the infinity or NaN itself (`itself`); where a query or key is not finite
+// neither is the score, so its weight's gradient is zero or NaN and its
+// product with the value NaN.
+template <typename T>
+__device__ __noinline__ void put_back(uint8_t* row, int lane, const T* y, int64_t stride, int y0, int y1, int channels,
+                                      bool itself) {
+#pragma unroll 1
+  for (int j = y0; j < y1; ++j) {
+#pragma unroll 1
+    for (int i = 0; i < channels; ++i) {
+      const float x = St<T>::f(y[j * stride + i]);
+      if (isfinite(x)) continue;
+      T* e = reinterpret_cast<T*>(row + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2);
+      *e = St<T>::t(itself ? St<T>::f(*e) + x : __int_as_float(0x7fc00000));
+    }
+  }
 }
 
 template <typename T, int DP, bool KEYS>
@@ -153,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   uint64_t* drain = item_empty + kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  volatile int* cleaned = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 16);  // some tile of this CTA was
   uint32_t* go = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 20);  // steps whose second products may begin
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + C::kOffItems);
 
@@ -182,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     mbar_init(drain, 1);
     abort_flag[0] = 0;
     abort_flag[1] = 0;  // stays 0: the flag of waits that must not be aborted
+    *cleaned = 0;
     *go = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -456,11 +508,17 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
       if (!ok) break;
       Item it;
       it.n = items[islot].n; it.live = items[islot].live; it.row = items[islot].row; it.h = items[islot].h;
-      it.ny = items[islot].ny; it.steps = items[islot].steps; it.off = items[islot].off;
+      it.ny = items[islot].ny; it.steps = items[islot].steps; it.off = items[islot].off; it.y0 = items[islot].y0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[islot]);
       if (it.n == 0) break;
       const int total = it.steps * passes;
+      // steps edge0 .. edge1 - 1 (of a head) hold columns that some row does not see
+      int edge0 = 0, edge1 = 0;
+      if (p.pk.causal) {
+        if (KEYS) edge1 = (max(0, it.live - 1 + it.off) + kN - 1) / kN;
+        else if (it.off < it.ny) edge0 = max(0, it.off) / kN, edge1 = it.steps;
+      }
       float nlse = 0.f, ndelta = 0.f;
       if (!KEYS) {
         nlse = -INFINITY;
@@ -534,16 +592,9 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
           tmem_st8(td + c / 2, ds);
         }
         const int rows = it.ny - j * kN;  // of the tile that goes by
-        if (rows < kN) {
-          // rows of the next sequence: zero (both tiles, all channels)
-          uint8_t* y = sY + (gs % C::kStages) * 2 * C::kYBytes;
-          for (int e = rows * 8 + (tid & 255); e < kN * 8; e += 256) {
-#pragma unroll
-            for (int c = 0; c < 2 * C::kChunks; ++c)
-              *reinterpret_cast<uint4*>(y + c * C::kYChunk + e * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-        }
+        const bool edge = j >= edge0 && j < edge1;
+        if (edge || rows < kN)  // rows of the next sequence; infinities and NaN that some row does not see
+          clean_step<T, C::kChunks, KEYS>(sY + (gs % C::kStages) * 2 * C::kYBytes, rows, edge, tid & 255, cleaned);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -588,6 +639,16 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
             for (int i = 0; i < 8; ++i) x[i] = zero ? 0.f : __uint_as_float(o[8 * e + i]) * f;
             *reinterpret_cast<uint4*>(row + (((4 * h + e) ^ (lane & 7)) << 4)) =
                 make_uint4(St<T>::pack(x[0], x[1]), St<T>::pack(x[2], x[3]), St<T>::pack(x[4], x[5]), St<T>::pack(x[6], x[7]));
+          }
+        }
+        if (*cleaned != 0 && !zero) {
+          const Rows& y = p.y[KEYS && w == 0 ? 1 : 0];  // dV takes dO, dK and dQ take queries and keys
+          const int from = KEYS ? max(0, r + it.off) : edge0 * kN;
+          const int to = min(min(it.ny, edge1 * kN), KEYS ? it.ny : r + it.off);
+          for (int e = 0; e < passes; ++e) {
+            const int hy = KEYS ? it.h * p.group + e : it.h / p.group;
+            put_back<T>(row, lane, static_cast<const T*>(y.p) + (int64_t)it.y0 * y.t + (int64_t)hy * y.h + 64 * c, y.t,
+                        from, to, min(64, p.D - 64 * c), KEYS && w == 0);
           }
         }
         fence_proxy_async();
@@ -751,6 +812,8 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
       if ((rc = make_row_map(&p.y1, a.dtype, a.v, S, a.Hk, a.D, kN)) != UPLIFT_LA_OK) return rc;
     }
     if ((rc = make_row_map(&p.o0, a.dtype, a.dq, T, a.Hq, a.D, 32)) != UPLIFT_LA_OK) return rc;
+    p.y[0] = a.k;
+    p.y[1] = a.v;
     p.out0 = a.dq;
     p.heads = a.Hq;
     p.counter = counters;
@@ -768,6 +831,8 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
     }
     if ((rc = make_row_map(&p.o0, a.dtype, a.dv, S, a.Hk, a.D, 32)) != UPLIFT_LA_OK) return rc;
     if ((rc = make_row_map(&p.o1, a.dtype, a.dk, S, a.Hk, a.D, 32)) != UPLIFT_LA_OK) return rc;
+    p.y[0] = a.q;
+    p.y[1] = a.dout;
     p.out0 = a.dv;
     p.out1 = a.dk;
     p.heads = a.Hk;

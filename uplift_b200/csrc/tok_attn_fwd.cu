@@ -136,20 +136,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
 __device__ __forceinline__ uint32_t k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
 __device__ __forceinline__ uint32_t v_pos(int j, int tiles) { return min(2 * j + 2, 2 * tiles - 1); }
 
-template <typename T>
-__device__ __forceinline__ uint32_t nonfinite_probe(uint32_t acc, uint32_t x);  // acc stays 0 in both halves iff x is finite
-template <>
-__device__ __forceinline__ uint32_t nonfinite_probe<__nv_bfloat16>(uint32_t acc, uint32_t x) {
-  __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&x), __nv_bfloat162(__nv_bfloat16(0.f), __nv_bfloat16(0.f)),
-                             *reinterpret_cast<__nv_bfloat162*>(&acc));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-template <>
-__device__ __forceinline__ uint32_t nonfinite_probe<__half>(uint32_t acc, uint32_t x) {
-  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&x), __half2(__half(0.f), __half(0.f)), *reinterpret_cast<__half2*>(&acc));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-
 // The part of V row tid % 64 of a tile that thread tid of a group looks
 // through: every second 16-byte piece of each chunk of 64 channels.
 template <typename T, int CHUNKS>

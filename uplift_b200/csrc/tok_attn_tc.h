@@ -232,6 +232,19 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_probe(uint32_t acc, uint32_t x);  // acc stays 0 in both halves iff x is finite
+template <>
+__device__ __forceinline__ uint32_t nonfinite_probe<__nv_bfloat16>(uint32_t acc, uint32_t x) {
+  __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&x), __nv_bfloat162(__nv_bfloat16(0.f), __nv_bfloat16(0.f)),
+                             *reinterpret_cast<__nv_bfloat162*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t nonfinite_probe<__half>(uint32_t acc, uint32_t x) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&x), __half2(__half(0.f), __half(0.f)), *reinterpret_cast<__half2*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
