@@ -101,3 +101,23 @@ def test_an_infinite_gradient_reaches_the_keys_that_its_query_sees(dt, D, row):
     got_dk[:row + 1, 0] = dk[:row + 1, 0]
     assert torch.equal(got_dv, dv) and torch.equal(got_dk, dk)
     assert dq.isfinite().all(-1).sum() == 300 * 4 - 1
+
+
+# ------------------------------------------------- maxima that grow all along
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("Hq,Hk", [(4, 2), (3, 3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_maxima_that_grow_in_every_tile(dt, D, Hq, Hk, causal):
+    """Scores that rise by about 9 powers of two per 64 keys for some rows, less for others: sums are rescaled in
+    every key tile, and each run gives the same bits."""
+    gen = torch.Generator().manual_seed(63)
+    n = 1500
+    q, k, v = qkv(gen, n, n, Hq, Hk, D, dt, scale=0.5)
+    rise = torch.arange(n, device=DEV)[:, None] * (9 * math.log(2) / 64 / 16)
+    q[:, :, 0] = torch.randint(4, 18, (n, Hq), generator=gen).to(DEV)
+    k[:, :, 0] = rise.to(dt)
+    run = [ops.packed_attention(q, k, v, starts([n]), causal=causal, scale=1.0, return_lse=True) for _ in range(10)]
+    assert all(torch.equal(a, b) for r in run[1:] for a, b in zip(r, run[0]))
+    ref = R.attention(q, k, v, starts([n]), starts([n]), None, causal, 1.0, None, dt)
+    R.check(run[0][0], ref["out"], ref["out_tol"], "out")
+    R.check(run[0][1], ref["lse"], ref["lse_tol"], "lse")

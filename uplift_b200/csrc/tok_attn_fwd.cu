@@ -94,7 +94,7 @@ struct Cfg {
   static constexpr int kStageBytes = 32 * 128;           // a warp's 32 rows x 64 channels
   static constexpr int kOffRows = kOffStage + 8 * kStageBytes;  // [query tile][row]: maximum and the key tile it is of
   static constexpr int kOffBar = kOffRows + 2 * kM * 8;
-  static constexpr int kNumBars = 2 + 2 * kSlots + 4 + 4 + 4 + 2 * kItems + 2;
+  static constexpr int kNumBars = 2 + 2 * kSlots + 4 + 4 + 4 + 2 + 2 * kItems + 2;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffItems = kOffMisc + 32;
   static constexpr int kSmem = kOffItems + kItems * 32;
@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   uint64_t* kv_empty = kv_full + C::kSlots;   // [kSlots]
   uint64_t* s_full = kv_empty + C::kSlots;    // [2][2] scores: query tile, buffer
   uint64_t* p_full = s_full + 4;              // [2][2] weights
-  uint64_t* o_done = p_full + 4;              // [2] a product with V is complete
-  uint64_t* o_full = o_done + 2;              // [2] an item's last product is complete
+  uint64_t* o_done = p_full + 4;              // [2][2] a product with V is complete: query tile, parity of the key tile
+  uint64_t* o_full = o_done + 4;              // [2] an item's last product is complete
   uint64_t* item_full = o_full + 2;           // [kItems]
   uint64_t* item_empty = item_full + kItems;  // [kItems]
   uint64_t* drain = item_empty + kItems;      // [2]
@@ -240,11 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);  // 4 warps
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&o_done[i], 1);
-      mbar_init(&o_full[i], 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&o_full[i], 1);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 18);  // 16 softmax warps, 2 MMA warps
@@ -423,12 +421,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
               for (int ks = 0; ks < kN / 16; ++ks)
                 mma_tmem_a(o, w + 8 * (ks & 1) + 32 * (ks >> 1), v + ((2048 * ks) >> 4), kIdO, (j > 0 || ks > 0) ? 1u : 0u);
-            }
-            if (j + 2 < tiles) scores(ns + j + 2, gk, j + 2 < mine, j + 3 == mine);
-            if (j < mine) {
-              tc_commit(&o_done[t]);
+              // announced before the scores of tile j + 2 are: who sees those
+              // and waits for V_j+1's product must find this phase complete
+              tc_commit(&o_done[2 * t + ((ns + j) & 1)]);
               if (j + 1 == mine) tc_commit(&o_full[t]);
             }
+            if (j + 2 < tiles) scores(ns + j + 2, gk, j + 2 < mine, j + 3 == mine);
             tc_commit(&kv_empty[gv % C::kSlots]);
             atomicExch(issuing, 0);
           }
@@ -536,9 +534,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           adopt(before);
           const bool grow = (mj - m) * c2 > kRescale;  // also from m = -inf
           if (__any_sync(0xffffffffu, grow)) {
-            // the last product that wrote O has to be complete (the one
-            // before it is: the scores of this tile came after it)
-            ok = wait(&o_done[t], (nn - 1) & 1, 3);
+            // the last product that wrote O has to be complete; the one two
+            // before it, the last phase of the same barrier, is: it was
+            // announced long before the scores of this tile
+            ok = wait(&o_done[2 * t + ((nn - 1) & 1)], ((nn - 1) >> 1) & 1, 3);
             if (!ok) break;
             tc_fence_after();
             const float a = grow ? ex2((m - mj) * c2) : 1.f;
