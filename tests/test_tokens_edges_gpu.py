@@ -121,3 +121,32 @@ def test_maxima_that_grow_in_every_tile(dt, D, Hq, Hk, causal):
     ref = R.attention(q, k, v, starts([n]), starts([n]), None, causal, 1.0, None, dt)
     R.check(run[0][0], ref["out"], ref["out_tol"], "out")
     R.check(run[0][1], ref["lse"], ref["lse_tol"], "lse")
+
+
+# --------------------------------------- values shared by two query tiles
+@pytest.mark.parametrize("dt,D", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("Hq,Hk", [(3, 3), (3, 1), (2, 1)])
+@pytest.mark.parametrize("key", [0, 70, 127, 150])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_an_infinite_value_of_no_weight_gives_one_result(dt, D, Hq, Hk, key, bad):
+    """A value that is not finite, with a weight that rounds to zero for the rows from 128 on: wherever the row of
+    tiles takes it from, every run gives the same bits, rows that do not see it are as they were, and the others of
+    its item are not finite in its channel alone."""
+    gen = torch.Generator().manual_seed(65)
+    n = 300
+    q, k, v = qkv(gen, n, n, Hq, Hk, D, dt, scale=0.5)
+    q[:, :, 0], k[:, :, 0] = 0, 0
+    q[128:, :, 0], k[key, :, 0] = 30, -40  # a score of -1200 D^-1/2: exp of it is below 2^-150
+    clean = ops.packed_attention(q, k, v, starts([n]))
+    v[key, 0, 3] = bad
+    first = ops.packed_attention(q, k, v, starts([n]))
+    for _ in range(40):
+        again = ops.packed_attention(q, k, v, starts([n]))
+        assert torch.equal(again.view(torch.int16), first.view(torch.int16))
+    heads = Hq // Hk
+    assert torch.equal(first[:key], clean[:key]) and torch.equal(first[:, heads:], clean[:, heads:])
+    item = 256 if heads % 2 else 128
+    seen = first[key:item, :heads, 3]
+    assert bool((seen == bad).all()) if bad == math.inf else bool(seen.isnan().all())
+    first[key:, :heads, 3] = clean[key:, :heads, 3]
+    assert torch.equal(first, clean)

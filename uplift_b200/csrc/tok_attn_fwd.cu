@@ -42,7 +42,9 @@
 // -inf before the maximum.  P = 0 there, which an infinity or NaN in the same
 // V row would turn into NaN: in the tiles that some row sees only in part the
 // groups look V through, replace such values by zero and add them at the end
-// to the rows that see them.
+// to the rows that see them.  The two query tiles share V, so the tiles to look
+// through are the item's (from the first key that its first row does not see),
+// and the groups of both do so before their own products.
 //
 // D = 128 is bound by the tensor cores: a score product with 64 keys takes 48
 // cycles per 16 channels where 32 would do (128 keys: 64), but tiles of 128
@@ -495,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int first = t * p.row_step;            // first row of this tile
       const int rows = min(kM, it.n - first);      // its rows; may be <= 0
       const int see = p.pk.causal ? max(0, min(it.nk, it.see + first + r)) : it.nk;  // keys this row sees
-      // tiles from edge on hold keys that the tile's first row does not see
-      const int edge = (p.pk.causal ? max(0, min(it.nk, it.see + first)) : it.nk) / kN;
+      // tiles from edge on hold keys that the item's first row does not see
+      const int edge = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN;
       float m = -INFINITY, l = 0.f;  // l: of this group's key tiles, for the maximum m
       // l for a new maximum
       auto adopt = [&](float mn) {
@@ -584,8 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             *v_cleaned = 1;
             __threadfence_block();
             clean_row<T, C::kChunks>(tile, tid & 127);
-            fence_proxy_async();
           }
+          // also for what the other query tile's warps have cleaned
+          fence_proxy_async();
         }
         tmem_wait_st();
         tc_fence_before();
@@ -646,9 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           }
           if (fix && tiles > 0 && part == 0) {
             // add the values taken out of the tiles on the edge of this item
-            const int e0 = (p.pk.causal ? max(0, min(it.nk, it.see)) : it.nk) / kN * kN;
             add_nonfinite<T>(row, lane, static_cast<const T*>(p.v.p) + (int64_t)it.k0 * p.v.t + (it.h / p.group) * p.v.h + 64 * c,
-                             p.v.t, e0, see, 32 * group, min(32 * group + 32, p.D - 64 * c));
+                             p.v.t, edge * kN, see, 32 * group, min(32 * group + 32, p.D - 64 * c));
           }
           fence_proxy_async();
           named_bar(pair, 64);
