@@ -1,0 +1,83 @@
+"""Calls of the token-sequence operators at their edges that need no GPU: what
+tracers and dispatch modes see of them, and refusals."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from uplift_b200 import ops
+
+
+def qkv(T=4, S=4, Hq=2, Hk=1, D=16, dt=torch.float32):
+    return torch.randn(T, Hq, D).to(dt), torch.randn(S, Hk, D).to(dt), torch.randn(S, Hk, D).to(dt)
+
+
+def cu(*n):
+    return torch.tensor(n, dtype=torch.int32)
+
+
+def attention(q, k, v):
+    return ops.packed_attention(q, k, v, cu(0, 4))
+
+
+def rotated(q, k, v):
+    return ops.norm_rotate(q, k, None, None, torch.ones(4, 8), torch.ones(4, 8))
+
+
+CALLS = {"packed_attention": attention, "norm_rotate": rotated}
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("train", [False, True])
+def test_a_traced_call_is_recorded(name, train):
+    """make_fx records the operator (and with gradients its backward), not memory that nobody fills."""
+    def f(*args):
+        args = [t.detach().requires_grad_(train) for t in args]
+        out = CALLS[name](*args)
+        out = out if isinstance(out, tuple) else (out,)
+        return (*out, *torch.autograd.grad([o.sum() for o in out], args[:2])) if train else out
+
+    args = qkv()
+    graph = make_fx(f, tracing_mode="fake")(*args).graph
+    called = [str(n.target) for n in graph.nodes if n.op == "call_function"]
+    assert f"uplift_b200.{name}.default" in called
+    assert (f"uplift_b200.{name}_backward.default" in called) == train
+    assert not any("empty" in n for n in called)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_dispatch_modes_see_the_call(name):
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with FakeTensorMode():
+        args = qkv(dt=torch.bfloat16)
+        with Log():
+            CALLS[name](*args)
+    assert f"uplift_b200.{name}.default" in seen
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tensor_subclasses_are_handed_to_the_operator(name):
+    """Fake tensors outside of their mode: shapes and types, no launch."""
+    mode = FakeTensorMode()
+    args = [mode.from_tensor(t) for t in qkv(dt=torch.float16)]
+    extra = [mode.from_tensor(t) for t in (cu(0, 4), torch.ones(4, 8))]
+    if name == "packed_attention":
+        out = ops.packed_attention(*args, extra[0])
+        assert out.shape == args[0].shape and out.dtype == torch.float16
+    else:
+        a, b = ops.norm_rotate(args[0], args[1], None, None, extra[1], extra[1])
+        assert a.shape == args[0].shape and b.shape == args[1].shape
+
+
+def test_functionalized_calls_are_recorded():
+    def f(q, k, v):
+        return attention(q, k, v) + 1
+    graph = make_fx(torch.func.functionalize(f), tracing_mode="fake")(*qkv()).graph
+    assert any("uplift_b200.packed_attention" in str(n.target) for n in graph.nodes)

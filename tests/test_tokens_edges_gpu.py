@@ -150,3 +150,30 @@ def test_an_infinite_value_of_no_weight_gives_one_result(dt, D, Hq, Hk, key, bad
     assert bool((seen == bad).all()) if bad == math.inf else bool(seen.isnan().all())
     first[key:, :heads, 3] = clean[key:, :heads, 3]
     assert torch.equal(first, clean)
+
+
+# ------------------------------------------------------------------ tracers
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("tracer", ["make_fx", "jit"])
+def test_a_trace_computes_what_the_call_does(dt, tracer):
+    """A recorded call (with its gradients, where the tracer takes them), run on other inputs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    gen = torch.Generator().manual_seed(67)
+    one, two = (qkv(gen, 90, 90, 4, 2, 64, dt) for _ in range(2))
+    g = rand(gen, 90, 4, 64, dt=dt)
+    cu, ang = starts([30, 60]), rand(gen, 90, 32)
+    cos, sin, w = ang.cos(), ang.sin(), 1 + rand(gen, 64, scale=0.2).to(dt)
+
+    def f(q, k, v):
+        a, b = ops.norm_rotate(q, k, w, w, cos, sin)
+        return ops.packed_attention(a, b, v, cu)
+
+    def step(q, k, v):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(f(*leaves), leaves, g)
+
+    if tracer == "make_fx":
+        assert torch.equal(make_fx(f)(*one)(*two), f(*two))
+        assert all(torch.equal(a, b) for a, b in zip(make_fx(step)(*one)(*two), step(*two)))
+    else:
+        assert torch.equal(torch.jit.trace(f, one, check_trace=False)(*two), f(*two))

@@ -14,9 +14,9 @@ neighbours of a pixel) and the fast mode's layer norm (`glue.layernorm_act_`):
 Tensors are [rows, heads, D] on an sm_100 device in float32, bfloat16 or
 float16; views into a fused projection output are read in place.  Both are
 differentiable (gradients are deterministic) and registered as torch custom
-ops, so torch.compile traces them.  Launches go to the current stream of the
-tensors' device; workspaces come from torch's allocator, so calls on several
-streams and in captured graphs share nothing.  As with every differentiable
+ops, so torch.compile and other tracers record them.  Launches go to the
+current stream of the tensors' device; workspaces come from torch's allocator,
+so calls on several streams and in captured graphs share nothing.  As with every differentiable
 call, capture a backward pass into a CUDA graph only when no result of an
 eager call on the same leaves is alive: their gradients would be summed on the
 stream of that call, which is not being captured.
@@ -54,6 +54,23 @@ _HERE = nullcontext()
 def _on(index: int):
     """Context in which `index` (the device of CUDA tensors, so CUDA is initialised) is the current device."""
     return _HERE if _current_device() == index else torch.cuda.device(index)
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_modes, _tracing, _transforms = (torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state,
+                                 torch._C._functorch.maybe_current_level)
+
+
+def _recorded(*tensors) -> bool:
+    """Whether somebody follows the calls of torch's operators -- a compiler or tracer, a dispatch mode, a function
+    transform, a tensor subclass -- and so has to be shown the custom op; else it is left out, since it costs more
+    microseconds than some of the kernels take."""
+    if torch.compiler.is_compiling() or _modes() or _tracing() is not None or _transforms() is not None:
+        return True
+    for t in tensors:
+        if t.__class__ not in _PLAIN:
+            return True
+    return False
 
 
 def _device(what: str, names: str, *tensors) -> int:
@@ -326,7 +343,7 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("norm_rotate: cos and sin are constants and must not require gradients")
     eps, interleaved = float(eps), bool(interleaved)
-    if torch.compiler.is_compiling():
+    if _recorded(q, k):
         return torch.ops.uplift_b200.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
                                     (q_weight is not None and q_weight.requires_grad) or
@@ -519,7 +536,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
         cu_k = cu_q
     scale, causal = (float(scale) if scale is not None else q.shape[-1] ** -0.5), bool(causal)
     train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    if torch.compiler.is_compiling():
+    if _recorded(q, k, v):
         out, lse, _ = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale,
                                                              train or return_lse, train)
         lse = lse.detach()
