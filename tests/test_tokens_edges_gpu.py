@@ -1,5 +1,5 @@
 """The token-sequence operators where masks, types and forms meet: what a
-masked row may not reach in the gradients."""
+masked row may not reach in the gradients, and gradients of any size."""
 import math
 
 import pytest
@@ -177,3 +177,76 @@ def test_a_trace_computes_what_the_call_does(dt, tracer):
         assert all(torch.equal(a, b) for a, b in zip(make_fx(step)(*one)(*two), step(*two)))
     else:
         assert torch.equal(torch.jit.trace(f, one, check_trace=False)(*two), f(*two))
+
+
+# --------------------------------------------------------- gradients in fp16
+def test_large_gradients_in_fp16():
+    """dO of some 10^4: P (dP - delta) exceeds the largest fp16 value (9 10^4), the gradients do not."""
+    gen = torch.Generator().manual_seed(57)
+    n_q, n_k = [4, 3, 5, 2, 130], [2, 3, 8, 1, 4]
+    q, k, v = qkv(gen, sum(n_q), sum(n_k), 4, 2, 64, F16, scale=0.3)
+    v = 2 * v
+    g = rand(gen, *q.shape, scale=8000.0).clamp(-6e4, 6e4).to(F16)
+    g[-130:] *= 2.0 ** -6
+    ref = R.attention(q, k, v, starts(n_q), starts(n_k), None, False, None, g, F16)
+    most = max(ref[n].abs().max().item() for n in ("dq", "dk", "dv"))
+    assert most < 6e4  # all of them are fp16 values
+    _, *grads = attention_and_gradients(q, k, v, g, starts(n_q), starts(n_k), causal=False)
+    for n, d in zip(("dq", "dk", "dv"), grads):
+        R.check(d, ref[n], ref[n + "_tol"], n)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_small_gradients_in_fp16(causal):
+    """dO of some 2^-19 on a thousand keys: score gradients of 10^-9, below the smallest fp16 value, times keys of
+    some hundred.  dS may be off by u of itself and, among the subnormals, by 2^-25 where the largest |dO|
+    is brought to 2^-5 .. 2^-4; P by 2^-33."""
+    gen = torch.Generator().manual_seed(59)
+    n, D, u = 1000, 64, 2.0 ** -11
+    q, k, v = rand(gen, n, 2, D, dt=F16, scale=0.01), rand(gen, n, 2, D, dt=F16, scale=100.0), rand(gen, n, 2, D, dt=F16)
+    g = rand(gen, n, 2, D, scale=2.0 ** -19).to(F16)
+    _, dq, _, dv = attention_and_gradients(q, k, v, g, starts([n]), causal=causal)
+    scale = D ** -0.5
+    seen = torch.ones(n, n, dtype=torch.bool, device=DEV)
+    seen = seen.tril() if causal else seen
+    for h in range(2):
+        qs, ks, vs, gs = (t[:, h].double() for t in (q, k, v, g))
+        p = (qs @ ks.T * scale).masked_fill(~seen, -math.inf).softmax(1)
+        dp = gs @ vs.T
+        ds = p * (dp - (p * dp).sum(1, keepdim=True)) * scale
+        # scores, exponentials and sums in fp32: as in tokens_reference
+        c = 2 * (scale * (D + 4) * 2 * R.F32 * (qs.abs() @ ks.abs().T).max() + 2.0 ** -20) + 2 * n * R.F32
+        size = (gs.abs() @ vs.abs().T + (p @ (gs.abs() @ vs.abs().T).T).diagonal()[:, None]) * p * scale
+        # delta: that of out and what its rounding left, u^2 of it, and of the weights' rounding
+        e = (u + 2 * c) * ds.abs() + (2 * u + c + 2 * (D + 8) * R.F32) * size + 2.0 ** -20 * g.double().abs().max() * scale * seen
+        want = ds @ ks
+        R.check(dq[:, h], want, u * want.abs() + 2.0 ** -25 + (e + 2 * n * R.F32 * ds.abs()) @ ks.abs(), f"dq {h}")
+        want = p.T @ gs
+        tol = ((u + c + 2 * n * R.F32) * p + 2.0 ** -33 * seen).T @ gs.abs()
+        R.check(dv[:, h], want, u * want.abs() + 2.0 ** -25 + tol, f"dv {h}")
+
+
+
+def test_padding_does_not_set_the_size_of_gradients_in_fp16():
+    """Rows of no sequence hold the largest fp16 values; the gradients of the others are as without them."""
+    gen = torch.Generator().manual_seed(60)
+    q, k, v = qkv(gen, 400, 400, 2, 1, 64, F16)
+    g = rand(gen, 400, 2, 64, scale=2.0 ** -18).to(F16)
+    cu = starts([150, 180], 20)
+    _, *clean = attention_and_gradients(q, k, v, g, cu)
+    g[:20], g[350:] = 65504.0, -65504.0
+    _, *grads = attention_and_gradients(q, k, v, g, cu)
+    assert all(torch.equal(a, b) for a, b in zip(grads, clean))
+
+
+def test_many_equal_weights_in_fp16():
+    """200,000 keys of equal weight, 5 10^-6: each key's dv is that times dO, off by the weight's rounding (2^-33 at
+    most, and u), a few steps of fp32 and its own rounding."""
+    gen = torch.Generator().manual_seed(62)
+    n, u = 200_000, 2.0 ** -11
+    q, k, v = rand(gen, 1, 2, 64, dt=F16), torch.zeros(n, 1, 64, dtype=F16, device=DEV), rand(gen, n, 1, 64, dt=F16)
+    g = rand(gen, 1, 2, 64, scale=20000.0).clamp(-6e4, 6e4).to(F16)
+    _, _, _, dv = attention_and_gradients(q, k, v, g, starts([1]), starts([n]))
+    want = g.double().sum(1) / n
+    tol = (g.double().abs() * (u / n + 2.0 ** -33 + 2.0 ** -18 / n)).sum(1) + u * want.abs() + 2.0 ** -25
+    R.check(dv[:, 0], want.expand(n, 64), tol.expand(n, 64), "dv")

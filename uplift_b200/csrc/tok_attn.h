@@ -24,7 +24,7 @@ struct AttnArgs {
   int dtype;
   // backward
   Rows dout, dq, dk, dv;
-  float* delta;  // [Hq][T], then 16 words more
+  float* delta;  // [Hq][T], then 16 words: item counters of the two passes, fp16: the largest |dout|
 };
 
 // bf16 / fp16 attention on the tensor cores (tok_attn_fwd.cu).

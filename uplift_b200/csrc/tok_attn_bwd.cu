@@ -36,6 +36,14 @@
 // so that its CTAs take the SMs as the first pass leaves them; it ends only
 // after the first has.
 //
+// P and dS are rounded to the storage type between the products.  fp16 has few
+// exponents for that: dS of a large dO would overflow where dQ and dK do not,
+// and that of a small one vanish.  So dS is formed of f dO and f delta, with a
+// power of two f that brings the largest |dO| (the kernel that forms delta
+// finds it) into 2^-5 .. 2^9, and is 1 if it is there already, so that ordinary
+// gradients of one row do not depend on those of another.  P for dV is held 2^8
+// times.  The factors are taken out of the fp32 sums.
+//
 // Rows that go by behind the end of their sequence belong to the next one:
 // their P and dS are set to zero and the rows in shared memory too, since an
 // infinity or NaN in them would turn the products into NaN.  The same holds in
@@ -74,6 +82,7 @@ constexpr int kItems = 2;
 constexpr int kAux = 4;   // ring of lse / delta
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kHeld = 8;  // fp16: P for dV is held 2^8 times
 
 template <int DP>
 struct Cfg {
@@ -124,7 +133,17 @@ struct Params {
   uint64_t timeout_ns;
   unsigned int* host_status;
   int* counter;         // items given out, beyond the first of each CTA
+  const unsigned* most; // fp16: the largest |dO|, as bits of a float
 };
+
+// log2 of the factor that dO is taken times.
+template <typename T>
+__device__ __forceinline__ int dout_exponent(const Params& p) {
+  if constexpr (St<T>::kFmt != 0) return 0;
+  const int e = (int)(*p.most >> 23) - 127;
+  return e == -127 ? 0 : min(max(e, -5), 8) - e;  // dO may be zero throughout
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
                                           const WaitLimit& limit) {
@@ -179,6 +198,7 @@ __device__ __noinline__ void put_back(uint8_t* row, int lane, const T* y, int64_
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP>;
+  constexpr bool kScaled = St<T>::kFmt == 0;  // fp16
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((su32(smem) & 1023u) != 0) {  // the swizzled tiles need it, and the declaration asks for it
     if (threadIdx.x == 0) atomicCAS(&g_tok_bwd_status, 0u, 1u);
@@ -436,6 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
   } else if (warp == 18) {
     // ------------------------------------- lse and delta of the columns
     if (KEYS) {
+      constexpr float held = kScaled ? (float)kHeld : 0.f;
+      const float fd = kScaled ? power_of_two(dout_exponent<T>(p) - kHeld) : 1.f;
       bool ok = true;
       uint32_t g = 0;
       for (int n = 0; ok; ++n) {
@@ -463,8 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
                 d = delta[i];
               }
               // negated, in powers of two; rows without keys: P = 0
-              sAux[s * 2 * kN + c + lane] = l == -INFINITY ? -INFINITY : -l * kLog2e;
-              sAux[s * 2 * kN + kN + c + lane] = -d;
+              sAux[s * 2 * kN + c + lane] = l == -INFINITY ? -INFINITY : held - l * kLog2e;
+              sAux[s * 2 * kN + kN + c + lane] = -d * fd;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[s]);
@@ -499,6 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
     const int r = 32 * q + lane;  // row that stays = TMEM lane
     const uint32_t lane_off = (uint32_t)(32 * q) << 16;
     const float c2 = p.scale * kLog2e;
+    const int fexp = dout_exponent<T>(p);
+    const float fdp = kScaled && KEYS ? power_of_two(fexp - kHeld) : 1.f;  // of dP; without KEYS the weights take it
     uint8_t* stage = smem + C::kOffStage + warp * C::kStageBytes;
     uint32_t g = 0, na = 0;
     bool ok = true;
@@ -525,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
         if (r < it.n) {
           const int64_t at = (int64_t)it.h * p.pk.T + it.row + r;
           const float l = p.lse[at];
-          nlse = l == -INFINITY ? -INFINITY : -l * kLog2e;
+          nlse = l == -INFINITY ? -INFINITY : (kScaled ? (float)fexp - l * kLog2e : -l * kLog2e);
           ndelta = -p.delta[at];
         }
       }
@@ -567,8 +591,9 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
             const float2 x0 = __ffma2_rn(make_float2(fs[e], fs[e + 1]), c22, make_float2(nl.x, nl.y));
             const float2 x1 = __ffma2_rn(make_float2(fs[e + 2], fs[e + 3]), c22, make_float2(nl.z, nl.w));
             const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
-            const float2 d0 = __fmul2_rn(p0, __fadd2_rn(make_float2(fd[e], fd[e + 1]), make_float2(nd.x, nd.y)));
-            const float2 d1 = __fmul2_rn(p1, __fadd2_rn(make_float2(fd[e + 2], fd[e + 3]), make_float2(nd.z, nd.w)));
+            auto less = [&](float2 dp, float2 d) { return kScaled && KEYS ? __ffma2_rn(dp, make_float2(fdp, fdp), d) : __fadd2_rn(dp, d); };
+            const float2 d0 = __fmul2_rn(p0, less(make_float2(fd[e], fd[e + 1]), make_float2(nd.x, nd.y)));
+            const float2 d1 = __fmul2_rn(p1, less(make_float2(fd[e + 2], fd[e + 3]), make_float2(nd.z, nd.w)));
             fs[e] = p0.x; fs[e + 1] = p0.y; fs[e + 2] = p1.x; fs[e + 3] = p1.y;
             fd[e] = d0.x; fd[e + 1] = d0.y; fd[e + 2] = d1.x; fd[e + 3] = d1.y;
           }
@@ -616,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
       // else the first halves store a chunk of dQ each
       const CUtensorMap* map = KEYS && w == 1 ? &p.o1 : &p.o0;
       const Rows& out = KEYS && w == 1 ? p.out1 : p.out0;
-      const float f = KEYS && w == 0 ? 1.f : p.scale;
+      const float f = KEYS && w == 0 ? (kScaled ? power_of_two(-kHeld) : 1.f) : (kScaled ? p.scale * power_of_two(-fexp) : p.scale);
       const int c = KEYS ? half : (half == 0 ? w : C::kChunks);
       const int wrows = min(32, it.n - 32 * q);
       if (c < C::kChunks && 64 * c < p.D) {
@@ -714,13 +739,29 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
 // taken as out + out_lo: the rounding of out alone would be the largest error
 // of dS in rows that see few keys.  Bound by HBM: 29 us for the three tensors
 // of 5986 tokens of 32 heads of 128 in bf16 (147 MB, 5.1 TB/s).
-// Also sets the item counters of the passes that follow to zero.
+// Also sets the item counters of the passes that follow to zero, and with
+// fp16 finds the largest |dO| in the rows of the sequences (most, zero before
+// the launch; 16-byte pieces with an infinity or NaN do not count).
 template <typename T>
-__global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo, float* delta, int* counters, int T_, int Hq, int D) {
+__global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo, float* delta, int* counters, unsigned* most, Packing pk,
+                                                    int Hq, int D) {
+  const int T_ = pk.T;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const int64_t item = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
   const int l = threadIdx.x & 7;
+  __shared__ unsigned top;
+  int first = 0, end = 0;  // rows of the sequences
+  unsigned big = 0;        // bits of two |dO|
+  if (St<T>::kFmt == 0) {
+    if (threadIdx.x == 0) top = 0;
+    if (pk.B > 0) {
+      const int2 last = segment(pk.cu_q, pk.B - 1, T_);
+      first = segment(pk.cu_q, 0, T_).x;
+      end = last.x + last.y;
+    }
+    __syncthreads();
+  }
   float sum = 0.f;
   const bool live = item < (int64_t)T_ * Hq;
   const int64_t t = live ? item / Hq : 0;
@@ -736,6 +777,12 @@ __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo
         const float2 x = St<T>::unpack(ua[i]), y = St<T>::unpack(ub[i]);
         sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
       }
+      if (St<T>::kFmt == 0) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, ua[i] & 0x7fff7fffu);
+        if (max(m & 0xffffu, m >> 16) < 0x7c00u) big = __vmaxu2(big, m);
+      }
       if (lo.p != nullptr) {
         const uint4 d = *reinterpret_cast<const uint4*>(static_cast<const T*>(lo.p) + t * lo.t + (int64_t)h * lo.h + c);
         const uint32_t ud[4] = {d.x, d.y, d.z, d.w};
@@ -750,6 +797,14 @@ __global__ void __launch_bounds__(256) delta_kernel(Rows dout, Rows out, Rows lo
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (live && l == 0) delta[(int64_t)h * T_ + t] = sum;
+  if (St<T>::kFmt == 0) {
+    const unsigned bits = t >= first && t < end ? max(big & 0xffffu, big >> 16) : 0;
+    const unsigned of_warp = __reduce_max_sync(0xffffffffu, bits);
+    if ((threadIdx.x & 31) == 0) atomicMax(&top, of_warp);
+    __syncthreads();
+    // (in any order)
+    if (threadIdx.x == 0) atomicMax(most, __float_as_uint(__half2float(__ushort_as_half((unsigned short)top))));
+  }
 }
 
 // early: it may start before the kernel in front of it in the stream has ended.
@@ -800,8 +855,11 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
   int* counters = reinterpret_cast<int*>(a.delta + (int64_t)T * a.Hq);
   const int64_t blocks = std::max<int64_t>(1, ((int64_t)T * a.Hq + 31) / 32);
   if (blocks >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "attention backward: too many rows");
-  if (bf16) delta_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, T, a.Hq, a.D);
-  else delta_kernel<__half><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, T, a.Hq, a.D);
+  unsigned* most = reinterpret_cast<unsigned*>(counters + 2);
+  p.most = most;
+  if (!bf16 && cudaMemsetAsync(most, 0, sizeof(*most), s) != cudaSuccess) return launched("attention backward");
+  if (bf16) delta_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, most, a.pk, a.Hq, a.D);
+  else delta_kernel<__half><<<(int)blocks, 256, 0, s>>>(a.dout, a.out, a.out_lo, a.delta, counters, most, a.pk, a.Hq, a.D);
   if ((rc = launched("attention backward")) != UPLIFT_LA_OK) return rc;
   if (T > 0) {
     // queries stay; without keys no box is loaded and the maps stay empty
