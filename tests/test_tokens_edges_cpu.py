@@ -6,7 +6,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from uplift_b200 import ops
+from uplift_b200 import _native, ops, tokens
 
 
 def qkv(T=4, S=4, Hq=2, Hk=1, D=16, dt=torch.float32):
@@ -81,3 +81,29 @@ def test_functionalized_calls_are_recorded():
         return attention(q, k, v) + 1
     graph = make_fx(torch.func.functionalize(f), tracing_mode="fake")(*qkv()).graph
     assert any("uplift_b200.packed_attention" in str(n.target) for n in graph.nodes)
+
+
+# ----------------------------------------------------------------- refusals
+def test_heads_without_channels_and_single_numbers_are_refused():
+    """Also with the default scale, D ** -0.5."""
+    q, k, v = qkv()
+    for bad in ((q[..., :0], k[..., :0], v[..., :0]), (q.sum(), k, v), (q.sum(), k.sum(), v.sum()), (q, k.sum(), v)):
+        for kw in ({}, {"cu_k": cu(0, 4)}, {"scale": 0.5}):
+            with pytest.raises(ValueError):
+                ops.packed_attention(*bad, cu(0, 4), **kw)
+        with pytest.raises(ValueError):
+            ops.norm_rotate(bad[0], bad[1], None, None, torch.ones(4, 8), torch.ones(4, 8))
+
+
+def test_more_sequences_than_the_kernels_count_are_refused():
+    q, k, v = qkv()
+    many = cu(0).expand(1 << 31)
+    with pytest.raises(ValueError, match="at most"):
+        ops.packed_attention(q, k, v, many)
+    lib = _native.load(build_if_missing=True)
+    rows = [16, 128, 64] * 9
+    for B in ((1 << 31) - 1, (1 << 31) - 65536):
+        args = tokens._PA_ARGS.pack(tokens._PA_ARGS.size, *rows, 16, 16, 16, 16, 0, 16, 1 << 40, 40, 4, B, 2, 1, 64,
+                                    0.125, 1, _native.BF16, 0)
+        assert lib.uplift_tok_attention_forward(args, None) == _native.ERR_SHAPE
+        assert lib.uplift_tok_attention_backward(args, None) == _native.ERR_SHAPE

@@ -19,7 +19,7 @@ int check_sizes(const char* what, const uplift_tok_attention_args* a) {
     return fail(UPLIFT_LA_ERR_ARG, "%s: unknown dtype %d", what, a->dtype);
   // the row limit leaves room for tile arithmetic in 32 bits
   constexpr int64_t kMaxRows = (1ll << 31) - 65536;
-  if (a->B < 0 || a->T < 0 || a->S < 0 || a->T >= kMaxRows || a->S >= kMaxRows || a->Hq < 1 || a->Hk < 1 || a->Hq > 65536)
+  if (a->B < 0 || a->B >= kMaxRows || a->T < 0 || a->S < 0 || a->T >= kMaxRows || a->S >= kMaxRows || a->Hq < 1 || a->Hk < 1 || a->Hq > 65536)
     return fail(UPLIFT_LA_ERR_SHAPE, "%s: bad sizes B=%d T=%lld S=%lld Hq=%d Hk=%d", what, a->B, (long long)a->T,
                 (long long)a->S, a->Hq, a->Hk);
   if (a->Hq % a->Hk != 0)

@@ -353,10 +353,21 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
 
 
 # -------------------------------------------------------- packed_attention
+_MAX_SEQUENCES = (1 << 31) - 65536 - 1  # the kernels count them in 32 bits
+
+
 def _starts(what: str, name: str, t: torch.Tensor, entries: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != entries or entries < (name != "used_k"):
+    if (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != entries or entries < (name != "used_k") or
+            entries > _MAX_SEQUENCES + 1):
         raise ValueError(f"{what}: {name} must be an int32 vector of {entries} entries (sequences" +
-                         (")" if name == "used_k" else " + 1)") + f", got {tuple(t.shape)} {t.dtype}")
+                         (")" if name == "used_k" else " + 1)") + f", at most {_MAX_SEQUENCES} sequences, got {tuple(t.shape)} {t.dtype}")
+
+
+def _scale(q: torch.Tensor, scale: Optional[float]) -> float:
+    if scale is not None:
+        return float(scale)
+    D = q.shape[-1] if q.dim() else 0
+    return D ** -0.5 if D != 0 else 1.0  # (heads without channels are refused)
 
 
 def _attention_args(q, k, v, cu_q, cu_k, used_k, scale):
@@ -388,7 +399,7 @@ def _workspace_bytes(B, T, S, Hq, Hk, D, dtype) -> int:
 def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=None, need_lse=False, need_lo=False):
     """Launch uplift_tok_attention_forward (no autograd): (out, lse [Hq, T] fp32, out_lo: what the rounding of a
     16-bit out left); lse and out_lo are None when not needed."""
-    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    scale = _scale(q, scale)
     index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
     (T, Hq, D), (S, Hk, _) = q.shape, k.shape
     B = cu_q.shape[0] - 1
@@ -416,7 +427,7 @@ def packed_attention_raw(q, k, v, cu_q, cu_k, used_k=None, causal=True, scale=No
 
 def packed_attention_backward_raw(g, q, k, v, out, lse, lo, cu_q, cu_k, used_k=None, causal=True, scale=None):
     """Launch uplift_tok_attention_backward: (dq, dk, dv)."""
-    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    scale = _scale(q, scale)
     index = _attention_args(q, k, v, cu_q, cu_k, used_k, scale)
     return _packed_attention_backward(index, g.to(q.dtype), q, k, v, out, lse, lo, cu_q, cu_k, used_k, causal, scale)
 
@@ -531,10 +542,11 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
     [Hq, T], a constant for autograd.  Differentiable in q, k, v (once).
     """
     if cu_k is None:
-        if q.shape[0] != k.shape[0]:
-            raise ValueError(f"packed_attention: q has {q.shape[0]} rows and k has {k.shape[0]}: pass cu_k")
+        if q.shape[:1] != k.shape[:1]:
+            raise ValueError(f"packed_attention: q is {tuple(q.shape)} and k is {tuple(k.shape)}, not of the same rows: "
+                             f"pass cu_k")
         cu_k = cu_q
-    scale, causal = (float(scale) if scale is not None else q.shape[-1] ** -0.5), bool(causal)
+    scale, causal = _scale(q, scale), bool(causal)
     train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if _recorded(q, k, v):
         out, lse, _ = torch.ops.uplift_b200.packed_attention(q, k, v, cu_q, cu_k, used_k, causal, scale,
