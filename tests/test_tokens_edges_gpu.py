@@ -1,5 +1,6 @@
 """The token-sequence operators where masks, types and forms meet: what a
 masked row may not reach in the gradients, and gradients of any size."""
+import json
 import math
 
 import pytest
@@ -250,3 +251,35 @@ def test_many_equal_weights_in_fp16():
     want = g.double().sum(1) / n
     tol = (g.double().abs() * (u / n + 2.0 ** -33 + 2.0 ** -18 / n)).sum(1) + u * want.abs() + 2.0 ** -25
     R.check(dv[:, 0], want.expand(n, 64), tol.expand(n, 64), "dv")
+
+
+# ------------------------------------------------------- a limit on the CTAs
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_a_limit_on_the_ctas_holds_and_changes_no_result(dt, tmp_path):
+    """uplift_la_set_max_ctas: no more CTAs of these kernels at a time, in prompts, gradients and steps."""
+    gen = torch.Generator().manual_seed(69)
+    q, k, v = qkv(gen, 900, 900, 8, 2, 64, dt)
+    g, cu = rand(gen, 900, 8, 64, dt=dt), starts([500, 300, 100])
+    one, room = starts([1] * 3), starts([300] * 3)
+
+    def run():
+        return (*attention_and_gradients(q, k, v, g, cu), ops.packed_attention(q[:3], k, v, one, room))
+
+    full = run()
+    try:
+        for n in (37, 1):
+            _native.set_max_ctas(n)
+            assert all(torch.equal(a, b) for a, b in zip(full, run()))
+            with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+                run()
+                torch.cuda.synchronize()
+            prof.export_chrome_trace(str(tmp_path / "trace.json"))
+            events = json.loads((tmp_path / "trace.json").read_text())["traceEvents"]
+            ran = [(e["ts"], e["ts"] + e["dur"], e["args"]["grid"], e["name"]) for e in events
+                   if e.get("cat") == "kernel" and any(s in e["name"] for s in ("attention_kernel", "gradient_kernel", "chunk_kernel"))]
+            assert len(ran) == 4, ran
+            assert all(grid[0] * grid[1] * grid[2] <= n for _, _, grid, _ in ran), ran
+            dq, dkv = sorted(e for e in ran if "gradient_kernel" in e[3])
+            assert dkv[0] >= dq[1], ran
+    finally:
+        _native.set_max_ctas(0)

@@ -34,7 +34,9 @@
 // The passes do not need each other.  dQ runs first; when all of its CTAs are
 // running (and delta is there, which they have waited for) the other may start,
 // so that its CTAs take the SMs as the first pass leaves them; it ends only
-// after the first has.
+// after the first has.  Where the number of CTAs is limited, so that other
+// kernels get SMs, it starts after the first has ended: both at once would be
+// twice that many.
 //
 // P and dS are rounded to the storage type between the products.  fp16 has few
 // exponents for that: dS of a large dO would overflow where dQ and dK do not,
@@ -897,7 +899,8 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
     p.counter = counters + 1;
     const int64_t most = ((int64_t)S / kM + a.pk.B) * a.Hk;
     const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
-    rc = bf16 ? launch_d<__nv_bfloat16, true>(p, dev, grid, T > 0, s) : launch_d<__half, true>(p, dev, grid, T > 0, s);
+    const bool early = T > 0 && cta_budget(sms) == sms;
+    rc = bf16 ? launch_d<__nv_bfloat16, true>(p, dev, grid, early, s) : launch_d<__half, true>(p, dev, grid, early, s);
   }
   return rc;
 }

@@ -508,7 +508,9 @@ int chunks_for(int64_t T, int group, int Hk) {
 template <typename T, int DP>
 int run(const Params& p, int sms, cudaStream_t s) {
   const int64_t most = ((int64_t)p.pk.T * p.group / kRows + p.pk.B) * p.chunks * p.Hk;
-  const int grid = (int)std::min<int64_t>(most, (int64_t)sms * kCtasPerSm);
+  // a limit on the CTAs leaves SMs to other kernels, and n CTAs may be spread over n SMs
+  const int budget = cta_budget(sms);
+  const int grid = (int)std::min<int64_t>(most, budget < sms ? budget : sms * kCtasPerSm);
   if (p.D == DP) chunk_kernel<T, DP, true><<<grid, kThreads, 0, s>>>(p);
   else chunk_kernel<T, DP, false><<<grid, kThreads, 0, s>>>(p);
   int rc = launched("attention");
