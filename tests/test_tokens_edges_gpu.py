@@ -1,5 +1,6 @@
 """The token-sequence operators where masks, types and forms meet: what a
-masked row may not reach in the gradients, and gradients of any size."""
+masked row may not reach in the gradients, gradients of any size, and the weight
+gradients of the forms that take several heads at a time."""
 import json
 import math
 
@@ -283,3 +284,59 @@ def test_a_limit_on_the_ctas_holds_and_changes_no_result(dt, tmp_path):
             assert dkv[0] >= dq[1], ran
     finally:
         _native.set_max_ctas(0)
+
+
+# ------------------------------------- weight gradients over all of the rows
+def norm_rotate_sums(x, w, cos, sin, pos, eps, interleaved, g):
+    """z, dx and dw in 64 bits, and the sums of absolute values that their errors are counted from."""
+    x, g, w = x.double(), g.double(), w.double()
+    half = cos.shape[1]
+    a, b = R.pair_index(2 * half, interleaved)
+    there = (pos >= 0)[:, None, None]
+    c = torch.where(there, cos[pos.clamp(min=0).long()].double()[:, None], 1.0)
+    s = torch.where(there, sin[pos.clamp(min=0).long()].double()[:, None], 0.0)
+
+    def turned(y, c, s):
+        z = y.clone()
+        z[..., a], z[..., b] = y[..., a] * c - y[..., b] * s, y[..., b] * c + y[..., a] * s
+        return z
+
+    r = 1.0 / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+    h = x * r
+    gy, ga = turned(g, c, -s), g.abs()
+    ga[..., a], ga[..., b] = (g.abs()[..., i] * c.abs() + g.abs()[..., j] * s.abs() for i, j in ((a, b), (b, a)))
+    gw, gwa = gy * w, ga * w.abs()
+    dx = r * (gw - h * (gw * h).mean(-1, keepdim=True))
+    dxa = r * (gwa + h.abs() * (gwa * h.abs()).mean(-1, keepdim=True))
+    return turned(h * w, c, s), dx, (gy * h).sum((0, 1)), dxa, (ga * h.abs()).sum((0, 1))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dt,wdt,T,Hq,Hk,D,rot", [
+    (BF16, BF16, 3001, 10, 5, 64, 64), (F16, F32, 1203, 13, 6, 128, 64), (F32, F32, 1501, 6, 3, 128, 128),
+    (BF16, F32, 1100, 8, 2, 256, 256), (F32, F32, 2003, 9, 10, 64, 32), (F16, F16, 160, 300, 7, 64, 64),
+    (BF16, BF16, 130, 5, 290, 96, 96), (F32, F32, 700, 9, 5, 256, 128), (BF16, BF16, 1500, 9, 6, 36, 36)])
+def test_weight_gradients_of_many_rows(dt, wdt, T, Hq, Hk, D, rot, interleaved):
+    """Calls large enough for the forms that take several heads per group of lanes (and two that run a warp per row):
+    every dx and the sums over all rows, with weights of their own for queries and keys."""
+    gen = torch.Generator().manual_seed(61)
+    P = 997
+    q, k = rand(gen, T, Hq, D, dt=dt, scale=2.0), rand(gen, T, Hk, D, dt=dt, scale=2.0)
+    gq, gk = rand(gen, T, Hq, D, dt=dt), rand(gen, T, Hk, D, dt=dt)
+    ang = torch.randn(P, rot // 2, generator=gen, dtype=torch.float64) * 10
+    cos, sin = ang.cos().float().to(DEV), ang.sin().float().to(DEV)
+    pos = torch.randint(-1, P, (T,), generator=gen).int().to(DEV)
+    wq, wk = (1 + rand(gen, D, scale=0.3)).to(wdt), (1 + rand(gen, D, scale=0.3)).to(wdt)
+    leaves = [t.requires_grad_() for t in (q, k, wq, wk)]
+    out = ops.norm_rotate(*leaves, cos, sin, pos, 1e-6, interleaved)
+    grads = torch.autograd.grad(out, leaves, (gq, gk))
+    u, tiny = R.u_of(dt), torch.finfo(dt).tiny * R.u_of(dt) + 1e-30
+    f = 2 * (D + 16) * R.F32  # of a term, as in tokens_reference
+    for i, (x, w, g) in enumerate(((q, wq, gq), (k, wk, gk))):
+        z, dx, dw, dxa, dwa = norm_rotate_sums(x.detach(), w.detach(), cos, sin, pos, 1e-6, interleaved, g)
+        # |z| <= |a c| + |b s|: at most sqrt 2 of the pair's length
+        pair = z.abs().amax(-1, keepdim=True)
+        R.check(out[i], z, u * z.abs() + 2 * f * pair + tiny, ("q", "k")[i])
+        R.check(grads[i], dx, u * dx.abs() + f * dxa + tiny, ("dq", "dk")[i])
+        # a lane adds at most 32 rows in 32 bits, a block its groups (64 at most); the blocks are added in 64 bits
+        R.check(grads[2 + i], dw, (f + 2 * (32 + 64) * R.F32) * dwa + R.u_of(wdt) * dw.abs(), ("dwq", "dwk")[i])
