@@ -266,7 +266,8 @@ int uplift_la_device_status(int clear);
 int uplift_la_set_host_status_word(unsigned int* word);
 
 /* Testing only: fault = 1 makes the tensor-core kernels' guide producers issue
- * no loads, so the consumers' bounded waits run out; wait_limit_ns (0 =
+ * no loads (the attention's of uplift_tokens.h: none after a few tiles), so the
+ * consumers' bounded waits run out; wait_limit_ns (0 =
  * default 2 s) caps every mbarrier wait.  fault = 0 restores normal
  * operation.  Used to check that an expired wait is reported through
  * uplift_la_device_status() and leaves the context usable.  No reference

@@ -340,3 +340,34 @@ def test_weight_gradients_of_many_rows(dt, wdt, T, Hq, Hk, D, rot, interleaved):
         R.check(grads[i], dx, u * dx.abs() + f * dxa + tiny, ("dq", "dk")[i])
         # a lane adds at most 32 rows in 32 bits, a block its groups (64 at most); the blocks are added in 64 bits
         R.check(grads[2 + i], dw, (f + 2 * (32 + 64) * R.F32) * dwa + R.u_of(wdt) * dw.abs(), ("dwq", "dwk")[i])
+
+
+# ------------------------------------------------------ waits that run out
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("Hq,Hk", [(4, 2), (3, 3)])
+@pytest.mark.parametrize("part", ["forward", "backward"])
+def test_a_wait_that_runs_out_is_reported_and_the_context_survives(dt, D, Hq, Hk, part):
+    """The producers stop loading after a few tiles, so every role's wait runs out or is ended by another's (20 ms
+    here): the launch records it, drains and ends, the next call raises, and the one after that is right."""
+    lib = _native.load()
+    gen = torch.Generator().manual_seed(71)
+    q, k, v = qkv(gen, 1000, 1000, Hq, Hk, D, dt)
+    g, cu = rand(gen, *q.shape, dt=dt), starts([700, 300])
+    want = attention_and_gradients(q, k, v, g, cu)  # also registers the host's word
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.packed_attention(*leaves, cu)
+    torch.cuda.synchronize()
+    _native.check(lib.uplift_la_test_hook(1, 20_000_000), "test hook")
+    try:
+        if part == "forward":
+            ops.packed_attention(q, k, v, cu)
+        else:
+            torch.autograd.grad(out, leaves, g)
+        torch.cuda.synchronize()
+    finally:
+        lib.uplift_la_test_hook(0, 0)
+    with pytest.raises(_native.ExpiredWaitError):
+        ops.packed_attention(q, k, v, cu)
+    assert _native.device_status(clear=True) == 0  # raising cleared it
+    assert all(torch.equal(a, b) for a, b in zip(attention_and_gradients(q, k, v, g, cu), want))
+    assert _native.host_status.value() == 0

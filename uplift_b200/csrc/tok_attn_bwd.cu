@@ -134,6 +134,7 @@ struct Params {
   float scale;
   uint64_t timeout_ns;
   unsigned int* host_status;
+  int test_fault;       // 1: the producer issues no loads after a few (tests the waits that run out)
   int* counter;         // items given out, beyond the first of each CTA
   const unsigned* most; // fp16: the largest |dO|, as bits of a float
 };
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
               const int s = g % C::kStages;
               ok = mbar_wait(&y_empty[s], ((g / C::kStages) & 1) ^ 1, abort_flag, 1, tmo);
               if (!ok) break;
+              if (p.test_fault == 1 && g >= 3) continue;
               uint8_t* y = sY + s * 2 * C::kYBytes;
               mbar_expect_tx(&y_full[s], 2 * C::kYBytes);
 #pragma unroll
@@ -854,6 +856,7 @@ int attn_tc_backward(const AttnArgs& a, cudaStream_t s) {
   p.scale = a.scale;
   p.timeout_ns = tc_test_timeout_ns() != 0 ? tc_test_timeout_ns() : kTimeoutNs;
   p.host_status = host_status_word();
+  p.test_fault = tc_test_fault();
   int* counters = reinterpret_cast<int*>(a.delta + (int64_t)T * a.Hq);
   const int64_t blocks = std::max<int64_t>(1, ((int64_t)T * a.Hq + 31) / 32);
   if (blocks >= (1ll << 31)) return fail(UPLIFT_LA_ERR_SHAPE, "attention backward: too many rows");

@@ -125,6 +125,7 @@ struct Params {
   float scale;
   uint64_t timeout_ns;
   unsigned int* host_status;
+  int test_fault;  // 1: the producer issues no loads after a few (tests the waits that run out)
 };
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned where,
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               const int s = g % C::kSlots;
               ok = ok && mbar_wait(&kv_empty[s], ((g / C::kSlots) & 1) ^ 1, abort_flag, 1, tmo);
               ++g;
-              if (!ok) return;
+              if (!ok || (p.test_fault == 1 && g > 4)) return;  // (K_0, K_1, V_0, K_2: the first decisions and products)
               mbar_expect_tx(&kv_full[s], C::kSlotBytes);
 #pragma unroll
               for (int c = 0; c < C::kChunks; ++c)
@@ -764,6 +765,7 @@ int attn_tc_forward(const AttnArgs& a, cudaStream_t s) {
   p.scale = a.scale;
   p.timeout_ns = tc_test_timeout_ns() != 0 ? tc_test_timeout_ns() : kTimeoutNs;
   p.host_status = host_status_word();
+  p.test_fault = tc_test_fault();
   const int64_t most = ((int64_t)a.pk.T / (kM + p.row_step) + a.pk.B) * (a.Hq / p.heads);  // items, at most
   const int grid = (int)std::min<int64_t>(std::max<int64_t>(most, 1), cta_budget(sms));
   return a.dtype == UPLIFT_LA_BF16 ? launch<__nv_bfloat16>(p, dev, grid, s) : launch<__half>(p, dev, grid, s);
