@@ -371,3 +371,47 @@ def test_a_wait_that_runs_out_is_reported_and_the_context_survives(dt, D, Hq, Hk
     assert _native.device_status(clear=True) == 0  # raising cleared it
     assert all(torch.equal(a, b) for a, b in zip(attention_and_gradients(q, k, v, g, cu), want))
     assert _native.host_status.value() == 0
+
+
+# ------------------------------------------- prompts among single tokens
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("Hq,Hk", [(8, 2), (3, 3), (10, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_prompt_among_single_tokens(dt, D, Hq, Hk, causal):
+    """Few queries per sequence on average, many in one: the eight-row form walks a prompt, with gradients."""
+    gen = torch.Generator().manual_seed(73)
+    n_q = [1] * 30 + [300] + [1, 0, 2] * 10
+    n_k = [1 + 17 * i % 400 for i in range(30)] + [450] + [3, 5, 700] * 10
+    q, k, v = qkv(gen, sum(n_q), sum(n_k), Hq, Hk, D, dt)
+    assert sum(n_q) <= 8 * len(n_q)
+    g = rand(gen, *q.shape, dt=dt)
+    ref = R.attention(q, k, v, starts(n_q), starts(n_k), None, causal, None, g, dt)
+    got = attention_and_gradients(q, k, v, g, starts(n_q), starts(n_k), causal=causal)
+    for n, x in zip(("out", "dq", "dk", "dv"), got):
+        R.check(x, ref[n], ref[n + "_tol"], n)
+
+
+# ------------------------------------------------ offsets beyond 32 bits
+def test_prompts_and_gradients_beyond_32_bit_offsets():
+    """Queries and keys whose element offsets are above 2^31: results and gradients of the rows alone."""
+    T, D = 2_200_000, 128
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    gen = torch.Generator().manual_seed(75)
+    lens, n = [130, 170], 300
+    small = [rand(gen, n, 8, D, dt=BF16) for _ in range(4)]
+    want = attention_and_gradients(*small, starts(lens))
+    large = []
+    for t in small:
+        x = torch.zeros(T, 8, D, dtype=BF16, device=DEV)
+        x[-n:] = t
+        large.append(x)
+    got = attention_and_gradients(*large, starts(lens, T - n))
+    for a, b in zip(got, want):
+        assert torch.equal(a[-n:], b)
+        assert not a[:T - n].any()
+    cos, sin = (rand(gen, T, 64) for _ in range(2))
+    a, _ = ops.norm_rotate(large[0], large[1][:, :1], None, None, cos, sin)
+    b, _ = ops.norm_rotate(small[0], small[1][:, :1], None, None, cos[-n:], sin[-n:])
+    assert torch.equal(a[-n:], b)
+    assert not a[:T - n].any()
