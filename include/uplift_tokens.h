@@ -15,7 +15,8 @@
  * storage type.  The entry points allocate nothing, never synchronise, are
  * deterministic (no floating-point atomics) and can be captured into CUDA
  * graphs; each returns UPLIFT_LA_OK or an error code (message in
- * uplift_la_last_error()).  A tensor-core launch whose bounded wait ran out is
+ * uplift_la_last_error()).  uplift_la_set_max_ctas() holds for the attention's
+ * tensor-core launches.  A tensor-core launch whose bounded wait ran out is
  * reported by uplift_la_device_status() and the registered host status word.
  */
 #ifndef UPLIFT_TOKENS_H_
@@ -90,6 +91,10 @@ int64_t uplift_tok_norm_rotate_partial_floats(int D);
  * no sequence.  What keys that a query does not see hold (NaN, infinities)
  * does not reach its output or its gradient, nor does what that query and its
  * dout hold reach the gradients of these keys.
+ *
+ * fp16 gradients: the weights' gradients are rounded to fp16 as those of dout
+ * times a power of two, which is 1 while the largest |dout| lies between 2^-5 and
+ * 2^9 and brings it there otherwise.
  *
  * bf16 / fp16: D a multiple of 8; tensors 16-byte aligned, strides
  * multiples of 8 elements and row strides multiples of the head stride

@@ -56,10 +56,11 @@
 //
 // Bound by the chain of a step: scores and dP (tensor cores), P and dS (the
 // warps), products with them (tensor cores), with two steps in flight, which
-// TMEM allows.  Six documents of 300 to 2500 tokens, 32 heads on 8 of 128,
-// bf16, causal: dQ 157 us (720 TFLOP/s), dK and dV 186 us (810), 0.44 and 0.49 of a
-// large library product.  16 images of 1025, 6 heads of 64, fp16: 66 and 88 us (a
-// step of training 245 us; with one thread per row 266).
+// for which TMEM has room (a step takes 128 columns, the sums 64 to 256; a third
+// step, which would fit in all but one variant, is not built).  Six documents of
+// 300 to 2500 tokens, 32 heads on 8 of 128, bf16, causal: dQ 165 us (690 TFLOP/s),
+// dK and dV 196 us (770), 0.42 and 0.47 of a large library product.  16 images of
+// 1025, 6 heads of 64, fp16: 73 and 97 us (a step of training 245 us).
 
 #include <math.h>
 #include <string.h>
@@ -742,7 +743,8 @@ __global__ void __launch_bounds__(kThreads, 1) gradient_kernel(const __grid_cons
 // delta = rowsum(dO O): eight lanes per row, 16 bytes each at a time.  O is
 // taken as out + out_lo: the rounding of out alone would be the largest error
 // of dS in rows that see few keys.  Bound by HBM: 29 us for the three tensors
-// of 5986 tokens of 32 heads of 128 in bf16 (147 MB, 5.1 TB/s).
+// of 5986 tokens of 32 heads of 128 in bf16 (147 MB, 5.1 TB/s); in fp16 the search
+// for the largest |dO| takes 3 of 12 us for 16400 tokens of 6 heads of 64.
 // Also sets the item counters of the passes that follow to zero, and with
 // fp16 finds the largest |dO| in the rows of the sequences (most, zero before
 // the launch; 16-byte pieces with an infinity or NaN do not count).

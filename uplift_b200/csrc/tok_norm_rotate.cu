@@ -17,8 +17,9 @@
 // Bound by HBM.  12347 tokens of 32 + 8 heads of 128, bf16: 51 us, 5.1 TB/s (0.78
 // of a copy); 42640 of 6 + 6 heads of 64, fp32: 47 us, 5.5 TB/s (0.85); the
 // gradients of 8192 tokens of 32 + 8 heads of 128, bf16: 57 + 4 us, 4.4 TB/s (0.68).
-// Shapes that the lanes cannot take (an odd D or R, odd addresses) run at a
-// warp per row: 8192 tokens of 32 + 8 heads of 36, bf16: 131 and 365 us.
+// Shapes that the lanes cannot take (D or R no multiple of 16 bytes, odd
+// addresses, more than 32 lanes to a row: fp32 heads above 128) run at a warp per
+// row: 8192 tokens of 32 + 8 heads of 36, bf16: 131 and 365 us.
 
 #include <cuda_runtime.h>
 #include <math.h>
@@ -565,7 +566,8 @@ int run(Args a, int dtype, bool inter, bool bwd, int* partial_rows, cudaStream_t
   // keep more loads in flight; one where several would leave SMs without work.
   // 32 + 8 heads of 128 in bf16, forward and backward, several / one (us): 128
   // tokens 3.2 / 2.5 and 3.7 / 4.1, 512: 4.8 / 4.9 and 6.7 / 7.2, 1024: 6.3 / 8.1
-  // and 9.1 / 11.4, 8192: 28 / 50 and 54 / 89.
+  // and 9.1 / 11.4, 8192: 28 / 50 and 54 / 89.  One threshold serves both, though
+  // the backward would gain its 0.4 us below it too.
   const int hpg = vec && rows * lanes >= 148ll * 2048 ? (bwd ? kManyHeadsBwd : kManyHeads) : 1;
   for (int i = 0; i < 2; ++i) a.side[i].chunks = (a.side[i].heads + hpg - 1) / hpg;
   if (bwd) {

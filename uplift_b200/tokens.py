@@ -538,6 +538,12 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
     defaults to D ** -0.5.  Queries that see no key, and rows of no sequence,
     get zeros (lse -inf) and gradients zero.
 
+    One form of the kernels serves the whole call, by its average tokens per
+    sequence: prompts and single tokens are faster in calls of their own.
+    Tensors are read in place, but for 16-bit ones whose rows are not 16-byte
+    aligned or whose row stride is not a multiple of the head stride (a cache
+    laid out [Hk, S, D]): these are copied on every call.
+
     With return_lse also returns log(sum_j exp(scale q_i . k_j)), fp32
     [Hq, T], a constant for autograd.  Differentiable in q, k, v (once).
     """
