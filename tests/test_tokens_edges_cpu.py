@@ -107,3 +107,19 @@ def test_more_sequences_than_the_kernels_count_are_refused():
                                     0.125, 1, _native.BF16, 0)
         assert lib.uplift_tok_attention_forward(args, None) == _native.ERR_SHAPE
         assert lib.uplift_tok_attention_backward(args, None) == _native.ERR_SHAPE
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(name, which):
+    """Tangents would be left out of the result without an error."""
+    from torch.autograd import forward_ad
+    with FakeTensorMode(), forward_ad.dual_level():
+        args = list(qkv())
+        CALLS[name](*args)  # no tangents: as ever
+        args[which] = forward_ad.make_dual(args[which], torch.randn(args[which].shape))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            CALLS[name](*args)
+    args = qkv()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda *a: CALLS[name](*a), args, tuple(torch.ones_like(a) for a in args))

@@ -415,3 +415,25 @@ def test_prompts_and_gradients_beyond_32_bit_offsets():
     b, _ = ops.norm_rotate(small[0], small[1][:, :1], None, None, cos[-n:], sin[-n:])
     assert torch.equal(a[-n:], b)
     assert not a[:T - n].any()
+
+
+# -------------------------------------------------- captured fp16 gradients
+def test_a_captured_fp16_step_takes_gradients_of_any_size():
+    """A training step in a CUDA graph: the largest dO is found anew in each replay."""
+    gen = torch.Generator().manual_seed(77)
+    q, k, v = qkv(gen, 400, 400, 4, 2, 64, F16)
+    g, cu = rand(gen, 400, 4, 64, dt=F16), starts([150, 250])
+    static = g.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention_and_gradients(q, k, v, static, cu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = attention_and_gradients(q, k, v, static, cu)
+    for factor in (1.0, 2.0 ** 12, 2.0 ** -14, 0.0, 1.0):
+        static.copy_(g * factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, attention_and_gradients(q, k, v, g * factor, cu)))

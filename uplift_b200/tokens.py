@@ -30,6 +30,7 @@ from contextlib import nullcontext
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -71,6 +72,13 @@ def _recorded(*tensors) -> bool:
         if t.__class__ not in _PLAIN:
             return True
     return False
+
+
+def _refuse_tangents(what: str, *tensors) -> None:
+    """Raises in forward-mode differentiation, which torch would leave out without a word."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative (it is differentiable by backward)")
 
 
 def _device(what: str, names: str, *tensors) -> int:
@@ -342,6 +350,8 @@ def norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, in
     """
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("norm_rotate: cos and sin are constants and must not require gradients")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("norm_rotate", q, k, q_weight, k_weight, cos, sin)
     eps, interleaved = float(eps), bool(interleaved)
     if _recorded(q, k):
         return torch.ops.uplift_b200.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
@@ -552,6 +562,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, used_k=None, causal=True, scale=N
             raise ValueError(f"packed_attention: q is {tuple(q.shape)} and k is {tuple(k.shape)}, not of the same rows: "
                              f"pass cu_k")
         cu_k = cu_q
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("packed_attention", q, k, v)
     scale, causal = _scale(q, scale), bool(causal)
     train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if _recorded(q, k, v):
