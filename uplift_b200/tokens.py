@@ -16,10 +16,10 @@ float16; views into a fused projection output are read in place.  Both are
 differentiable (gradients are deterministic) and registered as torch custom
 ops, so torch.compile and other tracers record them.  Launches go to the
 current stream of the tensors' device; workspaces come from torch's allocator,
-so calls on several streams and in captured graphs share nothing.  As with every differentiable
-call, capture a backward pass into a CUDA graph only when no result of an
-eager call on the same leaves is alive: their gradients would be summed on the
-stream of that call, which is not being captured.
+so calls on several streams and in captured graphs share nothing.  As with
+every differentiable call, capture a backward pass into a CUDA graph only when
+no result of an eager call on the same leaves is alive: their gradients would be
+summed on the stream of that call, which is not being captured.
 """
 from __future__ import annotations
 
@@ -370,7 +370,8 @@ def _starts(what: str, name: str, t: torch.Tensor, entries: int) -> None:
     if (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != entries or entries < (name != "used_k") or
             entries > _MAX_SEQUENCES + 1):
         raise ValueError(f"{what}: {name} must be an int32 vector of {entries} entries (sequences" +
-                         (")" if name == "used_k" else " + 1)") + f", at most {_MAX_SEQUENCES} sequences, got {tuple(t.shape)} {t.dtype}")
+                         (")" if name == "used_k" else " + 1)") + f", at most {_MAX_SEQUENCES} sequences, "
+                         f"got {tuple(t.shape)} {t.dtype}")
 
 
 def _scale(q: torch.Tensor, scale: Optional[float]) -> float:
